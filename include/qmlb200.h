@@ -371,6 +371,54 @@ size_t qmlb_packed_upper_elements(int F);
 int qmlb_pack_upper(const double *ZTZ, int F, double *packed, qmlb_stream_t stream);
 int qmlb_unpack_upper(const double *packed, int F, double *ZTZ, qmlb_stream_t stream);
 
+/* ---- rows that belong to groups: order by key, table lookup, matrix products -------------------- */
+
+/* Operators for learned per-element (or per-species, per-token) parameters beside the fixed projection matrices above.
+ * They have no counterpart in the upstream project, which gathers the rows of one element at a time with boolean masks
+ * (models/hadamard_features.py:99-111).  Element types: */
+#define QMLB_F32 0
+#define QMLB_F16 1
+#define QMLB_BF16 2
+
+/* Stable order of n integer keys (int32 for key_bits = 32, int64 for 64).
+ *   order i32[n]              positions of the keys by ascending key, equal keys in their original order; keys outside
+ *                             [0, nkeys) (-1 for a padded slot) follow behind all groups, in their original order
+ *   group_start i32[nkeys+1]  first position of every key; group_start[nkeys] = number of keys inside [0, nkeys)
+ * n < 2^31, 0 < nkeys < 2^31 - 1.  scratch: qmlb_group_by_key_scratch_bytes bytes of device memory, 4-byte aligned. */
+size_t qmlb_group_by_key_scratch_bytes(size_t n, int nkeys);
+int qmlb_group_by_key(const void *keys, int key_bits, size_t n, int nkeys, int *order, int *group_start, void *scratch,
+                      size_t scratch_bytes, qmlb_stream_t stream);
+
+/* out[i, :] = scale * table[index[i], :], a zero row where index[i] is outside [0, rows).  table [rows, width] and out
+ * [n, width] have the element type `dtype`; the product is formed in 32 bits and rounded once. */
+int qmlb_embedding(const void *index, int index_bits, const void *table, int dtype, size_t n, int64_t rows, int width, float scale,
+                   void *out, qmlb_stream_t stream);
+
+/* Gradient of the table: dtable[v, :] = scale * sum of dout[i, :] over the i with index[i] = v; rows that no index names
+ * become zero (dtable is fully overwritten).  order and group_start are what qmlb_group_by_key(index, ..., rows) wrote.
+ * Sums are 32-bit, in an order that depends on the sizes alone.  scratch: qmlb_embedding_grad_scratch_bytes bytes of
+ * device memory, 16-byte aligned. */
+size_t qmlb_embedding_grad_scratch_bytes(size_t n, int rows, int width);
+int qmlb_embedding_grad(const void *dout, int dtype, const void *index, int index_bits, const int *order, const int *group_start,
+                        size_t n, int rows, int width, float scale, void *dtable, void *scratch, size_t scratch_bytes,
+                        qmlb_stream_t stream);
+
+/* One matrix per group of rows.  W [ngroups, K, N]; the rows of group g are group_start[g] <= r < group_start[g+1]
+ * (i32[ngroups+1], ascending; groups may be empty and of any size).
+ *   transpose = 0: out [n, N], out[r] = x[r] . W[g]       x [n, K]
+ *   transpose = 1: out [n, K], out[r] = x[r] . W[g]^T     x [n, N]   (gradient of the rows)
+ * Rows in front of the first group or behind the last become zero rows.  32-bit sums, one rounding to `dtype`.
+ * ngroups <= 1024.  workspace: qmlb_grouped_matmul_workspace_bytes bytes of device memory, 256-byte aligned. */
+size_t qmlb_grouped_matmul_workspace_bytes(size_t n, int ngroups, int K, int N, int dtype, int transpose);
+int qmlb_grouped_matmul(const void *x, const void *W, const int *group_start, int dtype, size_t n, int ngroups, int K, int N,
+                        int transpose, void *out, void *workspace, size_t workspace_bytes, qmlb_stream_t stream);
+
+/* Gradient of the matrices: dW[g] = sum over the rows r of group g of x[r]^T dy[r] ([ngroups, K, N], zero for an empty
+ * group).  32-bit sums in an order that depends on the sizes and group bounds alone, one rounding to `dtype`. */
+size_t qmlb_grouped_matmul_wgrad_workspace_bytes(size_t n, int ngroups, int K, int N, int dtype);
+int qmlb_grouped_matmul_wgrad(const void *x, const void *dy, const int *group_start, int dtype, size_t n, int ngroups, int K, int N,
+                              void *dW, void *workspace, size_t workspace_bytes, qmlb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

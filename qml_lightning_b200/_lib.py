@@ -10,6 +10,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('QMLB200_LIB', os.path.join(HERE, 'lib', 'libqmlb200.so'))
 
 c_int, c_float, c_size_t, c_void_p = ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_void_p
+c_int64 = ctypes.c_int64
 
 
 class FchlParamsC(ctypes.Structure):
@@ -85,6 +86,18 @@ SIGNATURES = {
     'qmlb_packed_upper_elements': (c_size_t, [c_int]),
     'qmlb_pack_upper': (c_int, [c_void_p, c_int, c_void_p, c_void_p]),
     'qmlb_unpack_upper': (c_int, [c_void_p, c_int, c_void_p, c_void_p]),
+    'qmlb_group_by_key_scratch_bytes': (c_size_t, [c_size_t, c_int]),
+    'qmlb_group_by_key': (c_int, [c_void_p, c_int, c_size_t, c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    'qmlb_embedding': (c_int, [c_void_p, c_int, c_void_p, c_int, c_size_t, c_int64, c_int, c_float, c_void_p, c_void_p]),
+    'qmlb_embedding_grad_scratch_bytes': (c_size_t, [c_size_t, c_int, c_int]),
+    'qmlb_embedding_grad': (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_size_t, c_int, c_int, c_float, c_void_p,
+                                    c_void_p, c_size_t, c_void_p]),
+    'qmlb_grouped_matmul_workspace_bytes': (c_size_t, [c_size_t, c_int, c_int, c_int, c_int, c_int]),
+    'qmlb_grouped_matmul': (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_size_t, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
+                                    c_size_t, c_void_p]),
+    'qmlb_grouped_matmul_wgrad_workspace_bytes': (c_size_t, [c_size_t, c_int, c_int, c_int, c_int]),
+    'qmlb_grouped_matmul_wgrad': (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_size_t, c_int, c_int, c_int, c_void_p, c_void_p,
+                                          c_size_t, c_void_p]),
 }
 
 _lib = None

@@ -617,6 +617,138 @@ def rff_train_features(x, dx, W, b, grouping, atom_counts, nb, A):
     return Z, G
 
 
+# ---- rows that belong to groups: order by key, table lookup, one matrix per group -----------------------------------
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}     # QMLB_F32, QMLB_F16, QMLB_BF16
+
+
+def _dtype(t, name):
+    if t.dtype not in _DTYPES:
+        raise RuntimeError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
+    return _DTYPES[t.dtype]
+
+
+def _index_bits(t, name):
+    if t.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError(f"{name} must be int32 or int64, got {t.dtype}")
+    return 32 if t.dtype == torch.int32 else 64
+
+
+def _together(first, **others):
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise RuntimeError(f"{name} must be on {first.device}, got {t.device}")
+
+
+def _output(out, shape, dtype, device, name='out'):
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != device:
+        raise RuntimeError(f"{name} must be {dtype} {tuple(shape)} on {device}, got {out.dtype} {tuple(out.shape)} on {out.device}")
+    return out
+
+
+def group_by_key(keys, nkeys):
+    """Stable order of integer keys (``qmlb_group_by_key``): ``(order i32[n], group_start i32[nkeys + 1])``; keys outside
+    ``[0, nkeys)`` (the -1 of a padded slot) follow behind all groups.  ``keys`` may have any shape and counts flat."""
+    nkeys = int(nkeys)
+    bits = _index_bits(keys, 'keys')
+    if not 0 < nkeys < 2 ** 31 - 1:
+        raise RuntimeError(f"group_by_key: nkeys must be between 1 and 2^31 - 2, got {nkeys}")
+    p = _p(keys, None, 'keys')
+    n, dev = keys.numel(), keys.device
+    order = torch.empty(n, dtype=torch.int32, device=dev)
+    start = torch.empty(nkeys + 1, dtype=torch.int32, device=dev)
+    lib = _lib.load()
+    nbytes = lib.qmlb_group_by_key_scratch_bytes(n, nkeys)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    check(lib.qmlb_group_by_key(p, bits, n, nkeys, _p(order), _p(start), _p(scratch), nbytes, _stream(dev)), 'qmlb_group_by_key')
+    return order, start
+
+
+def embedding(indices, table, scale=1.0, out=None):
+    """``scale * table[indices]`` (``qmlb_embedding``); a zero row for an index outside the table."""
+    bits, dtype = _index_bits(indices, 'indices'), _dtype(table, 'table')
+    if table.dim() != 2:
+        raise RuntimeError("table must be [rows, width]")
+    pi, pt = _p(indices, None, 'indices'), _p(table, None, 'table')
+    _together(table, indices=indices)
+    out = _output(out, tuple(indices.shape) + (table.shape[1],), table.dtype, table.device)
+    if out.numel():
+        check(_lib.load().qmlb_embedding(pi, bits, pt, dtype, indices.numel(), table.shape[0], table.shape[1], float(scale),
+                                         _p(out, None, 'out'), _stream(table.device)), 'qmlb_embedding')
+    return out
+
+
+def embedding_grad(grad, indices, order, group_start, scale=1.0, out=None):
+    """Gradient of the table of :func:`embedding` (``qmlb_embedding_grad``): ``[rows, width]`` in the type of ``grad``, with
+    ``order, group_start = group_by_key(indices, rows)``."""
+    bits, dtype = _index_bits(indices, 'indices'), _dtype(grad, 'grad')
+    if tuple(grad.shape[:-1]) != tuple(indices.shape) or grad.dim() != indices.dim() + 1:
+        raise RuntimeError("grad must have the shape of indices and one dimension more")
+    rows, width, n = group_start.numel() - 1, grad.shape[-1], indices.numel()
+    if order.numel() != n or rows < 0:
+        raise RuntimeError("order and group_start must come from group_by_key(indices, rows)")
+    pg, pi = _p(grad, None, 'grad'), _p(indices, None, 'indices')
+    po, ps = _p(order, torch.int32, 'order'), _p(group_start, torch.int32, 'group_start')
+    _together(grad, indices=indices, order=order, group_start=group_start)
+    out = _output(out, (rows, width), grad.dtype, grad.device)
+    if out.numel():
+        lib = _lib.load()
+        nbytes = lib.qmlb_embedding_grad_scratch_bytes(n, rows, width)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=grad.device)
+        check(lib.qmlb_embedding_grad(pg, dtype, pi, bits, po, ps, n, rows, width, float(scale), _p(out, None, 'out'), _p(scratch), nbytes,
+                                      _stream(grad.device)), 'qmlb_embedding_grad')
+    return out
+
+
+def grouped_matmul(x, W, group_start, transpose=False, out=None):
+    """One matrix per group of rows (``qmlb_grouped_matmul``): ``out[r] = x[r] @ W[g]`` (``W[g].T`` with ``transpose``) for
+    ``group_start[g] <= r < group_start[g + 1]``; zero rows outside the groups.  W ``[groups, K, N]``."""
+    dtype = _dtype(W, 'W')
+    if W.dim() != 3 or x.dim() != 2:
+        raise RuntimeError("W must be [groups, K, N] and x [rows, columns]")
+    G, K, N = W.shape
+    n, transpose = x.shape[0], bool(transpose)
+    if x.shape[1] != (N if transpose else K):
+        raise RuntimeError(f"x has {x.shape[1]} columns, W needs {N if transpose else K}")
+    if group_start.numel() != G + 1:
+        raise RuntimeError("group_start must have one entry per group and one more")
+    px, pw, ps = _p(x, W.dtype, 'x'), _p(W, None, 'W'), _p(group_start, torch.int32, 'group_start')
+    _together(W, x=x, group_start=group_start)
+    out = _output(out, (n, K if transpose else N), W.dtype, W.device)
+    if out.numel() == 0:
+        return out
+    if x.shape[1] == 0:
+        return out.zero_()
+    lib = _lib.load()
+    nbytes = lib.qmlb_grouped_matmul_workspace_bytes(n, G, K, N, dtype, int(transpose))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=W.device)
+    check(lib.qmlb_grouped_matmul(px, pw, ps, dtype, n, G, K, N, int(transpose), _p(out, None, 'out'), _p(ws), nbytes, _stream(W.device)),
+          'qmlb_grouped_matmul')
+    return out
+
+
+def grouped_matmul_wgrad(x, dy, group_start, out=None):
+    """Gradient of the matrices of :func:`grouped_matmul` (``qmlb_grouped_matmul_wgrad``): ``out[g] = x_g.T @ dy_g``."""
+    dtype = _dtype(x, 'x')
+    if x.dim() != 2 or dy.dim() != 2 or x.shape[0] != dy.shape[0]:
+        raise RuntimeError("x must be [rows, K] and dy [rows, N]")
+    G, n, K, N = group_start.numel() - 1, x.shape[0], x.shape[1], dy.shape[1]
+    if G < 1:
+        raise RuntimeError("group_start must have one entry per group and one more")
+    px, pd, ps = _p(x, None, 'x'), _p(dy, x.dtype, 'dy'), _p(group_start, torch.int32, 'group_start')
+    _together(x, dy=dy, group_start=group_start)
+    out = _output(out, (G, K, N), x.dtype, x.device)
+    if out.numel() == 0:
+        return out
+    lib = _lib.load()
+    nbytes = lib.qmlb_grouped_matmul_wgrad_workspace_bytes(n, G, K, N, dtype)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    check(lib.qmlb_grouped_matmul_wgrad(px, pd, ps, dtype, n, G, K, N, _p(out, None, 'out'), _p(ws), nbytes, _stream(x.device)),
+          'qmlb_grouped_matmul_wgrad')
+    return out
+
+
 def _on_tensor_device(fn):
     """Run ``fn`` with the device of its first CUDA tensor argument current: kernel launches, per-device caches
     inside the library (cuBLAS handle, built-in scratch address) and ``cudaFuncSetAttribute`` all act on the current

@@ -1,0 +1,281 @@
+// Stable order of integer keys: order[] lists the positions of the keys by ascending key, equal keys in their original
+// order, and group_start[v] = number of valid keys below v.  Keys outside [0, nkeys) (the -1 of a padded slot) count as
+// the key nkeys: they come behind all groups, in their original order.
+//
+// Least-significant-digit radix sort with digits of at most RADIX_BITS bits, so up to 1,023 keys (every element or
+// species numbering) take ONE pass and 1,048,575 take two.  A pass over blocks of TILE keys:
+//   1. histogram : counts[digit][block]
+//   2. scan      : one block per digit turns its row into an exclusive prefix over the blocks and writes the digit's total
+//   3. scatter   : every block ranks its keys again (the same order, so the result never depends on scheduling) and
+//                  writes position and key to base(digit) + counts[digit][block] + rank
+// Rank inside a block: each warp owns a contiguous run of its keys; the lanes that hold the same digit find one another
+// with one ballot per digit bit, and the warp's running count per digit stays in shared memory.  What bounds a pass is
+// latency and the scattered writes, not arithmetic: 8 + 8 bytes per key and pass.
+// With one pass the digit totals are the group sizes; with more, group_start comes from a binary search per key in the
+// sorted keys.
+#include "typed.cuh"
+
+namespace {
+
+constexpr int RADIX_BITS = 10;                 // widest digit
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int ITEMS = 16;                      // keys per thread
+constexpr int TILE = THREADS * ITEMS;          // keys per block
+constexpr int WARP_TILE = 32 * ITEMS;
+
+__host__ __device__ inline int bits_for(unsigned nkeys) {   // digits of the values 0 .. nkeys (nkeys = "outside")
+    int b = 1;
+    while (b < 32 && (nkeys >> b)) ++b;
+    return b;
+}
+
+template <typename K>
+__device__ __forceinline__ uint32_t clamp_key(K k, uint32_t nkeys) {
+    return (k >= 0 && (unsigned long long)k < (unsigned long long)nkeys) ? (uint32_t)k : nkeys;
+}
+
+// lanes whose value agrees with mine in the lowest `nbits` bits (all lanes of the warp take part; lanes with
+// `in` = false match nobody that has it true)
+__device__ __forceinline__ unsigned same_digit(uint32_t d, int nbits, bool in) {
+    unsigned m = __ballot_sync(QMLB_FULL_MASK, in);
+    if (!in) m = ~m;
+    for (int b = 0; b < nbits; ++b) {
+        const unsigned v = __ballot_sync(QMLB_FULL_MASK, (d >> b) & 1u);
+        m &= ((d >> b) & 1u) ? v : ~v;
+    }
+    return m;
+}
+
+// FIRST: keys come from the caller's tensor; else from the pairs of the previous pass
+template <typename K, bool FIRST>
+__global__ void __launch_bounds__(THREADS)
+histogram_kernel(const K *__restrict__ keys, const uint32_t *__restrict__ pair_keys, uint32_t n, uint32_t nkeys, int shift, int nbits,
+                 uint32_t *__restrict__ counts) {
+    extern __shared__ uint32_t hist[];
+    const int nd = 1 << nbits;
+    for (int d = threadIdx.x; d < nd; d += THREADS) hist[d] = 0;
+    __syncthreads();
+    const uint32_t base = blockIdx.x * (uint32_t)TILE;
+#pragma unroll 4
+    for (int i = 0; i < ITEMS; ++i) {
+        const uint32_t at = base + i * THREADS + threadIdx.x;
+        const bool in = at < n;
+        uint32_t d = 0;
+        if (in) d = ((FIRST ? clamp_key(keys[at], nkeys) : pair_keys[at]) >> shift) & (uint32_t)(nd - 1);
+        // few distinct digits: one shared-memory add per distinct digit and warp instead of 32 colliding ones
+        const unsigned m = same_digit(d, nbits, in);
+        if (in && (threadIdx.x & 31) == __ffs(m) - 1) atomicAdd(&hist[d], (uint32_t)__popc(m));
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < nd; d += THREADS) counts[(size_t)d * gridDim.x + blockIdx.x] = hist[d];
+}
+
+// exclusive prefix of a value over the block's threads; total in *sum
+__device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t *warp_sums, uint32_t *sum) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t t = __shfl_up_sync(QMLB_FULL_MASK, inc, o);
+        if (lane >= o) inc += t;
+    }
+    __syncthreads();
+    if (lane == 31) warp_sums[warp] = inc;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) {
+        const uint32_t s = warp_sums[w];
+        if (w < warp) before += s;
+        all += s;
+    }
+    *sum = all;
+    return before + inc - v;
+}
+
+__global__ void __launch_bounds__(THREADS)
+scan_kernel(uint32_t *__restrict__ counts, uint32_t nblocks, uint32_t *__restrict__ totals) {
+    __shared__ uint32_t warp_sums[WARPS];
+    uint32_t *row = counts + (size_t)blockIdx.x * nblocks;
+    uint32_t carry = 0;
+    for (uint32_t b = 0; b < nblocks; b += THREADS) {
+        const uint32_t at = b + threadIdx.x;
+        const uint32_t v = at < nblocks ? row[at] : 0;
+        uint32_t sum;
+        const uint32_t ex = block_prefix(v, warp_sums, &sum);
+        if (at < nblocks) row[at] = carry + ex;
+        carry += sum;
+    }
+    if (threadIdx.x == 0) totals[blockIdx.x] = carry;
+}
+
+// LAST: writes order[] (and, when START, group_start from the digit totals: one-pass sorts)
+template <typename K, bool FIRST, bool LAST>
+__global__ void __launch_bounds__(THREADS)
+scatter_kernel(const K *__restrict__ keys, const uint32_t *__restrict__ pair_keys, const uint32_t *__restrict__ pair_pos, uint32_t n,
+               uint32_t nkeys, int shift, int nbits, const uint32_t *__restrict__ counts, const uint32_t *__restrict__ totals,
+               uint32_t *__restrict__ out_keys, uint32_t *__restrict__ out_pos, int *__restrict__ group_start) {
+    extern __shared__ uint32_t sm[];           // [nd] digit bases, then [WARPS][nd] running counts
+    __shared__ uint32_t warp_sums[WARPS];
+    const int nd = 1 << nbits;
+    uint32_t *base = sm, *run = sm + nd;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int i = threadIdx.x; i < WARPS * nd; i += THREADS) run[i] = 0;
+    // digit bases: exclusive prefix over the totals (every block computes the same)
+    uint32_t carry = 0;
+    for (int d0 = 0; d0 < nd; d0 += THREADS) {
+        const int d = d0 + threadIdx.x;
+        uint32_t sum;
+        const uint32_t t = d < nd ? totals[d] : 0;
+        const uint32_t ex = block_prefix(t, warp_sums, &sum);
+        if (d < nd) base[d] = carry + ex;
+        if (FIRST && LAST && blockIdx.x == 0 && d <= (int)nkeys) group_start[d] = (int)(carry + ex);
+        carry += sum;
+    }
+    __syncthreads();
+    // pass over the warp's run: digit and rank of every key
+    const uint32_t w0 = blockIdx.x * (uint32_t)TILE + warp * (uint32_t)WARP_TILE;
+    uint32_t key[ITEMS], pos[ITEMS];
+    uint16_t rank[ITEMS];
+    uint32_t *mine = run + warp * nd;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const uint32_t at = w0 + i * 32 + lane;
+        key[i] = 0;
+        pos[i] = at;
+        if (at < n) {
+            key[i] = FIRST ? clamp_key(keys[at], nkeys) : pair_keys[at];
+            if (!FIRST) pos[i] = pair_pos[at];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const bool in = w0 + i * 32 + lane < n;
+        const uint32_t d = (key[i] >> shift) & (uint32_t)(nd - 1);
+        const unsigned m = same_digit(d, nbits, in);
+        const uint32_t before = in ? mine[d] : 0;
+        __syncwarp();
+        rank[i] = (uint16_t)(before + __popc(m & ((1u << lane) - 1u)));
+        if (in && lane == __ffs(m) - 1) mine[d] = before + __popc(m);
+        __syncwarp();
+    }
+    __syncthreads();
+    // first place of every (warp, digit) of this block
+    for (int d = threadIdx.x; d < nd; d += THREADS) {
+        uint32_t at = base[d] + counts[(size_t)d * gridDim.x + blockIdx.x];
+        for (int w = 0; w < WARPS; ++w) {
+            const uint32_t c = run[w * nd + d];
+            run[w * nd + d] = at;
+            at += c;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        if (w0 + i * 32 + lane < n) {
+            const uint32_t to = mine[(key[i] >> shift) & (uint32_t)(nd - 1)] + rank[i];
+            out_pos[to] = pos[i];
+            if (!(FIRST && LAST)) out_keys[to] = key[i];
+        }
+    }
+}
+
+// group_start[v] = first position whose sorted key is not below v
+__global__ void __launch_bounds__(THREADS)
+start_kernel(const uint32_t *__restrict__ sorted, uint32_t n, uint32_t nkeys, int *__restrict__ group_start) {
+    for (uint32_t v = blockIdx.x * THREADS + threadIdx.x; v <= nkeys; v += gridDim.x * THREADS) {
+        uint32_t lo = 0, hi = n;
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) >> 1;
+            if (sorted[mid] < v) lo = mid + 1; else hi = mid;
+        }
+        group_start[v] = (int)lo;
+    }
+}
+
+__global__ void empty_kernel(uint32_t nkeys, int *__restrict__ group_start) {
+    for (uint32_t v = blockIdx.x * THREADS + threadIdx.x; v <= nkeys; v += gridDim.x * THREADS) group_start[v] = 0;
+}
+
+struct Plan {
+    uint32_t blocks;
+    int passes, nbits;       // digit width
+    size_t counts, totals, keys, pos, bytes;      // offsets in scratch: counts, totals, two (keys, positions) pairs
+};
+
+Plan make_plan(size_t n, int nkeys) {
+    Plan p;
+    const int bits = bits_for((unsigned)nkeys);
+    p.passes = (bits + RADIX_BITS - 1) / RADIX_BITS;
+    p.nbits = (bits + p.passes - 1) / p.passes;
+    p.blocks = (uint32_t)((n + TILE - 1) / TILE);
+    auto round = [](size_t v) { return (v + 255) & ~(size_t)255; };
+    const size_t row = round(n * 4);
+    p.counts = 0;
+    p.totals = round(((size_t)p.blocks << p.nbits) * 4);
+    p.keys = p.totals + round((size_t)4 << p.nbits);
+    // a one-pass sort needs no pairs; two passes: pair A, and the sorted keys of the last pass; more: pairs A and B
+    p.pos = p.keys + (p.passes > 1 ? 2 * row : 0);
+    p.bytes = p.pos + (p.passes > 2 ? 2 * row : p.passes > 1 ? row : 0);
+    return p;
+}
+
+template <typename K>
+int run_sort(const K *keys, size_t n, int nkeys, int *order, int *group_start, unsigned char *scratch, cudaStream_t st) {
+    const Plan p = make_plan(n, nkeys);
+    uint32_t *counts = reinterpret_cast<uint32_t *>(scratch + p.counts), *totals = reinterpret_cast<uint32_t *>(scratch + p.totals);
+    const size_t row = (n * 4 + 255) & ~(size_t)255;
+    uint32_t *pk[2] = {reinterpret_cast<uint32_t *>(scratch + p.keys), reinterpret_cast<uint32_t *>(scratch + p.keys + row)};
+    uint32_t *pp[2] = {reinterpret_cast<uint32_t *>(scratch + p.pos), reinterpret_cast<uint32_t *>(scratch + p.pos + row)};
+    const size_t hist_smem = (size_t)4 << p.nbits, scat_smem = ((size_t)4 << p.nbits) * (1 + WARPS);
+    const uint32_t un = (uint32_t)n, uk = (uint32_t)nkeys;
+    uint32_t *pos_out = reinterpret_cast<uint32_t *>(order);
+    for (int i = 0; i < p.passes; ++i) {
+        const bool first = i == 0, last = i == p.passes - 1;
+        const int shift = i * p.nbits;
+        const uint32_t *ik = first ? nullptr : pk[(i - 1) & 1], *ip = first ? nullptr : pp[(i - 1) & 1];
+        if (first) histogram_kernel<K, true><<<p.blocks, THREADS, hist_smem, st>>>(keys, ik, un, uk, shift, p.nbits, counts);
+        else histogram_kernel<K, false><<<p.blocks, THREADS, hist_smem, st>>>(keys, ik, un, uk, shift, p.nbits, counts);
+        scan_kernel<<<1 << p.nbits, THREADS, 0, st>>>(counts, p.blocks, totals);
+        if (first && last) {
+            scatter_kernel<K, true, true><<<p.blocks, THREADS, scat_smem, st>>>(keys, ik, ip, un, uk, shift, p.nbits, counts, totals, nullptr,
+                                                                                pos_out, group_start);
+        } else if (first) {
+            scatter_kernel<K, true, false><<<p.blocks, THREADS, scat_smem, st>>>(keys, ik, ip, un, uk, shift, p.nbits, counts, totals, pk[0],
+                                                                                 pp[0], group_start);
+        } else if (last) {
+            scatter_kernel<K, false, true><<<p.blocks, THREADS, scat_smem, st>>>(keys, ik, ip, un, uk, shift, p.nbits, counts, totals, pk[i & 1],
+                                                                                 pos_out, group_start);
+            const uint32_t sb = (uk + THREADS) / THREADS;
+            start_kernel<<<sb < 1184 ? sb : 1184, THREADS, 0, st>>>(pk[i & 1], un, uk, group_start);
+        } else {
+            scatter_kernel<K, false, false><<<p.blocks, THREADS, scat_smem, st>>>(keys, ik, ip, un, uk, shift, p.nbits, counts, totals, pk[i & 1],
+                                                                                  pp[i & 1], group_start);
+        }
+    }
+    return qmlb::check_launch("qmlb_group_by_key");
+}
+
+}  // namespace
+
+extern "C" size_t qmlb_group_by_key_scratch_bytes(size_t n, int nkeys) {
+    if (n == 0 || n >= (size_t)1 << 31 || nkeys <= 0 || nkeys == INT32_MAX) return 256;
+    return make_plan(n, nkeys).bytes + 256;
+}
+
+extern "C" int qmlb_group_by_key(const void *keys, int key_bits, size_t n, int nkeys, int *order, int *group_start, void *scratch,
+                                 size_t scratch_bytes, qmlb_stream_t stream) {
+    QMLB_REQUIRE(group_start && ((keys && order && scratch) || n == 0), "qmlb_group_by_key: null tensor");
+    QMLB_REQUIRE(key_bits == 32 || key_bits == 64, "qmlb_group_by_key: keys must have 32 or 64 bits");
+    QMLB_REQUIRE(n < (size_t)1 << 31, "qmlb_group_by_key: fewer than 2^31 keys supported");
+    QMLB_REQUIRE(nkeys > 0 && nkeys < INT32_MAX, "qmlb_group_by_key: bad number of keys");
+    cudaStream_t st = qmlb::as_stream(stream);
+    if (n == 0) {
+        empty_kernel<<<((unsigned)nkeys + THREADS) / THREADS < 1184 ? ((unsigned)nkeys + THREADS) / THREADS : 1184, THREADS, 0, st>>>((uint32_t)nkeys, group_start);
+        return qmlb::check_launch("qmlb_group_by_key");
+    }
+    QMLB_REQUIRE(scratch_bytes >= qmlb_group_by_key_scratch_bytes(n, nkeys) - 256, "qmlb_group_by_key: scratch too small");
+    QMLB_REQUIRE(((uintptr_t)scratch & 3) == 0, "qmlb_group_by_key: scratch must be 4-byte aligned");
+    unsigned char *sc = static_cast<unsigned char *>(scratch);
+    return key_bits == 32 ? run_sort(static_cast<const int32_t *>(keys), n, nkeys, order, group_start, sc, st)
+                          : run_sort(static_cast<const int64_t *>(keys), n, nkeys, order, group_start, sc, st);
+}

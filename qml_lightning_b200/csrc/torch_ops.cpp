@@ -8,6 +8,8 @@
 // and one new operator, qml_lightning_b200::sorf_energy, that the rebuilt HadamardFeaturesModel.forward calls: the
 // whole FCHL19 -> PCA -> SORF -> energy chain with the coordinate gradient computed in the same pass (and its RFF
 // twin qml_lightning_b200::rff_energy for RandomFourrierFeaturesModel.forward).
+// qml_lightning_b200::{group_by_key, embedding, embedding_grad, grouped_matmul, grouped_matmul_wgrad} work on rows that
+// belong to groups (elements, species, tokens); all but the first are differentiable, any number of times.
 //
 // This file contains no device code: it only allocates tensors, picks the current stream and device, and forwards
 // raw pointers to libqmlb200.so.  Unlike upstream it honours the current CUDA stream and device of the inputs.
@@ -16,6 +18,7 @@
 #include <torch/all.h>
 #include <torch/script.h>
 
+#include <tuple>
 #include <vector>
 
 #include "qmlb200.h"
@@ -407,6 +410,242 @@ Tensor rff_energy(const Tensor &X, const Tensor &Z, const Tensor &atom_counts, c
                               n_atoms_upper, fast_math)[0];
 }
 
+// ---- qml_lightning_b200 : rows that belong to groups --------------------------------------------------------------
+
+int dtype_code(const Tensor &t, const char *name) {
+    switch (t.scalar_type()) {
+        case torch::kFloat32: return QMLB_F32;
+        case torch::kFloat16: return QMLB_F16;
+        case torch::kBFloat16: return QMLB_BF16;
+        default: TORCH_CHECK(false, name, " must be float32, float16 or bfloat16, got ", t.scalar_type());
+    }
+}
+
+int index_bits(const Tensor &t, const char *name) {
+    TORCH_CHECK(t.scalar_type() == torch::kInt32 || t.scalar_type() == torch::kInt64, name, " must be int32 or int64, got ", t.scalar_type());
+    return t.scalar_type() == torch::kInt32 ? 32 : 64;
+}
+
+void on_device(const Tensor &t, const torch::Device &dev, const char *name) {
+    TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+    TORCH_CHECK(t.device() == dev, name, " must be on ", dev, ", got ", t.device());
+}
+
+bool differentiable(const Tensor &a) { return at::GradMode::is_enabled() && a.requires_grad(); }
+bool differentiable(const Tensor &a, const Tensor &b) { return at::GradMode::is_enabled() && (a.requires_grad() || b.requires_grad()); }
+
+Tensor bytes_on(const Tensor &like, size_t bytes) { return torch::empty({(int64_t)bytes}, like.options().dtype(torch::kUInt8).requires_grad(false)); }
+
+std::tuple<Tensor, Tensor> group_by_key(const Tensor &keys, int64_t nkeys) {
+    TORCH_CHECK(keys.is_cuda(), "keys must be a CUDA tensor");
+    const int bits = index_bits(keys, "keys");
+    TORCH_CHECK(nkeys > 0 && nkeys < INT32_MAX, "group_by_key: nkeys must be between 1 and 2^31 - 2, got ", nkeys);
+    TORCH_CHECK(keys.numel() < (int64_t)1 << 31, "group_by_key: fewer than 2^31 keys supported");
+    c10::cuda::CUDAGuard guard(keys.device());
+    Tensor k = keys.contiguous();
+    const size_t n = (size_t)k.numel();
+    Tensor order = torch::empty({(int64_t)n}, k.options().dtype(torch::kInt32));
+    Tensor start = torch::empty({nkeys + 1}, k.options().dtype(torch::kInt32));
+    const size_t bytes = qmlb_group_by_key_scratch_bytes(n, (int)nkeys);
+    Tensor scratch = bytes_on(k, bytes);
+    check(qmlb_group_by_key(k.data_ptr(), bits, n, (int)nkeys, order.data_ptr<int>(), start.data_ptr<int>(), scratch.data_ptr(), bytes,
+                            current_stream()),
+          "group_by_key");
+    return {order, start};
+}
+
+Tensor embedding(const Tensor &indices, const Tensor &table, double scale);
+Tensor embedding_grad(const Tensor &grad, const Tensor &indices, const Tensor &order, const Tensor &group_start, int64_t rows, double scale);
+Tensor grouped_matmul_any(const Tensor &x, const Tensor &W, const Tensor &group_start, bool transpose);
+Tensor grouped_matmul_wgrad(const Tensor &x, const Tensor &dy, const Tensor &group_start);
+
+Tensor embedding_call(const Tensor &indices, const Tensor &table, double scale) {
+    TORCH_CHECK(table.is_cuda(), "table must be a CUDA tensor");
+    TORCH_CHECK(table.dim() == 2, "table must be [rows, width]");
+    on_device(indices, table.device(), "indices");
+    const int dt = dtype_code(table, "table"), bits = index_bits(indices, "indices");
+    TORCH_CHECK(table.size(1) < INT32_MAX, "embedding: table too wide");
+    c10::cuda::CUDAGuard guard(table.device());
+    Tensor idx = indices.contiguous(), t = table.contiguous();
+    std::vector<int64_t> shape = indices.sizes().vec();
+    shape.push_back(table.size(1));
+    Tensor out = torch::empty(shape, t.options().requires_grad(false));
+    if (out.numel() == 0) return out;
+    check(qmlb_embedding(idx.data_ptr(), bits, t.data_ptr(), dt, (size_t)idx.numel(), t.size(0), (int)t.size(1), (float)scale, out.data_ptr(),
+                         current_stream()),
+          "embedding");
+    return out;
+}
+
+Tensor embedding_grad_call(const Tensor &grad, const Tensor &indices, const Tensor &order, const Tensor &group_start, int64_t rows, double scale) {
+    TORCH_CHECK(grad.is_cuda(), "grad must be a CUDA tensor");
+    on_device(indices, grad.device(), "indices");
+    on_device(order, grad.device(), "order");
+    on_device(group_start, grad.device(), "group_start");
+    const int dt = dtype_code(grad, "grad"), bits = index_bits(indices, "indices");
+    TORCH_CHECK(grad.dim() == indices.dim() + 1 && grad.sizes().slice(0, indices.dim()) == indices.sizes(),
+                "grad must have the shape of indices and one dimension more");
+    const int64_t n = indices.numel(), width = grad.size(-1);
+    TORCH_CHECK(order.scalar_type() == torch::kInt32 && order.numel() == n, "order must be int32 with one entry per index");
+    TORCH_CHECK(rows >= 0 && rows < INT32_MAX, "embedding_grad: rows must be between 0 and 2^31 - 2, got ", rows);
+    TORCH_CHECK(group_start.scalar_type() == torch::kInt32 && group_start.numel() == rows + 1, "group_start must be int32 with rows + 1 entries");
+    TORCH_CHECK(width < INT32_MAX, "embedding_grad: table too wide");
+    c10::cuda::CUDAGuard guard(grad.device());
+    Tensor g = grad.contiguous(), idx = indices.contiguous(), ord = order.contiguous(), st = group_start.contiguous();
+    Tensor out = torch::empty({rows, width}, g.options().requires_grad(false));
+    if (out.numel() == 0) return out;
+    const size_t bytes = qmlb_embedding_grad_scratch_bytes((size_t)n, (int)rows, (int)width);
+    Tensor scratch = bytes_on(g, bytes);
+    check(qmlb_embedding_grad(g.data_ptr(), dt, idx.data_ptr(), bits, ord.data_ptr<int>(), st.data_ptr<int>(), (size_t)n, (int)rows, (int)width,
+                              (float)scale, out.data_ptr(), scratch.data_ptr(), bytes, current_stream()),
+          "embedding_grad");
+    return out;
+}
+
+class EmbeddingFn : public torch::autograd::Function<EmbeddingFn> {
+   public:
+    static variable_list forward(AutogradContext *ctx, Tensor indices, Tensor table, double scale) {
+        ctx->save_for_backward({indices});
+        ctx->saved_data["rows"] = table.size(0);
+        ctx->saved_data["scale"] = scale;
+        return {embedding_call(indices, table, scale)};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grad_output) {
+        Tensor indices = ctx->get_saved_variables()[0], u;
+        const int64_t rows = ctx->saved_data["rows"].toInt();
+        Tensor order, start;
+        if (rows > 0) std::tie(order, start) = group_by_key(indices, rows);
+        else {
+            order = torch::empty({indices.numel()}, indices.options().dtype(torch::kInt32));
+            start = torch::zeros({1}, indices.options().dtype(torch::kInt32));
+        }
+        return {u, embedding_grad(grad_output[0], indices, order, start, rows, ctx->saved_data["scale"].toDouble()), u};
+    }
+};
+
+class EmbeddingGradFn : public torch::autograd::Function<EmbeddingGradFn> {
+   public:
+    static variable_list forward(AutogradContext *ctx, Tensor grad, Tensor indices, Tensor order, Tensor group_start, int64_t rows, double scale) {
+        ctx->save_for_backward({indices});
+        ctx->saved_data["scale"] = scale;
+        return {embedding_grad_call(grad, indices, order, group_start, rows, scale)};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grad_output) {
+        Tensor u;
+        return {embedding(ctx->get_saved_variables()[0], grad_output[0], ctx->saved_data["scale"].toDouble()), u, u, u, u, u};
+    }
+};
+
+Tensor embedding(const Tensor &indices, const Tensor &table, double scale) {
+    return differentiable(table) ? EmbeddingFn::apply(indices, table, scale)[0] : embedding_call(indices, table, scale);
+}
+
+Tensor embedding_grad(const Tensor &grad, const Tensor &indices, const Tensor &order, const Tensor &group_start, int64_t rows, double scale) {
+    return differentiable(grad) ? EmbeddingGradFn::apply(grad, indices, order, group_start, rows, scale)[0]
+                                : embedding_grad_call(grad, indices, order, group_start, rows, scale);
+}
+
+void check_rows(const Tensor &t, const Tensor &like, const char *name, const char *shape) {
+    on_device(t, like.device(), name);
+    TORCH_CHECK(t.dim() == 2, name, " must be ", shape);
+    TORCH_CHECK(t.scalar_type() == like.scalar_type(), name, " must have dtype ", like.scalar_type(), ", got ", t.scalar_type());
+}
+
+Tensor bounds(const Tensor &group_start, const Tensor &like, int64_t groups) {
+    on_device(group_start, like.device(), "group_start");
+    TORCH_CHECK(group_start.dim() == 1 && (groups < 0 ? group_start.numel() >= 2 : group_start.numel() == groups + 1),
+                "group_start must have one entry per group and one more");
+    index_bits(group_start, "group_start");
+    return i32c(group_start);
+}
+
+Tensor grouped_matmul_call(const Tensor &x, const Tensor &W, const Tensor &group_start, bool transpose) {
+    TORCH_CHECK(W.is_cuda(), "W must be a CUDA tensor");
+    TORCH_CHECK(W.dim() == 3 && W.size(0) > 0, "W must be [groups, K, N] with at least one group");
+    check_rows(x, W, "x", "[rows, K]");
+    const int dt = dtype_code(W, "W");
+    const int64_t G = W.size(0), K = W.size(1), N = W.size(2), n = x.size(0);
+    TORCH_CHECK(x.size(1) == (transpose ? N : K), "x has ", x.size(1), " columns, W needs ", transpose ? N : K);
+    TORCH_CHECK(G < INT32_MAX && K < INT32_MAX && N < INT32_MAX, "grouped_matmul: W too large");
+    c10::cuda::CUDAGuard guard(W.device());
+    Tensor xc = x.contiguous(), Wc = W.contiguous(), st = bounds(group_start, W, G);
+    Tensor out = torch::empty({n, transpose ? K : N}, Wc.options().requires_grad(false));
+    if (out.numel() == 0) return out;
+    if (x.size(1) == 0) return out.zero_();
+    const size_t bytes = qmlb_grouped_matmul_workspace_bytes((size_t)n, (int)G, (int)K, (int)N, dt, transpose);
+    Tensor ws = bytes_on(xc, bytes);
+    check(qmlb_grouped_matmul(xc.data_ptr(), Wc.data_ptr(), st.data_ptr<int>(), dt, (size_t)n, (int)G, (int)K, (int)N, transpose, out.data_ptr(),
+                              ws.data_ptr(), bytes, current_stream()),
+          "grouped_matmul");
+    return out;
+}
+
+Tensor grouped_matmul_wgrad_call(const Tensor &x, const Tensor &dy, const Tensor &group_start) {
+    TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+    check_rows(x, x, "x", "[rows, K]");
+    check_rows(dy, x, "dy", "[rows, N]");
+    TORCH_CHECK(x.size(0) == dy.size(0), "x and dy must have the same number of rows");
+    const int dt = dtype_code(x, "x");
+    c10::cuda::CUDAGuard guard(x.device());
+    Tensor xc = x.contiguous(), dyc = dy.contiguous(), st = bounds(group_start, x, -1);
+    const int64_t G = st.numel() - 1, K = x.size(1), N = dy.size(1);
+    TORCH_CHECK(G < INT32_MAX && K < INT32_MAX && N < INT32_MAX, "grouped_matmul_wgrad: sizes too large");
+    Tensor out = torch::empty({G, K, N}, xc.options().requires_grad(false));
+    if (out.numel() == 0) return out;
+    const size_t bytes = qmlb_grouped_matmul_wgrad_workspace_bytes((size_t)x.size(0), (int)G, (int)K, (int)N, dt);
+    Tensor ws = bytes_on(xc, bytes);
+    check(qmlb_grouped_matmul_wgrad(xc.data_ptr(), dyc.data_ptr(), st.data_ptr<int>(), dt, (size_t)x.size(0), (int)G, (int)K, (int)N, out.data_ptr(),
+                                    ws.data_ptr(), bytes, current_stream()),
+          "grouped_matmul_wgrad");
+    return out;
+}
+
+// y = x W[g] (or x W[g]^T).  The three products of a linear map (forward, rows' gradient, matrices' gradient) are one
+// another's derivatives, so every backward calls the differentiable operators again.
+class GroupedMatmulFn : public torch::autograd::Function<GroupedMatmulFn> {
+   public:
+    static variable_list forward(AutogradContext *ctx, Tensor x, Tensor W, Tensor group_start, bool transpose) {
+        ctx->save_for_backward({x, W, group_start});
+        ctx->saved_data["transpose"] = transpose;
+        return {grouped_matmul_call(x, W, group_start, transpose)};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grad_output) {
+        auto s = ctx->get_saved_variables();
+        const bool transpose = ctx->saved_data["transpose"].toBool();
+        Tensor g = grad_output[0], dx, dW, u;
+        if (ctx->needs_input_grad(0)) dx = grouped_matmul_any(g, s[1], s[2], !transpose);
+        if (ctx->needs_input_grad(1)) dW = transpose ? grouped_matmul_wgrad(g, s[0], s[2]) : grouped_matmul_wgrad(s[0], g, s[2]);
+        return {dx, dW, u, u};
+    }
+};
+
+class GroupedWgradFn : public torch::autograd::Function<GroupedWgradFn> {
+   public:
+    static variable_list forward(AutogradContext *ctx, Tensor x, Tensor dy, Tensor group_start) {
+        ctx->save_for_backward({x, dy, group_start});
+        return {grouped_matmul_wgrad_call(x, dy, group_start)};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grad_output) {
+        auto s = ctx->get_saved_variables();
+        Tensor dx, ddy, u;
+        if (ctx->needs_input_grad(0)) dx = grouped_matmul_any(s[1], grad_output[0], s[2], true);
+        if (ctx->needs_input_grad(1)) ddy = grouped_matmul_any(s[0], grad_output[0], s[2], false);
+        return {dx, ddy, u};
+    }
+};
+
+Tensor grouped_matmul_any(const Tensor &x, const Tensor &W, const Tensor &group_start, bool transpose) {
+    return differentiable(x, W) ? GroupedMatmulFn::apply(x, W, group_start, transpose)[0] : grouped_matmul_call(x, W, group_start, transpose);
+}
+
+Tensor grouped_matmul(const Tensor &x, const Tensor &W, const Tensor &group_start, bool transpose) {
+    return grouped_matmul_any(x, W, group_start, transpose);
+}
+
+Tensor grouped_matmul_wgrad(const Tensor &x, const Tensor &dy, const Tensor &group_start) {
+    return differentiable(x, dy) ? GroupedWgradFn::apply(x, dy, group_start)[0] : grouped_matmul_wgrad_call(x, dy, group_start);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(qml_lightning_fchl, m) {
@@ -427,4 +666,10 @@ TORCH_LIBRARY(qml_lightning_b200, m) {
     m.def("sorf_energy", sorf_energy);
     m.def("rff_pack", rff_pack);
     m.def("rff_energy", rff_energy);
+    m.def("group_by_key(Tensor keys, int nkeys) -> (Tensor order, Tensor group_start)", group_by_key);
+    m.def("embedding(Tensor indices, Tensor table, float scale=1.0) -> Tensor", embedding);
+    m.def("embedding_grad(Tensor grad, Tensor indices, Tensor order, Tensor group_start, int rows, float scale=1.0) -> Tensor",
+          embedding_grad);
+    m.def("grouped_matmul(Tensor x, Tensor W, Tensor group_start, bool transpose=False) -> Tensor", grouped_matmul);
+    m.def("grouped_matmul_wgrad(Tensor x, Tensor dy, Tensor group_start) -> Tensor", grouped_matmul_wgrad);
 }
