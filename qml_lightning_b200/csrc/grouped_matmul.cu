@@ -7,6 +7,7 @@
 // Rows in front of the first and behind the last group give zero rows.  The group bounds live on the device and are
 // clamped to [0, n], so the host never waits for them and no value of theirs leads outside the tensors.
 // 64 x 64 tiles of FFMA products with 32-bit sums; any size, alignment and element type.
+#include "grouped_tc.cuh"
 #include "typed.cuh"
 
 namespace {
@@ -177,11 +178,14 @@ int run_wgrad(const void *x, const void *dy, const int *start, int G, int n, int
 
 }  // namespace
 
-extern "C" size_t qmlb_grouped_matmul_workspace_bytes(size_t, int, int, int, int, int) { return 256; }
+extern "C" size_t qmlb_grouped_matmul_workspace_bytes(size_t n, int ngroups, int K, int N, int dtype, int transpose) {
+    (void)transpose;
+    if (n == 0 || ngroups <= 0 || K <= 0 || N <= 0 || dtype == QMLB_F32) return 256;
+    return qmlb::grouped_tc_workspace(ngroups, K, N);
+}
 
 extern "C" int qmlb_grouped_matmul(const void *x, const void *W, const int *group_start, int dtype, size_t n, int ngroups, int K, int N,
                                    int transpose, void *out, void *workspace, size_t workspace_bytes, qmlb_stream_t stream) {
-    (void)workspace; (void)workspace_bytes;
     QMLB_REQUIRE(W && group_start && ((x && out) || n == 0), "qmlb_grouped_matmul: null tensor");
     QMLB_REQUIRE(qmlb::dtype_size(dtype) != 0, "qmlb_grouped_matmul: unknown element type %d", dtype);
     QMLB_REQUIRE(ngroups > 0 && ngroups <= MAX_GROUPS, "qmlb_grouped_matmul: 1..%d groups supported", MAX_GROUPS);
@@ -190,8 +194,10 @@ extern "C" int qmlb_grouped_matmul(const void *x, const void *W, const int *grou
     if (n == 0) return QMLB_OK;
     cudaStream_t st = qmlb::as_stream(stream);
     if (dtype == QMLB_F32) return run_product<float>(x, W, group_start, ngroups, (int)n, K, N, transpose, out, st);
-    if (dtype == QMLB_F16) return run_product<__half>(x, W, group_start, ngroups, (int)n, K, N, transpose, out, st);
-    return run_product<__nv_bfloat16>(x, W, group_start, ngroups, (int)n, K, N, transpose, out, st);
+    QMLB_REQUIRE(workspace && workspace_bytes >= qmlb_grouped_matmul_workspace_bytes(n, ngroups, K, N, dtype, transpose),
+                 "qmlb_grouped_matmul: workspace too small");
+    QMLB_REQUIRE(((uintptr_t)workspace & 255) == 0, "qmlb_grouped_matmul: workspace must be 256-byte aligned");
+    return qmlb::grouped_tc(x, W, group_start, dtype, n, ngroups, K, N, transpose, out, workspace, st);
 }
 
 extern "C" size_t qmlb_grouped_matmul_wgrad_workspace_bytes(size_t, int, int, int, int) { return 256; }

@@ -1,0 +1,399 @@
+// Products of ragged groups of rows with one 16-bit matrix each on the tensor cores (fp16 or bf16 operands, 32-bit sums):
+//
+//   out[r, :] = in[r, :] B_g,   B_g = W[g] (forward) or W[g]^T (gradient of the rows),   rows r of group g
+//
+// One persistent block per SM walks tiles of 128 rows of one group by NT columns, column tiles fastest so that the row
+// tile that neighbours share stays in L2.  Roles: warp 0 fetches 64-deep slices of both operands by TMA into a ring of
+// stages, warp 1 issues tcgen05.mma (M = 128, N = NT, K = 16) into one of two tensor-memory accumulators, warps 4-7 drain
+// the other one: 32 bits to the result type, through a padded shared-memory tile, out in whole 128-byte lines.  Warps 2-3
+// write the zero rows outside the groups.
+// The matrices are read where they are: their rows run along N, which makes them an operand whose lines run along N in the
+// forward product and along K in the transposed one; the instruction takes both.  A row tile may reach over the end of its
+// group: those rows are read and multiplied (rows do not mix) and not stored.
+// Rows whose address is no multiple of 16 bytes (odd widths, offset views) cannot be fetched by TMA; then warps 8-11 bring
+// them with cp.async of 8 or 4 bytes, or 2-byte loads, into the same swizzled stages.
+// Every wait is bounded; a block that gives up fills its remaining tiles with NaN and counts the event (qmlb_tc_timeouts).
+#include "grouped_tc.cuh"
+#include "tcgen.cuh"
+#include "typed.cuh"
+
+#include <type_traits>
+
+namespace {
+
+using namespace qmlb::tc;
+
+constexpr int BM = 128, BK = 64;                 // rows per tile, depth per stage (one 128-byte line)
+constexpr int MAX_STAGES = 8;
+constexpr uint32_t A_BYTES = BM * BK * 2;
+constexpr int TMA_WARP = 0, MMA_WARP = 1, EPI_WARP = 4, LOAD_WARP = 8;
+constexpr int NTHREADS = 256, NTHREADS_LOADED = 384;
+constexpr int STAGE_ROW = 144;                   // bytes per row of the epilogue's tile: 64 columns of 2 bytes, padded
+constexpr uint32_t EPI_BYTES = 4 * 32 * STAGE_ROW;
+constexpr uint32_t TMEM_COLS = 512, BUF_COLS = 256;
+constexpr size_t SMEM_LIMIT = 227 * 1024;
+
+__device__ int g_timeouts = 0;
+
+struct Shape {
+    int n, G, K, out;        // rows, groups, depth of the sums, columns of the result
+    int NT, ntiles;          // columns per tile, column tiles
+    int nchunks, stages;
+    uint32_t b_bytes;        // one stage of the matrix operand
+    int in_access;           // widest access that can follow the rows of `in` (16: TMA), in bytes
+    int out_access;
+};
+
+struct Groups {              // in shared memory
+    int *start;              // [G + 1] clamped bounds
+    int *tiles;              // [G + 1] row tiles before group g
+};
+
+// row tile -> group and rows
+__device__ __forceinline__ void locate(const Groups &s, int G, int mt, int &g, int &row0, int &row1) {
+    int lo = 0, hi = G - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s.tiles[mid] <= mt) lo = mid; else hi = mid - 1;
+    }
+    g = lo;
+    row0 = s.start[lo] + (mt - s.tiles[lo]) * BM;
+    row1 = max(s.start[lo + 1], s.start[lo]);
+}
+
+// Store one warp's 32 x 64 tile from shared memory; `w` bytes per access (a power of two that follows the result's rows).
+template <int W>
+__device__ __forceinline__ void store_rows(const unsigned char *tile, unsigned char *out, size_t row_bytes, int rows, int bytes, int lane) {
+    constexpr int PER_ROW = 128 / W;             // accesses per 128-byte line
+#pragma unroll 4
+    for (int i = lane; i < 32 * PER_ROW; i += 32) {
+        const int r = i / PER_ROW, c = (i % PER_ROW) * W;
+        if (r < rows && c < bytes)
+            *reinterpret_cast<typename qmlb::Word<W>::type *>(out + (size_t)r * row_bytes + c) =
+                *reinterpret_cast<const typename qmlb::Word<W>::type *>(tile + r * STAGE_ROW + c);
+    }
+}
+
+// One stage of rows that TMA cannot follow: 128 threads, W bytes per access (2: through registers).
+template <int W>
+__device__ __forceinline__ void load_rows(const unsigned char *in, size_t row_bytes, int row0, int n, int k_byte0, uint32_t dst, int t) {
+    constexpr int PER_ROW = 128 / W;
+#pragma unroll 8
+    for (int i = t; i < BM * PER_ROW; i += 128) {
+        const int r = i / PER_ROW, c = (i % PER_ROW) * W;
+        const bool wanted = row0 + r < n && (size_t)(k_byte0 + c) < row_bytes;
+        const unsigned char *src = wanted ? in + (size_t)(row0 + r) * row_bytes + k_byte0 + c : in;
+        const uint32_t to = dst + (uint32_t)r * 128u + ((uint32_t)c ^ ((uint32_t)(r & 7) << 4));      // the 128-byte swizzle
+        if (W >= 4) {
+            cp_async<W >= 4 ? W : 4>(to, src, wanted);
+        } else {
+            const uint16_t v = wanted ? *reinterpret_cast<const uint16_t *>(src) : (uint16_t)0;
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(v) : "memory");
+        }
+    }
+}
+
+template <typename T, bool TRANS, bool LOADED>
+__global__ void __launch_bounds__(LOADED ? NTHREADS_LOADED : NTHREADS, 1)
+grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant__ CUtensorMap map_w, const T *__restrict__ in,
+               const int *__restrict__ start, Shape p, T *__restrict__ out) {
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_free[2], done;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int failed;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    unsigned char *sp = smem_raw + (sbase - smem_u32(smem_raw));
+    const uint32_t stage_bytes = A_BYTES + p.b_bytes;
+    unsigned char *epi = sp + (size_t)p.stages * stage_bytes;
+    Groups gr;
+    gr.start = reinterpret_cast<int *>(epi + EPI_BYTES);
+    gr.tiles = gr.start + p.G + 1;
+    auto bar = [](const uint64_t &b) { return smem_u32(&b); };
+
+    if (tid == 0) {
+        for (int s = 0; s < p.stages; ++s) {
+            mbar_init(bar(full[s]), LOADED ? 5 : 1);        // the TMA issuer, and the four loading warps
+            mbar_init(bar(empty[s]), 1);
+        }
+        for (int i = 0; i < 2; ++i) { mbar_init(bar(acc_full[i]), 1); mbar_init(bar(acc_free[i]), 4); }
+        mbar_init(bar(done), 1);
+        failed = 0;
+        mbar_init_fence();
+        if (!LOADED) prefetch_map(&map_in);
+        prefetch_map(&map_w);
+    }
+    for (int g = tid; g <= p.G; g += blockDim.x) gr.start[g] = min(max(start[g], 0), p.n);
+    if (warp == MMA_WARP) tmem_alloc(smem_u32(&tmem_slot), TMEM_COLS);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 0) {                                        // row tiles before every group
+        int before = 0;
+        for (int g0 = 0; g0 < p.G; g0 += 32) {
+            const int g = g0 + lane;
+            const int t = g < p.G ? (max(gr.start[g + 1] - gr.start[g], 0) + BM - 1) / BM : 0;
+            int inc = t;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(QMLB_FULL_MASK, inc, o);
+                if (lane >= o) inc += v;
+            }
+            if (g < p.G) gr.tiles[g] = before + inc - t;
+            before += __shfl_sync(QMLB_FULL_MASK, inc, 31);
+        }
+        if (lane == 0) gr.tiles[p.G] = before;
+    }
+    __syncthreads();
+    const uint32_t tmem = tmem_slot;
+    const int total = gr.tiles[p.G] * p.ntiles;
+    const volatile int *gave_up = &failed;
+
+    if (warp == TMA_WARP) {
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+                int g, row0, row1;
+                locate(gr, p.G, tile / p.ntiles, g, row0, row1);
+                const int col0 = (tile % p.ntiles) * p.NT;
+                // forward: boxes of 64 columns by 64 deep, as many as reach into the matrix; transposed: one box of NT rows
+                const int boxes = TRANS ? 1 : min((p.NT + 63) / 64, (p.out - col0 + 63) / 64);
+                const uint32_t bytes = (LOADED ? 0u : A_BYTES) + (TRANS ? p.b_bytes : (uint32_t)boxes * 8192u);
+                for (int c = 0; c < p.nchunks; ++c, ++it) {
+                    const int s = it % p.stages;
+                    if (!mbar_wait(bar(empty[s]), ((uint32_t)(it / p.stages) & 1u) ^ 1u, gave_up)) { ok = false; break; }
+                    const uint32_t a = sbase + (uint32_t)s * stage_bytes, b = a + A_BYTES;
+                    mbar_expect_tx(bar(full[s]), bytes);
+                    if (!LOADED) tma_2d(a, &map_in, c * BK, row0, bar(full[s]));
+                    if (TRANS) tma_3d(b, &map_w, c * BK, col0, g, bar(full[s]));
+                    else
+                        for (int j = 0; j < boxes; ++j) tma_3d(b + (uint32_t)j * 8192u, &map_w, col0 + j * 64, c * BK, g, bar(full[s]));
+                }
+            }
+            if (!ok) failed = 1;
+            // no copy may be in flight when the block leaves
+            for (int i = max(0, it - p.stages); i < it; ++i)
+                for (int tries = 0; tries < WAIT_LIMIT && !mbar_try(bar(full[i % p.stages]), (uint32_t)(i / p.stages) & 1u); ++tries) {}
+        }
+    } else if (warp == MMA_WARP) {
+        const uint32_t idesc = instr_desc(sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value, false, !TRANS, BM, p.NT);
+        int it = 0, j = 0;
+        bool ok = true;
+        for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x, ++j) {
+            const int buf = j & 1;
+            bool w = mbar_wait(bar(acc_free[buf]), ((uint32_t)(j >> 1) & 1u) ^ 1u, gave_up);
+            for (int c = 0; c < p.nchunks; ++c, ++it) {
+                const int s = it % p.stages;
+                w = w && mbar_wait(bar(full[s]), (uint32_t)(it / p.stages) & 1u, gave_up);
+                if (!__all_sync(QMLB_FULL_MASK, w)) { ok = false; break; }
+                fence_after();
+                if (lane == 0) {
+                    const uint32_t a = sbase + (uint32_t)s * stage_bytes;
+                    const uint32_t al = desc_lo(a, 16), bl = desc_lo(a + A_BYTES, TRANS ? 16 : 8192);
+                    constexpr uint32_t b_step = TRANS ? 2u : 128u;          // 16 deep: 32 bytes along the lines, or 16 lines
+#pragma unroll
+                    for (int k = 0; k < BK / 16; ++k)
+                        mma_f16(tmem + (uint32_t)buf * BUF_COLS, al + k * 2u, DESC_HI_SW128, bl + k * b_step, DESC_HI_SW128, idesc, (c | k) ? 1u : 0u);
+                    mma_commit(bar(empty[s]));
+                    if (c == p.nchunks - 1) mma_commit(bar(acc_full[buf]));
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok) failed = 1;
+        if (lane == 0) mma_commit(bar(done));                   // everything issued has left the tensor pipe
+        __syncwarp();
+        for (int tries = 0; tries < WAIT_LIMIT && !mbar_try(bar(done), 0u); ++tries) {}
+    } else if (warp < EPI_WARP) {
+        // zero rows in front of the first group and behind the last
+        const int first = gr.start[0], last = max(gr.start[p.G], first);
+        const int outside = first + (p.n - last);
+        for (int i = blockIdx.x * 2 + (warp - 2); i < outside; i += gridDim.x * 2) {
+            T *row = out + (size_t)(i < first ? i : last + (i - first)) * p.out;
+            for (int c = lane; c < p.out; c += 32) row[c] = qmlb::from_f32<T>(0.f);
+        }
+    } else if (warp < LOAD_WARP) {
+        const int quarter = warp & 3;
+        unsigned char *mine = epi + quarter * 32 * STAGE_ROW;
+        const size_t row_bytes = (size_t)p.out * 2;
+        int j = 0;
+        bool ok = true;
+        for (int tile = blockIdx.x; tile < total; tile += gridDim.x, ++j) {
+            const int buf = j & 1;
+            int g, row0, row1;
+            locate(gr, p.G, tile / p.ntiles, g, row0, row1);
+            const int col0 = (tile % p.ntiles) * p.NT, row = row0 + quarter * 32;
+            const int rows = min(32, row1 - row);
+            ok = ok && mbar_wait(bar(acc_full[buf]), (uint32_t)(j >> 1) & 1u, gave_up);
+            ok = __all_sync(QMLB_FULL_MASK, ok);
+            if (!ok) failed = 1;                                // at once: the other roles stop waiting
+            fence_after();
+            const uint32_t from = tmem + (uint32_t)buf * BUF_COLS + ((uint32_t)(quarter * 32) << 16);
+            for (int c = 0; c < p.NT; c += 64) {
+                uint32_t v[64];
+                const int left = p.NT - c;
+                if (ok) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        if (u * 16 < left) tmem_ld16(from + (uint32_t)(c + u * 16), v + u * 16);
+                    tmem_ld_wait();
+                    if (c + 64 >= p.NT) {                       // the accumulator is free once it sits in registers
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bar(acc_free[buf]));
+                    }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 64; ++u) v[u] = 0x7fc00000u;
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    qmlb::Pack<T, 8> k;
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) k.item[q] = qmlb::from_f32<T>(__uint_as_float(v[u * 8 + q]));
+                    *reinterpret_cast<uint4 *>(mine + lane * STAGE_ROW + u * 16) = k.word;
+                }
+                __syncwarp();
+                const int bytes = min(min(64, left), p.out - col0 - c) * 2;
+                unsigned char *to = reinterpret_cast<unsigned char *>(out) + (size_t)row * row_bytes + (size_t)(col0 + c) * 2;
+                if (p.out_access == 16) store_rows<16>(mine, to, row_bytes, rows, bytes, lane);
+                else if (p.out_access == 8) store_rows<8>(mine, to, row_bytes, rows, bytes, lane);
+                else if (p.out_access == 4) store_rows<4>(mine, to, row_bytes, rows, bytes, lane);
+                else store_rows<2>(mine, to, row_bytes, rows, bytes, lane);
+                __syncwarp();
+            }
+        }
+    } else if (LOADED) {
+        const int t = tid - LOAD_WARP * 32;
+        const unsigned char *src = reinterpret_cast<const unsigned char *>(in);
+        const size_t row_bytes = (size_t)p.K * 2;
+        constexpr int AHEAD = 2;                                // stages whose copies are in flight behind the newest
+        int it = 0;
+        bool ok = true;
+        auto publish = [&](int i) {                             // this thread's copies of stage i have landed
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(full[i % p.stages]));
+        };
+        for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+            int g, row0, row1;
+            locate(gr, p.G, tile / p.ntiles, g, row0, row1);
+            for (int c = 0; c < p.nchunks; ++c, ++it) {
+                const int s = it % p.stages;
+                ok = __all_sync(QMLB_FULL_MASK, mbar_wait(bar(empty[s]), ((uint32_t)(it / p.stages) & 1u) ^ 1u, gave_up));
+                if (!ok) break;
+                const uint32_t a = sbase + (uint32_t)s * stage_bytes;
+                if (p.in_access >= 8) load_rows<8>(src, row_bytes, row0, p.n, c * BK * 2, a, t);
+                else if (p.in_access == 4) load_rows<4>(src, row_bytes, row0, p.n, c * BK * 2, a, t);
+                else load_rows<2>(src, row_bytes, row0, p.n, c * BK * 2, a, t);
+                cp_async_commit();
+                if (it >= AHEAD) {
+                    cp_async_wait<AHEAD>();
+                    publish(it - AHEAD);
+                }
+            }
+        }
+        cp_async_wait<0>();
+        for (int i = max(0, it - AHEAD); i < it; ++i) publish(i);
+        if (!ok) failed = 1;
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (tid == 0 && failed) atomicAdd(&g_timeouts, 1);
+    if (warp == MMA_WARP) tmem_free(tmem, TMEM_COLS);
+}
+
+// W [G][K][N] with rows that no 16-byte access can follow -> the same with rows padded to a multiple of 8 elements
+template <typename T>
+__global__ void __launch_bounds__(256)
+pad_kernel(const T *__restrict__ W, size_t rows, int N, int Np, T *__restrict__ to) {
+    const size_t total = rows * (size_t)Np;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
+        const size_t r = i / (unsigned)Np;
+        const int c = (int)(i - r * (unsigned)Np);
+        to[i] = c < N ? W[r * N + c] : qmlb::from_f32<T>(0.f);
+    }
+}
+
+bool needs_pad(const void *W, int N) { return ((uintptr_t)W & 15) != 0 || (N & 7) != 0; }
+
+template <typename T, bool TRANS, bool LOADED>
+int launch(const CUtensorMap &mi, const CUtensorMap &mw, const T *in, const int *start, const Shape &p, int blocks, T *out, cudaStream_t st) {
+    const size_t smem = (size_t)p.stages * (A_BYTES + p.b_bytes) + EPI_BYTES + (size_t)2 * (p.G + 1) * 4 + 1024;
+    auto kernel = grouped_kernel<T, TRANS, LOADED>;
+    if (int rc = qmlb::ensure_smem(kernel, smem, "qmlb_grouped_matmul")) return rc;
+    kernel<<<blocks, LOADED ? NTHREADS_LOADED : NTHREADS, smem, st>>>(mi, mw, in, start, p, out);
+    return qmlb::check_launch("qmlb_grouped_matmul");
+}
+
+template <typename T>
+int run(const void *x, const void *W, const int *start, size_t n, int G, int K, int N, int transpose, void *out, void *workspace, cudaStream_t st) {
+    const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+    Shape p;
+    p.n = (int)n;
+    p.G = G;
+    p.K = transpose ? N : K;
+    p.out = transpose ? K : N;
+    p.nchunks = (p.K + BK - 1) / BK;
+    p.in_access = qmlb::access_bytes((size_t)p.K * 2, 2, x);
+    p.out_access = qmlb::access_bytes((size_t)p.out * 2, 2, out);
+    // Columns per tile: as many as one accumulator holds, so that the rows are read once, in equal parts; fewer when the row
+    // tiles alone do not give every SM a tile.
+    const long mtiles = (long)((n + BM - 1) / BM);
+    long nt = (p.out + 255) / 256;
+    const long wanted = (148 + mtiles - 1) / mtiles, most = (p.out + 63) / 64;
+    if (nt < wanted) nt = wanted < most ? wanted : most;
+    p.NT = (int)(((p.out + nt - 1) / nt + 15) / 16 * 16);
+    p.ntiles = (p.out + p.NT - 1) / p.NT;
+    p.b_bytes = transpose ? (uint32_t)p.NT * 128u : (uint32_t)((p.NT + 63) / 64) * 8192u;
+    p.b_bytes = (p.b_bytes + 1023u) & ~1023u;
+    const size_t fixed = EPI_BYTES + (size_t)2 * (G + 1) * 4 + 1024 + 512;
+    p.stages = (int)((SMEM_LIMIT - fixed) / (A_BYTES + p.b_bytes));
+    if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+
+    const void *Wp = W;
+    int Np = N;
+    if (needs_pad(W, N)) {
+        Np = (N + 7) & ~7;
+        const size_t total = (size_t)G * K * Np, b = (total + 1023) / 1024;
+        pad_kernel<T><<<(unsigned)(b < 2368 ? b : 2368), 256, 0, st>>>(static_cast<const T *>(W), (size_t)G * K, N, Np, static_cast<T *>(workspace));
+        Wp = workspace;
+    }
+    CUtensorMap mi, mw;
+    if (int rc = qmlb::encode_tiles(&mw, Wp, bf16, (uint64_t)N, (uint64_t)K, (uint64_t)G, (uint64_t)Np * 2, transpose ? (uint32_t)p.NT : 64u,
+                                    "qmlb_grouped_matmul"))
+        return rc;
+    const bool loaded = p.in_access < 16;
+    mi = mw;
+    if (!loaded)
+        if (int rc = qmlb::encode_tiles(&mi, x, bf16, (uint64_t)p.K, (uint64_t)n, 0, (uint64_t)p.K * 2, BM, "qmlb_grouped_matmul")) return rc;
+    const long tiles = (mtiles + G) * p.ntiles;
+    const int blocks = (int)(tiles < 148 ? tiles : 148);
+    const T *xi = static_cast<const T *>(x);
+    T *o = static_cast<T *>(out);
+    if (transpose) return loaded ? launch<T, true, true>(mi, mw, xi, start, p, blocks, o, st) : launch<T, true, false>(mi, mw, xi, start, p, blocks, o, st);
+    return loaded ? launch<T, false, true>(mi, mw, xi, start, p, blocks, o, st) : launch<T, false, false>(mi, mw, xi, start, p, blocks, o, st);
+}
+
+}  // namespace
+
+namespace qmlb {
+
+size_t grouped_tc_workspace(int G, int K, int N) { return (size_t)G * K * ((N + 7) & ~7) * 2 + 256; }
+
+int grouped_tc(const void *x, const void *W, const int *start, int dtype, size_t n, int G, int K, int N, int transpose, void *out,
+               void *workspace, cudaStream_t st) {
+    return dtype == QMLB_F16 ? run<__half>(x, W, start, n, G, K, N, transpose, out, workspace, st)
+                             : run<__nv_bfloat16>(x, W, start, n, G, K, N, transpose, out, workspace, st);
+}
+
+int grouped_tc_timeouts() {
+    int v = -1;
+    if (cudaMemcpyFromSymbol(&v, g_timeouts, sizeof(int)) != cudaSuccess) return -1;
+    return v;
+}
+
+}  // namespace qmlb

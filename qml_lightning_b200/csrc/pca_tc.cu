@@ -302,13 +302,14 @@ pca_tc_kernel(const float *__restrict__ in, const float *__restrict__ P, const i
 namespace qmlb {
 int rff_tc_timeouts();   // rff_tc.cu
 int pca_tc2_timeouts();  // pca_tc2.cu
+int grouped_tc_timeouts();  // grouped_tc.cu
 }
 
 extern "C" int qmlb_tc_timeouts(void) {
     int v = -1;
     if (cudaMemcpyFromSymbol(&v, g_tc_timeouts, sizeof(int)) != cudaSuccess) return -1;
-    const int w = qmlb::rff_tc_timeouts(), u = qmlb::pca_tc2_timeouts();
-    return (w < 0 || u < 0) ? -1 : v + w + u;
+    const int w = qmlb::rff_tc_timeouts(), u = qmlb::pca_tc2_timeouts(), g = qmlb::grouped_tc_timeouts();
+    return (w < 0 || u < 0 || g < 0) ? -1 : v + w + u + g;
 }
 
 extern "C" int qmlb_pca_project_tc(const float *in, const float *reductors, const int *group_start, int nelements,
