@@ -200,11 +200,13 @@ extern "C" int qmlb_grouped_matmul(const void *x, const void *W, const int *grou
     return qmlb::grouped_tc(x, W, group_start, dtype, n, ngroups, K, N, transpose, out, workspace, st);
 }
 
-extern "C" size_t qmlb_grouped_matmul_wgrad_workspace_bytes(size_t, int, int, int, int) { return 256; }
+extern "C" size_t qmlb_grouped_matmul_wgrad_workspace_bytes(size_t n, int ngroups, int K, int N, int dtype) {
+    if (n == 0 || ngroups <= 0 || K <= 0 || N <= 0 || dtype == QMLB_F32) return 256;
+    return qmlb::grouped_wgrad_tc_workspace(n, ngroups, K, N);
+}
 
 extern "C" int qmlb_grouped_matmul_wgrad(const void *x, const void *dy, const int *group_start, int dtype, size_t n, int ngroups, int K, int N,
                                          void *dW, void *workspace, size_t workspace_bytes, qmlb_stream_t stream) {
-    (void)workspace; (void)workspace_bytes;
     QMLB_REQUIRE(dW && group_start && ((x && dy) || n == 0), "qmlb_grouped_matmul_wgrad: null tensor");
     const int es = qmlb::dtype_size(dtype);
     QMLB_REQUIRE(es != 0, "qmlb_grouped_matmul_wgrad: unknown element type %d", dtype);
@@ -217,6 +219,8 @@ extern "C" int qmlb_grouped_matmul_wgrad(const void *x, const void *dy, const in
         return QMLB_OK;
     }
     if (dtype == QMLB_F32) return run_wgrad<float>(x, dy, group_start, ngroups, (int)n, K, N, dW, st);
-    if (dtype == QMLB_F16) return run_wgrad<__half>(x, dy, group_start, ngroups, (int)n, K, N, dW, st);
-    return run_wgrad<__nv_bfloat16>(x, dy, group_start, ngroups, (int)n, K, N, dW, st);
+    QMLB_REQUIRE(workspace && workspace_bytes >= qmlb_grouped_matmul_wgrad_workspace_bytes(n, ngroups, K, N, dtype),
+                 "qmlb_grouped_matmul_wgrad: workspace too small");
+    QMLB_REQUIRE(((uintptr_t)workspace & 255) == 0, "qmlb_grouped_matmul_wgrad: workspace must be 256-byte aligned");
+    return qmlb::grouped_wgrad_tc(x, dy, group_start, dtype, n, ngroups, K, N, dW, workspace, st);
 }

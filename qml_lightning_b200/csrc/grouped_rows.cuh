@@ -1,0 +1,121 @@
+// Device helpers shared by the tensor-core kernels of the grouped products: group lookup, the epilogue's padded tile, and
+// loads of rows that TMA cannot follow.
+#pragma once
+
+#include "tcgen.cuh"
+#include "typed.cuh"
+
+namespace qmlb {
+namespace tc {
+
+constexpr int BK = 64;                           // depth per stage: one 128-byte line of 16-bit elements
+constexpr int MAX_STAGES = 8;
+constexpr int STAGE_ROW = 144;                   // bytes per row of a warp's epilogue tile: 128 bytes, padded against bank conflicts
+constexpr uint32_t EPI_BYTES = 4 * 32 * STAGE_ROW;
+constexpr uint32_t TMEM_COLS = 512, BUF_COLS = 256;
+constexpr size_t SMEM_LIMIT = 227 * 1024;
+
+struct Groups {              // in shared memory
+    int *start;              // [G + 1] clamped bounds
+    int *parts;              // [G + 1] parts (row tiles, or splits of the sum) before group g
+    int *split;              // null, or [G + 1]: parts before group g that belong to groups of several parts
+    __device__ __forceinline__ int rows(int g) const { return max(start[g + 1] - start[g], 0); }
+    // group that holds part `i`
+    __device__ __forceinline__ int find(int G, int i) const {
+        int lo = 0, hi = G - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (parts[mid] <= i) lo = mid; else hi = mid - 1;
+        }
+        return lo;
+    }
+};
+
+// Fill `start` (all threads) and `parts` (warp 0): a group of r rows has ceil(r / part_rows) parts.  Ends with a barrier.
+__device__ __forceinline__ void read_groups(const Groups &s, const int *__restrict__ start, int G, int n, int part_rows) {
+    for (int g = threadIdx.x; g <= G; g += blockDim.x) s.start[g] = min(max(start[g], 0), n);
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
+        for (int pass = 0; pass < (s.split ? 2 : 1); ++pass) {
+            int *to = pass ? s.split : s.parts;
+            int before = 0;
+            for (int g0 = 0; g0 < G; g0 += 32) {
+                const int g = g0 + lane;
+                int t = g < G ? (s.rows(g) + part_rows - 1) / part_rows : 0;
+                if (pass && t == 1) t = 0;
+                int inc = t;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int v = __shfl_up_sync(QMLB_FULL_MASK, inc, o);
+                    if (lane >= o) inc += v;
+                }
+                if (g < G) to[g] = before + inc - t;
+                before += __shfl_sync(QMLB_FULL_MASK, inc, 31);
+            }
+            if (lane == 0) to[G] = before;
+        }
+    }
+    __syncthreads();
+}
+
+// Store one warp's tile (32 rows of up to 128 bytes) from shared memory, W bytes per access.
+template <int W>
+__device__ __forceinline__ void store_rows(const unsigned char *tile, unsigned char *out, size_t row_bytes, int rows, int bytes, int lane) {
+    constexpr int PER_ROW = 128 / W;
+#pragma unroll 4
+    for (int i = lane; i < 32 * PER_ROW; i += 32) {
+        const int r = i / PER_ROW, c = (i % PER_ROW) * W;
+        if (r < rows && c < bytes)
+            *reinterpret_cast<typename Word<W>::type *>(out + (size_t)r * row_bytes + c) =
+                *reinterpret_cast<const typename Word<W>::type *>(tile + r * STAGE_ROW + c);
+    }
+}
+__device__ __forceinline__ void store_tile(const unsigned char *tile, unsigned char *out, size_t row_bytes, int rows, int bytes, int lane, int access) {
+    if (access == 16) store_rows<16>(tile, out, row_bytes, rows, bytes, lane);
+    else if (access == 8) store_rows<8>(tile, out, row_bytes, rows, bytes, lane);
+    else if (access == 4) store_rows<4>(tile, out, row_bytes, rows, bytes, lane);
+    else store_rows<2>(tile, out, row_bytes, rows, bytes, lane);
+}
+
+// 32 registers of 64 accumulator columns of this thread's row -> result type -> the warp's tile
+template <typename T>
+__device__ __forceinline__ void stage_row(unsigned char *tile, int lane, const uint32_t (&v)[64]) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        Pack<T, 8> k;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) k.item[q] = from_f32<T>(__uint_as_float(v[u * 8 + q]));
+        *reinterpret_cast<uint4 *>(tile + lane * STAGE_ROW + u * 16) = k.word;
+    }
+}
+
+// LINES lines of 128 bytes (64 elements) of consecutive rows into a swizzled box, W bytes per access (2: through registers),
+// by `threads` threads.  Rows from `end` on and bytes behind the row's end become zeros.
+template <int W>
+__device__ __forceinline__ void load_lines(const unsigned char *in, size_t row_bytes, int row0, int end, size_t byte0, uint32_t dst, int lines, int t,
+                                           int threads) {
+    constexpr int PER_ROW = 128 / W;
+#pragma unroll 8
+    for (int i = t; i < lines * PER_ROW; i += threads) {
+        const int r = i / PER_ROW, c = (i % PER_ROW) * W;
+        const bool wanted = row0 + r < end && byte0 + c < row_bytes;
+        const unsigned char *src = wanted ? in + (size_t)(row0 + r) * row_bytes + byte0 + c : in;
+        const uint32_t to = dst + (uint32_t)r * 128u + ((uint32_t)c ^ ((uint32_t)(r & 7) << 4));      // the 128-byte swizzle
+        if (W >= 4) {
+            cp_async<W >= 4 ? W : 4>(to, src, wanted);
+        } else {
+            const uint16_t v = wanted ? *reinterpret_cast<const uint16_t *>(src) : (uint16_t)0;
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(v) : "memory");
+        }
+    }
+}
+__device__ __forceinline__ void load_box(const unsigned char *in, size_t row_bytes, int row0, int end, size_t byte0, uint32_t dst, int lines, int t,
+                                         int threads, int access) {
+    if (access >= 8) load_lines<8>(in, row_bytes, row0, end, byte0, dst, lines, t, threads);
+    else if (access == 4) load_lines<4>(in, row_bytes, row0, end, byte0, dst, lines, t, threads);
+    else load_lines<2>(in, row_bytes, row0, end, byte0, dst, lines, t, threads);
+}
+
+}  // namespace tc
+}  // namespace qmlb

@@ -14,8 +14,7 @@
 // them with cp.async of 8 or 4 bytes, or 2-byte loads, into the same swizzled stages.
 // Every wait is bounded; a block that gives up fills its remaining tiles with NaN and counts the event (qmlb_tc_timeouts).
 #include "grouped_tc.cuh"
-#include "tcgen.cuh"
-#include "typed.cuh"
+#include "grouped_rows.cuh"
 
 #include <type_traits>
 
@@ -23,15 +22,10 @@ namespace {
 
 using namespace qmlb::tc;
 
-constexpr int BM = 128, BK = 64;                 // rows per tile, depth per stage (one 128-byte line)
-constexpr int MAX_STAGES = 8;
+constexpr int BM = 128;                          // rows per tile
 constexpr uint32_t A_BYTES = BM * BK * 2;
 constexpr int TMA_WARP = 0, MMA_WARP = 1, EPI_WARP = 4, LOAD_WARP = 8;
 constexpr int NTHREADS = 256, NTHREADS_LOADED = 384;
-constexpr int STAGE_ROW = 144;                   // bytes per row of the epilogue's tile: 64 columns of 2 bytes, padded
-constexpr uint32_t EPI_BYTES = 4 * 32 * STAGE_ROW;
-constexpr uint32_t TMEM_COLS = 512, BUF_COLS = 256;
-constexpr size_t SMEM_LIMIT = 227 * 1024;
 
 __device__ int g_timeouts = 0;
 
@@ -43,55 +37,6 @@ struct Shape {
     int in_access;           // widest access that can follow the rows of `in` (16: TMA), in bytes
     int out_access;
 };
-
-struct Groups {              // in shared memory
-    int *start;              // [G + 1] clamped bounds
-    int *tiles;              // [G + 1] row tiles before group g
-};
-
-// row tile -> group and rows
-__device__ __forceinline__ void locate(const Groups &s, int G, int mt, int &g, int &row0, int &row1) {
-    int lo = 0, hi = G - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (s.tiles[mid] <= mt) lo = mid; else hi = mid - 1;
-    }
-    g = lo;
-    row0 = s.start[lo] + (mt - s.tiles[lo]) * BM;
-    row1 = max(s.start[lo + 1], s.start[lo]);
-}
-
-// Store one warp's 32 x 64 tile from shared memory; `w` bytes per access (a power of two that follows the result's rows).
-template <int W>
-__device__ __forceinline__ void store_rows(const unsigned char *tile, unsigned char *out, size_t row_bytes, int rows, int bytes, int lane) {
-    constexpr int PER_ROW = 128 / W;             // accesses per 128-byte line
-#pragma unroll 4
-    for (int i = lane; i < 32 * PER_ROW; i += 32) {
-        const int r = i / PER_ROW, c = (i % PER_ROW) * W;
-        if (r < rows && c < bytes)
-            *reinterpret_cast<typename qmlb::Word<W>::type *>(out + (size_t)r * row_bytes + c) =
-                *reinterpret_cast<const typename qmlb::Word<W>::type *>(tile + r * STAGE_ROW + c);
-    }
-}
-
-// One stage of rows that TMA cannot follow: 128 threads, W bytes per access (2: through registers).
-template <int W>
-__device__ __forceinline__ void load_rows(const unsigned char *in, size_t row_bytes, int row0, int n, int k_byte0, uint32_t dst, int t) {
-    constexpr int PER_ROW = 128 / W;
-#pragma unroll 8
-    for (int i = t; i < BM * PER_ROW; i += 128) {
-        const int r = i / PER_ROW, c = (i % PER_ROW) * W;
-        const bool wanted = row0 + r < n && (size_t)(k_byte0 + c) < row_bytes;
-        const unsigned char *src = wanted ? in + (size_t)(row0 + r) * row_bytes + k_byte0 + c : in;
-        const uint32_t to = dst + (uint32_t)r * 128u + ((uint32_t)c ^ ((uint32_t)(r & 7) << 4));      // the 128-byte swizzle
-        if (W >= 4) {
-            cp_async<W >= 4 ? W : 4>(to, src, wanted);
-        } else {
-            const uint16_t v = wanted ? *reinterpret_cast<const uint16_t *>(src) : (uint16_t)0;
-            asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(v) : "memory");
-        }
-    }
-}
 
 template <typename T, bool TRANS, bool LOADED>
 __global__ void __launch_bounds__(LOADED ? NTHREADS_LOADED : NTHREADS, 1)
@@ -108,7 +53,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
     unsigned char *epi = sp + (size_t)p.stages * stage_bytes;
     Groups gr;
     gr.start = reinterpret_cast<int *>(epi + EPI_BYTES);
-    gr.tiles = gr.start + p.G + 1;
+    gr.parts = gr.start + p.G + 1;
+    gr.split = nullptr;
     auto bar = [](const uint64_t &b) { return smem_u32(&b); };
 
     if (tid == 0) {
@@ -123,30 +69,18 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
         if (!LOADED) prefetch_map(&map_in);
         prefetch_map(&map_w);
     }
-    for (int g = tid; g <= p.G; g += blockDim.x) gr.start[g] = min(max(start[g], 0), p.n);
     if (warp == MMA_WARP) tmem_alloc(smem_u32(&tmem_slot), TMEM_COLS);
     fence_before();
-    __syncthreads();
+    read_groups(gr, start, p.G, p.n, BM);
     fence_after();
-    if (warp == 0) {                                        // row tiles before every group
-        int before = 0;
-        for (int g0 = 0; g0 < p.G; g0 += 32) {
-            const int g = g0 + lane;
-            const int t = g < p.G ? (max(gr.start[g + 1] - gr.start[g], 0) + BM - 1) / BM : 0;
-            int inc = t;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(QMLB_FULL_MASK, inc, o);
-                if (lane >= o) inc += v;
-            }
-            if (g < p.G) gr.tiles[g] = before + inc - t;
-            before += __shfl_sync(QMLB_FULL_MASK, inc, 31);
-        }
-        if (lane == 0) gr.tiles[p.G] = before;
-    }
-    __syncthreads();
     const uint32_t tmem = tmem_slot;
-    const int total = gr.tiles[p.G] * p.ntiles;
+    const int total = gr.parts[p.G] * p.ntiles;
+    auto locate = [&](int tile, int &g, int &row0, int &row1) {
+        const int mt = tile / p.ntiles;
+        g = gr.find(p.G, mt);
+        row0 = gr.start[g] + (mt - gr.parts[g]) * BM;
+        row1 = gr.start[g + 1];
+    };
     const volatile int *gave_up = &failed;
 
     if (warp == TMA_WARP) {
@@ -155,7 +89,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
             bool ok = true;
             for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
                 int g, row0, row1;
-                locate(gr, p.G, tile / p.ntiles, g, row0, row1);
+                locate(tile, g, row0, row1);
                 const int col0 = (tile % p.ntiles) * p.NT;
                 // forward: boxes of 64 columns by 64 deep, as many as reach into the matrix; transposed: one box of NT rows
                 const int boxes = TRANS ? 1 : min((p.NT + 63) / 64, (p.out - col0 + 63) / 64);
@@ -222,7 +156,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
         for (int tile = blockIdx.x; tile < total; tile += gridDim.x, ++j) {
             const int buf = j & 1;
             int g, row0, row1;
-            locate(gr, p.G, tile / p.ntiles, g, row0, row1);
+            locate(tile, g, row0, row1);
             const int col0 = (tile % p.ntiles) * p.NT, row = row0 + quarter * 32;
             const int rows = min(32, row1 - row);
             ok = ok && mbar_wait(bar(acc_full[buf]), (uint32_t)(j >> 1) & 1u, gave_up);
@@ -247,20 +181,11 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
 #pragma unroll
                     for (int u = 0; u < 64; ++u) v[u] = 0x7fc00000u;
                 }
-#pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    qmlb::Pack<T, 8> k;
-#pragma unroll
-                    for (int q = 0; q < 8; ++q) k.item[q] = qmlb::from_f32<T>(__uint_as_float(v[u * 8 + q]));
-                    *reinterpret_cast<uint4 *>(mine + lane * STAGE_ROW + u * 16) = k.word;
-                }
+                stage_row<T>(mine, lane, v);
                 __syncwarp();
                 const int bytes = min(min(64, left), p.out - col0 - c) * 2;
                 unsigned char *to = reinterpret_cast<unsigned char *>(out) + (size_t)row * row_bytes + (size_t)(col0 + c) * 2;
-                if (p.out_access == 16) store_rows<16>(mine, to, row_bytes, rows, bytes, lane);
-                else if (p.out_access == 8) store_rows<8>(mine, to, row_bytes, rows, bytes, lane);
-                else if (p.out_access == 4) store_rows<4>(mine, to, row_bytes, rows, bytes, lane);
-                else store_rows<2>(mine, to, row_bytes, rows, bytes, lane);
+                store_tile(mine, to, row_bytes, rows, bytes, lane, p.out_access);
                 __syncwarp();
             }
         }
@@ -278,15 +203,13 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
         };
         for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
             int g, row0, row1;
-            locate(gr, p.G, tile / p.ntiles, g, row0, row1);
+            locate(tile, g, row0, row1);
             for (int c = 0; c < p.nchunks; ++c, ++it) {
                 const int s = it % p.stages;
                 ok = __all_sync(QMLB_FULL_MASK, mbar_wait(bar(empty[s]), ((uint32_t)(it / p.stages) & 1u) ^ 1u, gave_up));
                 if (!ok) break;
                 const uint32_t a = sbase + (uint32_t)s * stage_bytes;
-                if (p.in_access >= 8) load_rows<8>(src, row_bytes, row0, p.n, c * BK * 2, a, t);
-                else if (p.in_access == 4) load_rows<4>(src, row_bytes, row0, p.n, c * BK * 2, a, t);
-                else load_rows<2>(src, row_bytes, row0, p.n, c * BK * 2, a, t);
+                load_box(src, row_bytes, row0, p.n, (size_t)c * BK * 2, a, BM, t, 128, p.in_access);
                 cp_async_commit();
                 if (it >= AHEAD) {
                     cp_async_wait<AHEAD>();

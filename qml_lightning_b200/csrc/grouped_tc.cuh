@@ -11,4 +11,9 @@ int grouped_tc(const void *x, const void *W, const int *start, int dtype, size_t
                void *workspace, cudaStream_t st);
 int grouped_tc_timeouts();
 
+size_t grouped_wgrad_tc_workspace(size_t n, int G, int K, int N);
+int grouped_wgrad_tc(const void *x, const void *dy, const int *start, int dtype, size_t n, int G, int K, int N, void *dW, void *workspace,
+                     cudaStream_t st);
+int grouped_wgrad_tc_timeouts();
+
 }  // namespace qmlb

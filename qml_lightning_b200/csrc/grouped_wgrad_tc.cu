@@ -1,0 +1,372 @@
+// Gradient of the matrices of a grouped product on the tensor cores (fp16 or bf16 rows, 32-bit sums):
+//
+//   dW[g] = sum over the rows r of group g of x[r]^T dy[r]
+//
+// The rows are the depth of the product, so both operands lie in memory with their lines (64 columns of one row) across
+// the depth; tcgen05.mma takes them that way and nothing is transposed.  A unit of work is one tile of 128 columns of x by
+// NT columns of dy over at most `split` rows of one group.  Groups of one part are finished by their unit; the parts of the
+// others go to scratch in 32 bits and a second kernel adds them in order, so the result never depends on scheduling.
+// The split is chosen on the host from sizes alone: about one unit per SM when the tiles are few, several when they are many.
+// It is at most 16,384 rows, because the tensor core truncates when it adds: 1,024 additions are off by 3e-5 on average, far
+// below the half step of the result.
+// Roles as in the forward product.  The last slice of a part may hold rows of the next group: the issuing warp overwrites
+// the lines up to the next multiple of 16 rows with zeros and leaves the other multiples out.
+#include "grouped_rows.cuh"
+#include "grouped_tc.cuh"
+
+#include <string.h>
+
+#include <type_traits>
+
+namespace {
+
+using namespace qmlb::tc;
+
+constexpr int BM = 128;
+constexpr uint32_t BOX = 8192;                   // 64 rows x 64 columns
+constexpr int TMA_WARP = 0, MMA_WARP = 1, EPI_WARP = 4, LOAD_WARP = 8, LOAD_WARPS = 8;
+constexpr int NTHREADS = 256, NTHREADS_LOADED = NTHREADS + LOAD_WARPS * 32;
+
+__device__ int g_timeouts = 0;
+
+struct Shape {
+    int n, G, K, N;
+    int split;               // rows per part
+    int ktiles, ntiles, NT;
+    int stages;
+    uint32_t b_boxes;        // boxes per stage of dy
+    int x_access, dy_access, out_access;
+};
+
+template <typename T, bool LOADED>
+__global__ void __launch_bounds__(LOADED ? NTHREADS_LOADED : NTHREADS, 1)
+wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_dy, const T *__restrict__ x,
+             const T *__restrict__ dy, const int *__restrict__ start, Shape p, T *__restrict__ dW, float *__restrict__ partial) {
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_free[2], done;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int failed;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    unsigned char *sp = smem_raw + (sbase - smem_u32(smem_raw));
+    const uint32_t stage_bytes = (2 + p.b_boxes) * BOX;
+    unsigned char *epi = sp + (size_t)p.stages * stage_bytes;
+    Groups gr;
+    gr.start = reinterpret_cast<int *>(epi + EPI_BYTES);
+    gr.parts = gr.start + p.G + 1;
+    gr.split = gr.parts + p.G + 1;
+    auto bar = [](const uint64_t &b) { return smem_u32(&b); };
+    const bool tma_x = !LOADED || p.x_access == 16, tma_dy = !LOADED || p.dy_access == 16;
+
+    if (tid == 0) {
+        for (int s = 0; s < p.stages; ++s) {
+            mbar_init(bar(full[s]), LOADED ? 1 + LOAD_WARPS : 1);
+            mbar_init(bar(empty[s]), 1);
+        }
+        for (int i = 0; i < 2; ++i) { mbar_init(bar(acc_full[i]), 1); mbar_init(bar(acc_free[i]), 4); }
+        mbar_init(bar(done), 1);
+        failed = 0;
+        mbar_init_fence();
+        if (tma_x) prefetch_map(&map_x);
+        if (tma_dy) prefetch_map(&map_dy);
+    }
+    if (warp == MMA_WARP) tmem_alloc(smem_u32(&tmem_slot), TMEM_COLS);
+    fence_before();
+    read_groups(gr, start, p.G, p.n, p.split);
+    fence_after();
+    const uint32_t tmem = tmem_slot;
+    const int tiles = p.ktiles * p.ntiles, total = gr.parts[p.G] * tiles;
+    const volatile int *gave_up = &failed;
+    // unit -> group, rows [r0, r1), first columns of x and dy
+    auto locate = [&](int unit, int &g, int &r0, int &r1, int &k0, int &n0) {
+        const int part = unit / tiles, tile = unit - part * tiles;
+        g = gr.find(p.G, part);
+        r0 = gr.start[g] + (part - gr.parts[g]) * p.split;
+        r1 = min(r0 + p.split, gr.start[g + 1]);
+        k0 = (tile / p.ntiles) * BM;
+        n0 = (tile % p.ntiles) * p.NT;
+    };
+
+    if (warp == TMA_WARP) {
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            for (int unit = blockIdx.x; unit < total && ok; unit += gridDim.x) {
+                int g, r0, r1, k0, n0;
+                locate(unit, g, r0, r1, k0, n0);
+                const int xb = min(2, (p.K - k0 + 63) / 64), db = min((p.NT + 63) / 64, (p.N - n0 + 63) / 64);
+                const uint32_t bytes = (uint32_t)((tma_x ? xb : 0) + (tma_dy ? db : 0)) * BOX;
+                for (int r = r0; r < r1; r += BK, ++it) {
+                    const int s = it % p.stages;
+                    if (!mbar_wait(bar(empty[s]), ((uint32_t)(it / p.stages) & 1u) ^ 1u, gave_up)) { ok = false; break; }
+                    const uint32_t a = sbase + (uint32_t)s * stage_bytes, b = a + 2 * BOX;
+                    if (bytes) mbar_expect_tx(bar(full[s]), bytes);
+                    else mbar_arrive(bar(full[s]));
+                    if (tma_x)
+                        for (int j = 0; j < xb; ++j) tma_2d(a + (uint32_t)j * BOX, &map_x, k0 + j * 64, r, bar(full[s]));
+                    if (tma_dy)
+                        for (int j = 0; j < db; ++j) tma_2d(b + (uint32_t)j * BOX, &map_dy, n0 + j * 64, r, bar(full[s]));
+                }
+            }
+            if (!ok) failed = 1;
+            for (int i = max(0, it - p.stages); i < it; ++i)          // no copy may be in flight when the block leaves
+                for (int tries = 0; tries < WAIT_LIMIT && !mbar_try(bar(full[i % p.stages]), (uint32_t)(i / p.stages) & 1u); ++tries) {}
+        }
+    } else if (warp == MMA_WARP) {
+        const uint32_t idesc = instr_desc(std::is_same<T, __nv_bfloat16>::value, true, true, BM, p.NT);
+        int it = 0, j = 0;
+        bool ok = true;
+        for (int unit = blockIdx.x; unit < total && ok; unit += gridDim.x, ++j) {
+            int g, r0, r1, k0, n0;
+            locate(unit, g, r0, r1, k0, n0);
+            const int buf = j & 1;
+            bool w = mbar_wait(bar(acc_free[buf]), ((uint32_t)(j >> 1) & 1u) ^ 1u, gave_up);
+            for (int r = r0; r < r1; r += BK, ++it) {
+                const int s = it % p.stages;
+                w = w && mbar_wait(bar(full[s]), (uint32_t)(it / p.stages) & 1u, gave_up);
+                if (!__all_sync(QMLB_FULL_MASK, w)) { ok = false; break; }
+                const uint32_t a = sbase + (uint32_t)s * stage_bytes;
+                const int valid = min(BK, r1 - r), steps = (valid + 15) >> 4;
+                if (valid & 15) {                                     // lines that belong to no row of this part
+                    unsigned char *st = sp + (size_t)s * stage_bytes;
+                    const int per_box = (steps * 16 - valid) * 8;
+                    for (int i = lane; i < per_box * (int)(2 + p.b_boxes); i += 32)
+                        *reinterpret_cast<uint4 *>(st + (size_t)(i / per_box) * BOX + (size_t)valid * 128 + (i % per_box) * 16) = make_uint4(0, 0, 0, 0);
+                    fence_async_smem();
+                    __syncwarp();
+                }
+                fence_after();
+                if (lane == 0) {
+                    const uint32_t al = desc_lo(a, BOX), bl = desc_lo(a + 2 * BOX, BOX);
+                    for (int k = 0; k < steps; ++k)
+                        mma_f16(tmem + (uint32_t)buf * BUF_COLS, al + k * 128u, DESC_HI_SW128, bl + k * 128u, DESC_HI_SW128, idesc, (r > r0 || k) ? 1u : 0u);
+                    mma_commit(bar(empty[s]));
+                    if (r + BK >= r1) mma_commit(bar(acc_full[buf]));
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok) failed = 1;
+        if (lane == 0) mma_commit(bar(done));
+        __syncwarp();
+        for (int tries = 0; tries < WAIT_LIMIT && !mbar_try(bar(done), 0u); ++tries) {}
+    } else if (warp >= EPI_WARP && warp < LOAD_WARP) {
+        const int quarter = warp & 3;
+        unsigned char *mine = epi + quarter * 32 * STAGE_ROW;
+        int j = 0;
+        bool ok = true;
+        for (int unit = blockIdx.x; unit < total; unit += gridDim.x, ++j) {
+            int g, r0, r1, k0, n0;
+            locate(unit, g, r0, r1, k0, n0);
+            const int buf = j & 1;
+            const size_t slot = (size_t)(gr.split[g] + unit / tiles - gr.parts[g]);      // of a part of a sum
+            const bool whole = gr.parts[g + 1] - gr.parts[g] == 1;
+            const int row = k0 + quarter * 32, rows = min(32, p.K - row);
+            ok = ok && mbar_wait(bar(acc_full[buf]), (uint32_t)(j >> 1) & 1u, gave_up);
+            ok = __all_sync(QMLB_FULL_MASK, ok);
+            if (!ok) failed = 1;
+            fence_after();
+            const uint32_t from = tmem + (uint32_t)buf * BUF_COLS + ((uint32_t)(quarter * 32) << 16);
+            for (int c = 0; c < p.NT; c += 64) {
+                uint32_t v[64];
+                const int left = min(p.NT - c, p.N - n0 - c);
+                if (ok) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        if (u * 16 < left) tmem_ld16(from + (uint32_t)(c + u * 16), v + u * 16);
+                    tmem_ld_wait();
+                    if (c + 64 >= p.NT) {
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bar(acc_free[buf]));
+                    }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 64; ++u) v[u] = 0x7fc00000u;
+                }
+                if (left <= 0) continue;
+                if (whole) {
+                    stage_row<T>(mine, lane, v);
+                    __syncwarp();
+                    const size_t row_bytes = (size_t)p.N * 2;
+                    unsigned char *to = reinterpret_cast<unsigned char *>(dW) + ((size_t)g * p.K + row) * row_bytes + (size_t)(n0 + c) * 2;
+                    store_tile(mine, to, row_bytes, rows, min(64, left) * 2, lane, p.out_access);
+                    __syncwarp();
+                } else {
+                    // part of a sum: 32 bits, [slot][K][ntiles * NT]
+                    const size_t row_bytes = (size_t)p.ntiles * p.NT * 4;
+                    unsigned char *to = reinterpret_cast<unsigned char *>(partial) + (slot * p.K + row) * row_bytes + (size_t)(n0 + c) * 4;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                        for (int u = 0; u < 8; ++u)
+                            *reinterpret_cast<uint4 *>(mine + lane * STAGE_ROW + u * 16) =
+                                make_uint4(v[h * 32 + u * 4], v[h * 32 + u * 4 + 1], v[h * 32 + u * 4 + 2], v[h * 32 + u * 4 + 3]);
+                        __syncwarp();
+                        // columns up to the tile's padding are written: the tile has room for them
+                        const int cols = min(32, p.NT - c - h * 32);
+                        if (cols > 0) store_rows<16>(mine, to + h * 128, row_bytes, rows, cols * 4, lane);
+                        __syncwarp();
+                    }
+                }
+            }
+        }
+    } else if (LOADED && warp >= LOAD_WARP) {
+        const int t = tid - LOAD_WARP * 32;
+        const unsigned char *xs = reinterpret_cast<const unsigned char *>(x), *ds = reinterpret_cast<const unsigned char *>(dy);
+        constexpr int AHEAD = 2;
+        int it = 0;
+        bool ok = true;
+        auto publish = [&](int i) {
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(full[i % p.stages]));
+        };
+        for (int unit = blockIdx.x; unit < total && ok; unit += gridDim.x) {
+            int g, r0, r1, k0, n0;
+            locate(unit, g, r0, r1, k0, n0);
+            const int xb = min(2, (p.K - k0 + 63) / 64), db = min((p.NT + 63) / 64, (p.N - n0 + 63) / 64);
+            for (int r = r0; r < r1; r += BK, ++it) {
+                const int s = it % p.stages;
+                ok = __all_sync(QMLB_FULL_MASK, mbar_wait(bar(empty[s]), ((uint32_t)(it / p.stages) & 1u) ^ 1u, gave_up));
+                if (!ok) break;
+                const uint32_t a = sbase + (uint32_t)s * stage_bytes, b = a + 2 * BOX;
+                if (!tma_x)
+                    for (int q = 0; q < xb; ++q)
+                        load_box(xs, (size_t)p.K * 2, r, r1, (size_t)(k0 + q * 64) * 2, a + (uint32_t)q * BOX, BK, t, LOAD_WARPS * 32, p.x_access);
+                if (!tma_dy)
+                    for (int q = 0; q < db; ++q)
+                        load_box(ds, (size_t)p.N * 2, r, r1, (size_t)(n0 + q * 64) * 2, b + (uint32_t)q * BOX, BK, t, LOAD_WARPS * 32, p.dy_access);
+                cp_async_commit();
+                if (it >= AHEAD) {
+                    cp_async_wait<AHEAD>();
+                    publish(it - AHEAD);
+                }
+            }
+        }
+        cp_async_wait<0>();
+        for (int i = max(0, it - AHEAD); i < it; ++i) publish(i);
+        if (!ok) failed = 1;
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (tid == 0 && failed) atomicAdd(&g_timeouts, 1);
+    if (warp == MMA_WARP) tmem_free(tmem, TMEM_COLS);
+}
+
+// Groups of several parts: their sum, in order.  Groups without rows: zeros.  blockIdx.y walks the groups.
+template <typename T>
+__global__ void __launch_bounds__(256)
+join_kernel(const int *__restrict__ start, const float *__restrict__ partial, Shape p, T *__restrict__ dW) {
+    extern __shared__ int sm[];
+    Groups gr;
+    gr.start = sm;
+    gr.parts = sm + p.G + 1;
+    gr.split = gr.parts + p.G + 1;
+    read_groups(gr, start, p.G, p.n, p.split);
+    const size_t row = (size_t)p.ntiles * p.NT;
+    for (int g = blockIdx.y; g < p.G; g += gridDim.y) {
+        const int parts = gr.parts[g + 1] - gr.parts[g];
+        if (parts == 1) continue;
+        const unsigned per_row = ((unsigned)p.N + 3u) / 4u;
+        for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < (size_t)p.K * per_row; i += (size_t)gridDim.x * 256) {
+            const unsigned k = (unsigned)(i / per_row), c = (unsigned)(i - (size_t)k * per_row) * 4u;
+            const float *src = partial + ((size_t)gr.split[g] * p.K + k) * row + c;
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+            for (int q = 0; q < parts; ++q) {
+                const float4 v = *reinterpret_cast<const float4 *>(src + (size_t)q * p.K * row);
+                s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
+            }
+            T *to = dW + ((size_t)g * p.K + k) * p.N + c;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (c + q < (unsigned)p.N) to[q] = qmlb::from_f32<T>(s[q]);
+        }
+    }
+}
+
+Shape make_shape(size_t n, int G, int K, int N) {
+    Shape p;
+    p.n = (int)n;
+    p.G = G;
+    p.K = K;
+    p.N = N;
+    const int nt = (N + 255) / 256;
+    p.NT = ((N + nt - 1) / nt + 15) / 16 * 16;
+    p.ntiles = (N + p.NT - 1) / p.NT;
+    p.ktiles = (K + BM - 1) / BM;
+    p.b_boxes = (uint32_t)((p.NT + 63) / 64);
+    // Rows per part.  Few tiles: (n / split + G) * tiles units, one for every SM, so that all end together; many: three or
+    // more units per SM.  No fewer than 256 rows: a part costs two passes over its tile in 32 bits.
+    const long tiles = (long)p.ktiles * p.ntiles, units = tiles * G;
+    const double sms = 148.0;
+    double split = units * 2 <= 148 ? (double)n * tiles / (sms - units) : (double)n * tiles / (sms * 3);
+    if (split < 256) split = 256;
+    if (split > 16384) split = 16384;
+    p.split = ((int)split + BK - 1) / BK * BK;
+    return p;
+}
+
+template <typename T>
+int run(const void *x, const void *dy, const int *start, size_t n, int G, int K, int N, void *dW, void *workspace, cudaStream_t st) {
+    const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+    Shape p = make_shape(n, G, K, N);
+    p.x_access = qmlb::access_bytes((size_t)K * 2, 2, x);
+    p.dy_access = qmlb::access_bytes((size_t)N * 2, 2, dy);
+    p.out_access = qmlb::access_bytes((size_t)N * 2, 2, dW);
+    const uint32_t stage = (2 + p.b_boxes) * BOX;
+    const size_t fixed = EPI_BYTES + (size_t)3 * (G + 1) * 4 + 1024;
+    p.stages = (int)((SMEM_LIMIT - fixed - 512) / stage);
+    if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+    const bool loaded = p.x_access < 16 || p.dy_access < 16;
+    CUtensorMap mx, md;
+    memset(&mx, 0, sizeof(mx));
+    memset(&md, 0, sizeof(md));
+    if (p.x_access == 16)
+        if (int rc = qmlb::encode_tiles(&mx, x, bf16, (uint64_t)K, (uint64_t)n, 0, (uint64_t)K * 2, BK, "qmlb_grouped_matmul_wgrad")) return rc;
+    if (p.dy_access == 16)
+        if (int rc = qmlb::encode_tiles(&md, dy, bf16, (uint64_t)N, (uint64_t)n, 0, (uint64_t)N * 2, BK, "qmlb_grouped_matmul_wgrad")) return rc;
+    const long units = ((long)(n / p.split) + G) * p.ktiles * p.ntiles;
+    const int blocks = (int)(units < 148 ? units : 148);
+    const size_t smem = fixed + (size_t)p.stages * stage;
+    float *partial = static_cast<float *>(workspace);
+    T *out = static_cast<T *>(dW);
+    if (loaded) {
+        if (int rc = qmlb::ensure_smem(wgrad_kernel<T, true>, smem, "qmlb_grouped_matmul_wgrad")) return rc;
+        wgrad_kernel<T, true><<<blocks, NTHREADS_LOADED, smem, st>>>(mx, md, static_cast<const T *>(x), static_cast<const T *>(dy), start, p, out, partial);
+    } else {
+        if (int rc = qmlb::ensure_smem(wgrad_kernel<T, false>, smem, "qmlb_grouped_matmul_wgrad")) return rc;
+        wgrad_kernel<T, false><<<blocks, NTHREADS, smem, st>>>(mx, md, static_cast<const T *>(x), static_cast<const T *>(dy), start, p, out, partial);
+    }
+    const size_t per = ((size_t)K * ((N + 3) / 4) + 255) / 256;
+    const size_t most = (size_t)(148 * 8 + G - 1) / G;           // most groups need nothing when there are many
+    join_kernel<T><<<dim3((unsigned)(per < most ? per : most), (unsigned)G), 256, (size_t)3 * (G + 1) * 4, st>>>(start, partial, p, out);
+    return qmlb::check_launch("qmlb_grouped_matmul_wgrad");
+}
+
+}  // namespace
+
+namespace qmlb {
+
+size_t grouped_wgrad_tc_workspace(size_t n, int G, int K, int N) {
+    const Shape p = make_shape(n, G, K, N);
+    // parts of groups of several parts: a group of r > split rows has at most 2 r / split
+    const size_t parts = n / p.split, slots = parts < (size_t)G ? 2 * parts : parts + G;
+    return slots * K * p.ntiles * p.NT * 4 + 256;
+}
+
+int grouped_wgrad_tc(const void *x, const void *dy, const int *start, int dtype, size_t n, int G, int K, int N, void *dW, void *workspace,
+                     cudaStream_t st) {
+    return dtype == QMLB_F16 ? run<__half>(x, dy, start, n, G, K, N, dW, workspace, st) : run<__nv_bfloat16>(x, dy, start, n, G, K, N, dW, workspace, st);
+}
+
+int grouped_wgrad_tc_timeouts() {
+    int v = -1;
+    if (cudaMemcpyFromSymbol(&v, g_timeouts, sizeof(int)) != cudaSuccess) return -1;
+    return v;
+}
+
+}  // namespace qmlb
