@@ -176,11 +176,13 @@ int run_wgrad(const void *x, const void *dy, const int *start, int G, int n, int
     return qmlb::check_launch("qmlb_grouped_matmul_wgrad");
 }
 
+bool few_rows(size_t n) { return n < 256; }
+
 }  // namespace
 
 extern "C" size_t qmlb_grouped_matmul_workspace_bytes(size_t n, int ngroups, int K, int N, int dtype, int transpose) {
-    (void)transpose;
-    if (n == 0 || ngroups <= 0 || K <= 0 || N <= 0 || dtype == QMLB_F32) return 256;
+    if (n == 0 || ngroups <= 0 || K <= 0 || N <= 0) return 256;
+    if (dtype == QMLB_F32) return few_rows(n) ? 256 : qmlb::grouped_pair_workspace(n, ngroups, K, N, transpose);
     return qmlb::grouped_tc_workspace(ngroups, K, N);
 }
 
@@ -193,15 +195,19 @@ extern "C" int qmlb_grouped_matmul(const void *x, const void *W, const int *grou
     QMLB_REQUIRE(n < ((size_t)1 << 31) - (1 << 20), "qmlb_grouped_matmul: too many rows");
     if (n == 0) return QMLB_OK;
     cudaStream_t st = qmlb::as_stream(stream);
-    if (dtype == QMLB_F32) return run_product<float>(x, W, group_start, ngroups, (int)n, K, N, transpose, out, st);
+    if (dtype == QMLB_F32 && few_rows(n)) return run_product<float>(x, W, group_start, ngroups, (int)n, K, N, transpose, out, st);
     QMLB_REQUIRE(workspace && workspace_bytes >= qmlb_grouped_matmul_workspace_bytes(n, ngroups, K, N, dtype, transpose),
                  "qmlb_grouped_matmul: workspace too small");
     QMLB_REQUIRE(((uintptr_t)workspace & 255) == 0, "qmlb_grouped_matmul: workspace must be 256-byte aligned");
+    if (dtype == QMLB_F32)
+        return qmlb::grouped_pair(static_cast<const float *>(x), static_cast<const float *>(W), group_start, n, ngroups, K, N, transpose,
+                                  static_cast<float *>(out), workspace, st);
     return qmlb::grouped_tc(x, W, group_start, dtype, n, ngroups, K, N, transpose, out, workspace, st);
 }
 
 extern "C" size_t qmlb_grouped_matmul_wgrad_workspace_bytes(size_t n, int ngroups, int K, int N, int dtype) {
-    if (n == 0 || ngroups <= 0 || K <= 0 || N <= 0 || dtype == QMLB_F32) return 256;
+    if (n == 0 || ngroups <= 0 || K <= 0 || N <= 0) return 256;
+    if (dtype == QMLB_F32) return few_rows(n) ? 256 : qmlb::grouped_wgrad_pair_workspace(n, ngroups, K, N);
     return qmlb::grouped_wgrad_tc_workspace(n, ngroups, K, N);
 }
 
@@ -218,9 +224,12 @@ extern "C" int qmlb_grouped_matmul_wgrad(const void *x, const void *dy, const in
         if (cudaMemsetAsync(dW, 0, (size_t)ngroups * K * N * es, st) != cudaSuccess) return qmlb::check_launch("qmlb_grouped_matmul_wgrad(memset)");
         return QMLB_OK;
     }
-    if (dtype == QMLB_F32) return run_wgrad<float>(x, dy, group_start, ngroups, (int)n, K, N, dW, st);
+    if (dtype == QMLB_F32 && few_rows(n)) return run_wgrad<float>(x, dy, group_start, ngroups, (int)n, K, N, dW, st);
     QMLB_REQUIRE(workspace && workspace_bytes >= qmlb_grouped_matmul_wgrad_workspace_bytes(n, ngroups, K, N, dtype),
                  "qmlb_grouped_matmul_wgrad: workspace too small");
     QMLB_REQUIRE(((uintptr_t)workspace & 255) == 0, "qmlb_grouped_matmul_wgrad: workspace must be 256-byte aligned");
+    if (dtype == QMLB_F32)
+        return qmlb::grouped_wgrad_pair(static_cast<const float *>(x), static_cast<const float *>(dy), group_start, n, ngroups, K, N,
+                                        static_cast<float *>(dW), workspace, st);
     return qmlb::grouped_wgrad_tc(x, dy, group_start, dtype, n, ngroups, K, N, dW, workspace, st);
 }

@@ -256,36 +256,44 @@ wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
     if (warp == MMA_WARP) tmem_free(tmem, TMEM_COLS);
 }
 
-// Groups of several parts: their sum, in order.  Groups without rows: zeros.  blockIdx.y walks the groups.
+// Groups of several parts: their sum, in order.  Groups without rows: zeros.  blockIdx.y walks the groups; `row` is the
+// row length of the parts.
 template <typename T>
 __global__ void __launch_bounds__(256)
-join_kernel(const int *__restrict__ start, const float *__restrict__ partial, Shape p, T *__restrict__ dW) {
+join_kernel(const int *__restrict__ start, const float *__restrict__ partial, int n, int G, int K, int N, int split, size_t row, T *__restrict__ dW) {
     extern __shared__ int sm[];
     Groups gr;
     gr.start = sm;
-    gr.parts = sm + p.G + 1;
-    gr.split = gr.parts + p.G + 1;
-    read_groups(gr, start, p.G, p.n, p.split);
-    const size_t row = (size_t)p.ntiles * p.NT;
-    for (int g = blockIdx.y; g < p.G; g += gridDim.y) {
+    gr.parts = sm + G + 1;
+    gr.split = gr.parts + G + 1;
+    read_groups(gr, start, G, n, split);
+    for (int g = blockIdx.y; g < G; g += gridDim.y) {
         const int parts = gr.parts[g + 1] - gr.parts[g];
         if (parts == 1) continue;
-        const unsigned per_row = ((unsigned)p.N + 3u) / 4u;
-        for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < (size_t)p.K * per_row; i += (size_t)gridDim.x * 256) {
+        const unsigned per_row = ((unsigned)N + 3u) / 4u;
+        for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < (size_t)K * per_row; i += (size_t)gridDim.x * 256) {
             const unsigned k = (unsigned)(i / per_row), c = (unsigned)(i - (size_t)k * per_row) * 4u;
-            const float *src = partial + ((size_t)gr.split[g] * p.K + k) * row + c;
+            const float *src = partial + ((size_t)gr.split[g] * K + k) * row + c;
             float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
             for (int q = 0; q < parts; ++q) {
-                const float4 v = *reinterpret_cast<const float4 *>(src + (size_t)q * p.K * row);
+                const float4 v = *reinterpret_cast<const float4 *>(src + (size_t)q * K * row);
                 s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
             }
-            T *to = dW + ((size_t)g * p.K + k) * p.N + c;
+            T *to = dW + ((size_t)g * K + k) * N + c;
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                if (c + q < (unsigned)p.N) to[q] = qmlb::from_f32<T>(s[q]);
+                if (c + q < (unsigned)N) to[q] = qmlb::from_f32<T>(s[q]);
         }
     }
+}
+
+template <typename T>
+int join(T *dW, const int *start, size_t n, int G, int K, int N, int split, size_t row, const float *partial, cudaStream_t st) {
+    const size_t per = ((size_t)K * ((N + 3) / 4) + 255) / 256, most = (size_t)(148 * 8 + G - 1) / G;   // most groups need nothing when there are many
+    join_kernel<T><<<dim3((unsigned)(per < most ? per : most), (unsigned)G), 256, (size_t)3 * (G + 1) * 4, st>>>(start, partial, (int)n, G, K, N,
+                                                                                                                split, row, dW);
+    return qmlb::check_launch("qmlb_grouped_matmul_wgrad");
 }
 
 Shape make_shape(size_t n, int G, int K, int N) {
@@ -299,14 +307,7 @@ Shape make_shape(size_t n, int G, int K, int N) {
     p.ntiles = (N + p.NT - 1) / p.NT;
     p.ktiles = (K + BM - 1) / BM;
     p.b_boxes = (uint32_t)((p.NT + 63) / 64);
-    // Rows per part.  Few tiles: (n / split + G) * tiles units, one for every SM, so that all end together; many: three or
-    // more units per SM.  No fewer than 256 rows: a part costs two passes over its tile in 32 bits.
-    const long tiles = (long)p.ktiles * p.ntiles, units = tiles * G;
-    const double sms = 148.0;
-    double split = units * 2 <= 148 ? (double)n * tiles / (sms - units) : (double)n * tiles / (sms * 3);
-    if (split < 256) split = 256;
-    if (split > 16384) split = 16384;
-    p.split = ((int)split + BK - 1) / BK * BK;
+    p.split = qmlb::wgrad_split(n, G, p.ktiles, p.ntiles);
     return p;
 }
 
@@ -341,21 +342,39 @@ int run(const void *x, const void *dy, const int *start, size_t n, int G, int K,
         if (int rc = qmlb::ensure_smem(wgrad_kernel<T, false>, smem, "qmlb_grouped_matmul_wgrad")) return rc;
         wgrad_kernel<T, false><<<blocks, NTHREADS, smem, st>>>(mx, md, static_cast<const T *>(x), static_cast<const T *>(dy), start, p, out, partial);
     }
-    const size_t per = ((size_t)K * ((N + 3) / 4) + 255) / 256;
-    const size_t most = (size_t)(148 * 8 + G - 1) / G;           // most groups need nothing when there are many
-    join_kernel<T><<<dim3((unsigned)(per < most ? per : most), (unsigned)G), 256, (size_t)3 * (G + 1) * 4, st>>>(start, partial, p, out);
-    return qmlb::check_launch("qmlb_grouped_matmul_wgrad");
+    return join<T>(out, start, n, G, K, N, p.split, (size_t)p.ntiles * p.NT, partial, st);
 }
 
 }  // namespace
 
 namespace qmlb {
 
+// Rows per part.  Few tiles: (n / split + G) * tiles units, one for every SM, so that all end together; many: three or more
+// units per SM.  No fewer than 256 rows: a part costs two passes over its tile in 32 bits.
+int wgrad_split(size_t n, int G, int ktiles, int ntiles) {
+    const long tiles = (long)ktiles * ntiles, units = tiles * G;
+    const double sms = 148.0;
+    double split = units * 2 <= 148 ? (double)n * tiles / (sms - units) : (double)n * tiles / (sms * 3);
+    if (split < 256) split = 256;
+    if (split > 16384) split = 16384;
+    return ((int)split + BK - 1) / BK * BK;
+}
+
+// parts of groups of several parts: a group of r > split rows has at most 2 r / split
+size_t wgrad_slots(size_t n, int G, int split) {
+    const size_t parts = n / split;
+    return parts < (size_t)G ? 2 * parts : parts + G;
+}
+
+int wgrad_join(void *dW, int dtype, const int *start, size_t n, int G, int K, int N, int split, int row, const float *partial, cudaStream_t st) {
+    if (dtype == QMLB_F32) return join<float>(static_cast<float *>(dW), start, n, G, K, N, split, (size_t)row, partial, st);
+    if (dtype == QMLB_F16) return join<__half>(static_cast<__half *>(dW), start, n, G, K, N, split, (size_t)row, partial, st);
+    return join<__nv_bfloat16>(static_cast<__nv_bfloat16 *>(dW), start, n, G, K, N, split, (size_t)row, partial, st);
+}
+
 size_t grouped_wgrad_tc_workspace(size_t n, int G, int K, int N) {
     const Shape p = make_shape(n, G, K, N);
-    // parts of groups of several parts: a group of r > split rows has at most 2 r / split
-    const size_t parts = n / p.split, slots = parts < (size_t)G ? 2 * parts : parts + G;
-    return slots * K * p.ntiles * p.NT * 4 + 256;
+    return wgrad_slots(n, G, p.split) * K * p.ntiles * p.NT * 4 + 256;
 }
 
 int grouped_wgrad_tc(const void *x, const void *dy, const int *start, int dtype, size_t n, int G, int K, int N, void *dW, void *workspace,

@@ -304,14 +304,15 @@ int rff_tc_timeouts();   // rff_tc.cu
 int pca_tc2_timeouts();  // pca_tc2.cu
 int grouped_tc_timeouts();  // grouped_tc.cu
 int grouped_wgrad_tc_timeouts();  // grouped_wgrad_tc.cu
+int grouped_pair_timeouts();  // grouped_pair_tc.cu
 }
 
 extern "C" int qmlb_tc_timeouts(void) {
     int v = -1;
     if (cudaMemcpyFromSymbol(&v, g_tc_timeouts, sizeof(int)) != cudaSuccess) return -1;
     const int w = qmlb::rff_tc_timeouts(), u = qmlb::pca_tc2_timeouts();
-    const int g = qmlb::grouped_tc_timeouts(), d = qmlb::grouped_wgrad_tc_timeouts();
-    return (w < 0 || u < 0 || g < 0 || d < 0) ? -1 : v + w + u + g + d;
+    const int g = qmlb::grouped_tc_timeouts(), d = qmlb::grouped_wgrad_tc_timeouts(), f = qmlb::grouped_pair_timeouts();
+    return (w < 0 || u < 0 || g < 0 || d < 0 || f < 0) ? -1 : v + w + u + g + d + f;
 }
 
 extern "C" int qmlb_pca_project_tc(const float *in, const float *reductors, const int *group_start, int nelements,

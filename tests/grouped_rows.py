@@ -2,7 +2,10 @@
 
 Bounds.  u = 2^-24 is the unit roundoff of float32, h = eps / 2 that of the result's type.  A float32 sum of m terms in any
 order, where every addition may also truncate (2 u instead of u), is off by at most 2 m u * sum|terms|; float32 operands
-that enter a product as three 16-bit parts lose at most 4 u of every product.  The result is rounded once (h of its value).
+that enter a product as two fp16 parts x = h + l + r have |l| <= 2^-11 |x| and |r| <= 2^-11 |l| <= 2^-22 |x| = 4 u |x|; the
+product h h' + h l' + l h' leaves out r x', x r' and l l', at most 3 * 2^-22 = 12 u of it.  (Parts below fp16's normal range are
+off by 2^-39 of the largest value of their 64-value stretch, which these inputs keep far below 12 u of the sum.)  The result
+is rounded once (h of its value).
 """
 import torch
 
@@ -48,7 +51,7 @@ def lookup_grad(indices, grad, rows, scale):
 
 def sum_bound(exact, magnitude, terms, dtype):
     tiny = torch.finfo(dtype).tiny * torch.finfo(dtype).eps
-    return magnitude * (2 * terms + 6) * U + exact.abs() * half_step(dtype) * 1.01 + tiny
+    return magnitude * (2 * terms + 14) * U + exact.abs() * half_step(dtype) * 1.01 + tiny
 
 
 def groups_of(start, n):
