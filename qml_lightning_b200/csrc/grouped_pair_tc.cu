@@ -9,16 +9,18 @@
 // the stretches in registers in 32 bits, rounded, undoing both scales on the way.  Against 64 bits the results are off by
 // about 2e-7 of their norm, like a float32 product, and rows and columns keep their own magnitudes.
 //
-// Work split.  One persistent block of 16 warps per SM takes tiles of 128 x NT (NT <= 256) results:
-//   warp 0     bulk copies of the matrix operand's images (products of rows; the images are made by a packing kernel)
-//   warp 1     issues tcgen05.mma, two tensor-memory accumulators in turn
-//   warps 2-3  zero rows outside the groups
-//   warps 4-7  load float32 rows, find the scales, split, and write the swizzled operand images to shared memory
-//   warps 8-15 add the finished accumulator to their 128 x 32 registers while the next one fills, and store the tile
-// Registers are moved from the first eight warps to the last eight (setmaxnreg), which hold 128 sums per thread.
-//
-// The gradient of the matrices is the same kernel with both operands loaded by warps 4-7: the depth runs over the rows of
-// the group, so the operands' lines run across it, and the stretches are 64 rows of one column.
+// Work split.  One persistent block per SM takes tiles of 128 x NT results:
+//   warp 0          bulk copies of the matrix operand's images (products of rows; a packing kernel makes the images)
+//   warp 1          issues tcgen05.mma, several tensor-memory accumulators in turn
+//   warps 2-3       zero rows outside the groups
+//   loading warps   load float32 rows, find the scales, split, and write the swizzled operand images to shared memory
+//   folding warps   (eight) add the finished accumulators to their registers, and store the tile
+// Products of rows: NT <= 256, 4 loading warps, 128 sums per folding thread.  Gradient of the matrices: both operands are loaded
+// by the loading warps (the depth runs over the rows of the group, the operands' lines run across it, the stretches are 64 rows
+// of one column), so their chains of loads, shuffles and conversions bound the kernel; NT <= 128 leaves registers for eight of
+// them, two per scheduler.  Measured on 210,000 x (336, 256): gradient 486 us with 4 and NT = 256, 368 us with 8 and NT = 128;
+// products of rows 182 us with 4 and NT = 256, 251 us with 8 and NT = 128 (there every row is split twice).
+// Registers are moved between the warps by setmaxnreg.
 #include <cuda_fp16.h>
 #include <string.h>
 
@@ -31,10 +33,22 @@ using namespace qmlb::tc;
 
 constexpr int BM = 128;
 constexpr uint32_t A_HALF = BM * BK * 2;          // one image (high or low parts) of the 128-wide operand
-constexpr int NTHREADS = 512;
-constexpr int TMA_WARP = 0, MMA_WARP = 1, LOAD_WARP = 4, FOLD_WARP = 8;
+constexpr int TMA_WARP = 0, MMA_WARP = 1, LOAD_WARP = 4;
 constexpr int MAXST = 4;
-constexpr uint32_t SCALE_FLOATS = 128 + 256;      // per chunk: scales of the rows and of the columns of the tile
+template <bool GRAD>
+struct Config {
+    static constexpr int LOADERS = GRAD ? 8 : 4, FOLD_WARP = LOAD_WARP + LOADERS, THREADS = (FOLD_WARP + 8) * 32;
+    static constexpr int NT = GRAD ? 128 : 256;   // widest tile
+    static constexpr int ACCS = 512 / NT;         // accumulators in tensor memory
+    // registers: launched with, then in the first warpgroup, the loading and the folding warps; their sum over the warpgroups
+    // does not exceed what the block was launched with
+    static constexpr int R_LAUNCH = GRAD ? 96 : 128, R_FIRST = 40, R_LOAD = 112, R_FOLD = GRAD ? 104 : 176;
+    static_assert(R_FIRST * 4 + R_LOAD * LOADERS + R_FOLD * 8 <= R_LAUNCH * (4 + LOADERS + 8), "register split");
+    // per chunk: inverse scales of the 128 rows and of the columns of the tile; gradient: also the factors by which the columns'
+    // units change with this chunk, and a flag per loading warp that says whether any does
+    static constexpr int RATIO = 128 + NT, FLAGS = RATIO + NT, SLOT = GRAD ? FLAGS + 8 : 128 + NT;
+};
+constexpr int AHEAD = 4;                          // stretches by which rows are asked into L2 in front of their loads
 constexpr uint32_t EPI = 8 * 2048;                // 32 rows x 16 columns per folding warp
 
 __device__ int g_timeouts = 0;
@@ -49,34 +63,42 @@ struct Shape {
     int a_access, b_access, out_access;
 };
 
-// power of two that takes `m` (bits of the largest magnitude) to [2^14, 2^15), and its inverse; both normal numbers
-__device__ __forceinline__ void scales(uint32_t m, float &s, float &inv) {
-    const int e = min(max(268 - (int)(m >> 23), 1), 253);
+// power of two that takes the largest magnitude `m` to [2^(top - 254), 2^(top - 253)), and its inverse; both normal numbers
+__device__ __forceinline__ void scales(float m, int top, float &s, float &inv) {
+    const int e = min(top - (int)(__float_as_uint(m) >> 23), 253);
     s = __uint_as_float((uint32_t)e << 23);
     inv = __uint_as_float((uint32_t)(254 - e) << 23);
 }
-__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-__device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
-    const __half2 h = __floats2half2_rn(a, b);
+// x s = h + l: high and low parts of two values
+__device__ __forceinline__ void split2(float2 x, float2 s, uint32_t &hi, uint32_t &lo) {
+    const __half2 h = __float22half2_rn(__fmul2_rn(x, s));
     const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    const __half2 l = __float22half2_rn(__ffma2_rn(x, s, make_float2(-f.x, -f.y)));      // exact: s is a power of two
     hi = *reinterpret_cast<const uint32_t *>(&h);
     lo = *reinterpret_cast<const uint32_t *>(&l);
 }
-// N consecutive floats of which `valid` exist
-template <int N>
-__device__ __forceinline__ void load_floats(const float *src, int valid, int access, float *v) {
-    if (valid >= N && access == 16) {
-#pragma unroll
-        for (int q = 0; q < N; q += 4) {
-            const float4 t = *reinterpret_cast<const float4 *>(src + q);
-            v[q] = t.x; v[q + 1] = t.y; v[q + 2] = t.z; v[q + 3] = t.w;
-        }
-    } else {
-#pragma unroll
-        for (int q = 0; q < N; ++q) v[q] = q < valid ? src[q] : 0.f;
-    }
+// Four consecutive floats, of which the first `valid` exist (the others become zeros).  Predicated loads without a branch: behind
+// a branch the compiler waits for each load before the next.
+__device__ __forceinline__ void load4(const float *src, bool wanted, float2 (&v)[2]) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "mov.f32 %0, 0f00000000;\n\tmov.f32 %1, 0f00000000;\n\tmov.f32 %2, 0f00000000;\n\tmov.f32 %3, 0f00000000;\n\t"
+        "@p ld.global.v4.f32 {%0, %1, %2, %3}, [%4];\n\t}"
+        : "=&f"(v[0].x), "=&f"(v[0].y), "=&f"(v[1].x), "=&f"(v[1].y)
+        : "l"(__cvta_generic_to_global(src)), "r"((int)wanted));
 }
+__device__ __forceinline__ void load1(const float *src, bool wanted, float &v) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.f32 %0, 0f00000000;\n\t@p ld.global.f32 %0, [%1];\n\t}"
+                 : "=&f"(v)
+                 : "l"(__cvta_generic_to_global(src)), "r"((int)wanted));
+}
+__device__ __forceinline__ void load4_narrow(const float *src, int valid, float2 (&v)[2]) {
+    load1(src, valid > 0, v[0].x);
+    load1(src + 1, valid > 1, v[0].y);
+    load1(src + 2, valid > 2, v[1].x);
+    load1(src + 3, valid > 3, v[1].y);
+}
+__device__ __forceinline__ void prefetch_l2(const void *src) { asm volatile("prefetch.global.L2 [%0];" ::"l"(__cvta_generic_to_global(src)) : "memory"); }
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                  "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(bar)
@@ -92,20 +114,22 @@ __device__ __forceinline__ void sts64(uint32_t at, uint32_t a, uint32_t b) {
 // Products of rows: a = x [n, K], packed/pack_scales = images of the matrices, result y [n, out].
 // GRAD: a = x [n, K], b = dy [n, out], result dW [G, K, out], partial = parts of split groups.
 template <bool GRAD>
-__global__ void __launch_bounds__(NTHREADS, 1)
+__global__ void __launch_bounds__(Config<GRAD>::THREADS, 1)
 pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, const unsigned char *__restrict__ packed,
             const float *__restrict__ pack_scales, const int *__restrict__ start, Shape p, float *__restrict__ out, float *__restrict__ partial) {
+    using C = Config<GRAD>;
+    constexpr int NACC = C::ACCS, NT_MAX = C::NT, FOLD_WARP = C::FOLD_WARP, SLOT = C::SLOT, RATIO = C::RATIO, FLAGS = C::FLAGS, HALF = C::NT / 2;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t full[MAXST], empty[MAXST], acc_full[2], acc_free[2], done;
+    __shared__ __align__(8) uint64_t full[MAXST], empty[MAXST], acc_full[NACC], acc_free[NACC], done;
     __shared__ uint32_t tmem_slot;
     __shared__ int failed;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
     unsigned char *sp = smem_raw + (sbase - smem_u32(smem_raw));
     const uint32_t stage_bytes = 2 * A_HALF + 2 * p.b_half;
-    const int slots = p.stages + 2;               // scales outlive their stage until the accumulator is folded
+    const int slots = p.stages + NACC + 1;        // scales outlive their stage until the accumulator is folded and stored
     float *scale = reinterpret_cast<float *>(sp + (size_t)p.stages * stage_bytes);
-    unsigned char *epi = reinterpret_cast<unsigned char *>(scale + (size_t)slots * SCALE_FLOATS);
+    unsigned char *epi = reinterpret_cast<unsigned char *>(scale + (size_t)slots * SLOT);
     Groups gr;
     gr.start = reinterpret_cast<int *>(epi + EPI);
     gr.parts = gr.start + p.G + 1;
@@ -114,10 +138,10 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
 
     if (tid == 0) {
         for (int s = 0; s < p.stages; ++s) {
-            mbar_init(bar(full[s]), GRAD ? 4 : 5);     // the four loading warps, and the issuer of the bulk copies
+            mbar_init(bar(full[s]), C::LOADERS + (GRAD ? 0 : 1));     // the loading warps, and the issuer of the bulk copies
             mbar_init(bar(empty[s]), 1);
         }
-        for (int i = 0; i < 2; ++i) { mbar_init(bar(acc_full[i]), 1); mbar_init(bar(acc_free[i]), 8); }
+        for (int i = 0; i < NACC; ++i) { mbar_init(bar(acc_full[i]), 1); mbar_init(bar(acc_free[i]), 8); }
         mbar_init(bar(done), 1);
         failed = 0;
         mbar_init_fence();
@@ -143,7 +167,7 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
     auto chunks_of = [&](int r0, int r1) { return GRAD ? (r1 - r0 + BK - 1) / BK : p.nchunks; };
 
     if (warp < LOAD_WARP) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::R_FIRST));
         if (warp == TMA_WARP) {
             if (!GRAD && lane == 0) {
                 int it = 0, slot = 0;
@@ -157,7 +181,7 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
                         if (!mbar_wait(bar(empty[s]), ((uint32_t)(it / p.stages) & 1u) ^ 1u, gave_up)) { ok = false; break; }
                         mbar_expect_tx(bar(full[s]), 2 * p.b_half + (uint32_t)p.NT * 4u);
                         bulk_copy(sbase + (uint32_t)s * stage_bytes + 2 * A_HALF, packed + (image + c) * (2 * p.b_half), 2 * p.b_half, bar(full[s]));
-                        bulk_copy(smem_u32(scale + (size_t)slot * SCALE_FLOATS + 128), pack_scales + (image + c) * p.NT, (uint32_t)p.NT * 4u, bar(full[s]));
+                        bulk_copy(smem_u32(scale + (size_t)slot * SLOT + 128), pack_scales + (image + c) * p.NT, (uint32_t)p.NT * 4u, bar(full[s]));
                         slot = slot + 1 == slots ? 0 : slot + 1;
                     }
                 }
@@ -175,20 +199,26 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
                 locate(unit, g, part, r0, r1, k0, nt);
                 const int chunks = chunks_of(r0, r1), depth = GRAD ? r1 - r0 : p.K;
                 for (int c = 0; c < chunks; ++c, ++it) {
-                    const int s = it % p.stages, buf = it & 1;
-                    bool w = mbar_wait(bar(acc_free[buf]), ((uint32_t)(it >> 1) & 1u) ^ 1u, gave_up);
+                    const int s = it % p.stages, buf = it % NACC;
+                    bool w = mbar_wait(bar(acc_free[buf]), ((uint32_t)(it / NACC) & 1u) ^ 1u, gave_up);
                     w = w && mbar_wait(bar(full[s]), (uint32_t)(it / p.stages) & 1u, gave_up);
                     if (!__all_sync(QMLB_FULL_MASK, w)) { ok = false; break; }
                     fence_after();
-                    if (lane == 0) {
-                        const int steps = min(BK / 16, (depth - c * BK + 15) / 16);
-                        const uint32_t a = sbase + (uint32_t)s * stage_bytes, b = a + 2 * A_HALF, d = tmem + (uint32_t)buf * BUF_COLS;
-                        const uint32_t ah = desc_lo(a, block), al = desc_lo(a + A_HALF, block), bh = desc_lo(b, block), bl = desc_lo(b + p.b_half, block);
-                        for (int k = 0; k < steps; ++k) {
+                    const int steps = min(BK / 16, (depth - c * BK + 15) / 16);
+                    const uint32_t a = sbase + (uint32_t)s * stage_bytes, b = a + 2 * A_HALF, d = tmem + (uint32_t)buf * NT_MAX;
+                    const uint32_t ah = desc_lo(a, block), al = desc_lo(a + A_HALF, block), bh = desc_lo(b, block), bl = desc_lo(b + p.b_half, block);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < BK / 16; ++k) {
+                            if (k >= steps) break;
                             mma_f16(d, ah + k * step, DESC_HI_SW128, bl + k * step, DESC_HI_SW128, idesc, k ? 1u : 0u);
                             mma_f16(d, al + k * step, DESC_HI_SW128, bh + k * step, DESC_HI_SW128, idesc, 1u);
                         }
-                        for (int k = 0; k < steps; ++k) mma_f16(d, ah + k * step, DESC_HI_SW128, bh + k * step, DESC_HI_SW128, idesc, 1u);
+#pragma unroll
+                        for (int k = 0; k < BK / 16; ++k) {
+                            if (k >= steps) break;
+                            mma_f16(d, ah + k * step, DESC_HI_SW128, bh + k * step, DESC_HI_SW128, idesc, 1u);
+                        }
                         mma_commit(bar(empty[s]));
                         mma_commit(bar(acc_full[buf]));
                     }
@@ -207,113 +237,236 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
             }
         }
     } else if (warp < FOLD_WARP) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+        if constexpr (C::R_LOAD < C::R_LAUNCH) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::R_LOAD));
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::R_LOAD));
         const int w = warp - LOAD_WARP;
-        int it = 0, slot = 0;
         bool ok = true;
         if (!GRAD) {
-            // a row is 8 lanes of 8 values; 8 passes of 4 rows per warp
+            // A row is 8 lanes of 8 values, a pass 4 rows per warp.  Two halves of 4 passes each: while one is split and stored,
+            // the loads of the other are in flight.
             const int lr = lane >> 3, kc = lane & 7;
-            for (int unit = blockIdx.x; unit < total && ok; unit += gridDim.x) {
+            float2 v[2][4][4];
+            int unit = blockIdx.x, c = 0, row = 0, end = 0;          // what is loaded next
+            auto place = [&]() {
                 int g, part, r0, r1, k0, nt;
-                locate(unit, g, part, r0, r1, k0, nt);
-                const int row = r0 + w * 32 + lr;
-                for (int c = 0; c < p.nchunks; ++c, ++it) {
-                    const int s = it % p.stages, k = c * BK + kc * 8, left = p.K - k;
-                    float v[8][8];
+                if (unit < total) {
+                    locate(unit, g, part, r0, r1, k0, nt);
+                    row = r0 + w * 32 + lr;
+                    end = r1;
+                }
+            };
+            auto fetch = [&](int h, float2 (&t)[4][4]) {
+                if (unit >= total) return;
+                const int k = c * BK + kc * 8, left = p.K - k;
+                const float *src = a_in + (size_t)(row + h * 16) * p.K + k;
+                if (p.a_access == 16) {                              // a depth that is a multiple of 4: all four exist, or none
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) load_floats<8>(a_in + (size_t)(row + i * 4) * p.K + k, row + i * 4 < r1 ? left : 0, p.a_access, v[i]);
-                    ok = __all_sync(QMLB_FULL_MASK, mbar_wait(bar(empty[s]), ((uint32_t)(it / p.stages) & 1u) ^ 1u, gave_up));
-                    if (!ok) break;
-                    const uint32_t a = sbase + (uint32_t)s * stage_bytes;
+                    for (int i = 0; i < 4; ++i) {
+                        const bool in = row + (h * 4 + i) * 4 < end;
+                        load4(src + (size_t)(i * 4) * p.K, in && left > 0, reinterpret_cast<float2(&)[2]>(t[i][0]));
+                        load4(src + (size_t)(i * 4) * p.K + 4, in && left > 4, reinterpret_cast<float2(&)[2]>(t[i][2]));
+                    }
+                } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        uint32_t m = 0;
+                    for (int i = 0; i < 4; ++i) {
+                        const int valid = row + (h * 4 + i) * 4 < end ? left : 0;
+                        load4_narrow(src + (size_t)(i * 4) * p.K, valid, reinterpret_cast<float2(&)[2]>(t[i][0]));
+                        load4_narrow(src + (size_t)(i * 4) * p.K + 4, valid - 4, reinterpret_cast<float2(&)[2]>(t[i][2]));
+                    }
+                }
+            };
+            auto next = [&]() {
+                if (++c == p.nchunks) {
+                    c = 0;
+                    unit += gridDim.x;
+                    place();
+                }
+            };
+            // Rows on their way into L2, AHEAD stretches in front: the registers hold too few loads in flight for the latency of
+            // the memory, but enough for that of the cache.
+            int pu = blockIdx.x, pc = 0, prow = 0, pend = 0;
+            auto pplace = [&]() {
+                int g, part, r0, k0, nt;
+                if (pu < total) {
+                    locate(pu, g, part, r0, pend, k0, nt);
+                    prow = r0 + w * 32 + lane;
+                }
+            };
+            auto prefetch = [&]() {
+                if (pu >= total) return;
+                if (prow < pend) {
+                    const float *src = a_in + (size_t)prow * p.K + pc * BK;
+                    prefetch_l2(src);
+                    if (pc * BK + 32 < p.K) prefetch_l2(src + 32);
+                }
+                if (++pc == p.nchunks) {
+                    pc = 0;
+                    pu += gridDim.x;
+                    pplace();
+                }
+            };
+            pplace();
+            for (int i = 0; i < AHEAD; ++i) prefetch();
+            place();
+            fetch(0, v[0]);
+            fetch(1, v[1]);
+            int s = 0, slot = 0;
+            uint32_t phase = 1;
+            while (unit < total) {
+                ok = __all_sync(QMLB_FULL_MASK, mbar_wait(bar(empty[s]), phase, gave_up));
+                if (!ok) break;
+                const uint32_t a = sbase + (uint32_t)s * stage_bytes;
+                auto put = [&](int h, const float2 (&t)[4][4]) {
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) m = max(m, magnitude(v[i][q]));
+                    for (int i = 0; i < 4; ++i) {
+                        float m = 0.f;
 #pragma unroll
-                        for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(QMLB_FULL_MASK, m, o));
+                        for (int q = 0; q < 4; ++q) m = fmaxf(m, fmaxf(fabsf(t[i][q].x), fabsf(t[i][q].y)));
+#pragma unroll
+                        for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(QMLB_FULL_MASK, m, o));
                         float sc, inv;
-                        scales(m, sc, inv);
-                        const int r = w * 32 + i * 4 + lr;
-                        if (kc == 0) scale[(size_t)slot * SCALE_FLOATS + r] = inv;
+                        scales(m, 268, sc, inv);
+                        const int r = w * 32 + (h * 4 + i) * 4 + lr;
+                        if (kc == 0) scale[(size_t)slot * SLOT + r] = inv;
                         uint32_t hi[4], lo[4];
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) split2(v[i][q * 2] * sc, v[i][q * 2 + 1] * sc, hi[q], lo[q]);
+                        for (int q = 0; q < 4; ++q) split2(t[i][q], make_float2(sc, sc), hi[q], lo[q]);
                         const uint32_t at = a + (uint32_t)r * 128u + ((uint32_t)(kc ^ (r & 7)) << 4);
                         sts128(at, hi);
                         sts128(at + A_HALF, lo);
                     }
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bar(full[s]));
-                    slot = slot + 1 == slots ? 0 : slot + 1;
-                }
+                };
+                prefetch();
+                put(0, v[0]);
+                next();
+                fetch(0, v[0]);
+                put(1, v[1]);
+                fetch(1, v[1]);
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(full[s]));
+                slot = slot + 1 == slots ? 0 : slot + 1;
+                if (++s == p.stages) { s = 0; phase ^= 1u; }
             }
         } else {
-            // slabs of 16 columns: 4 lanes of 4 columns, 8 lanes of rows, 8 rows each
-            const int cg = lane & 3, rr = lane >> 2;
-            for (int unit = blockIdx.x; unit < total && ok; unit += gridDim.x) {
-                int g, part, r0, r1, k0, nt;
-                locate(unit, g, part, r0, r1, k0, nt);
-                const int n0 = nt * p.NT, slabs = 8 + p.NT / 16;
-                for (int r = r0; r < r1; r += BK, ++it) {
-                    const int s = it % p.stages;
-                    float v[2][8][4];
-                    auto fetch = [&](int slab, float (&t)[8][4]) {
-                        const bool is_b = slab >= 8;
-                        const int col = (is_b ? n0 + (slab - 8) * 16 : k0 + slab * 16) + cg * 4, width = is_b ? p.out : p.K;
-                        const float *src = (is_b ? b_in : a_in) + (size_t)(r + rr) * width + col;
+            // Slabs of 16 columns: 4 lanes of 4 columns, 8 lanes of rows, 8 rows each.  A warp takes one slab of x and one of dy.
+            const int cg = lane & 3, rr = lane >> 2, col = w * 16 + cg * 4;
+            const bool has_b = w * 16 < p.NT;
+            float2 v[2][8][2];
+            struct Cursor { int unit, r, r1, k0, n0; };
+            auto place = [&](Cursor &u) {
+                if (u.unit >= total) return;
+                int g, part, nt;
+                locate(u.unit, g, part, u.r, u.r1, u.k0, nt);
+                u.n0 = nt * p.NT;
+            };
+            auto advance = [&](Cursor &u) {                           // true: another part begins
+                u.r += BK;
+                if (u.r < u.r1) return false;
+                u.unit += gridDim.x;
+                place(u);
+                return true;
+            };
+            auto fetch = [&](const Cursor &u, const float *in, int first, int width, int access, float2 (&t)[8][2]) {
+                if (u.unit >= total) return;
+                const int rows = u.r1 - u.r - rr;
+                const float *src = in + (size_t)(u.r + rr) * width + first + col;
+                if (access == 16) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            load_floats<4>(src + (size_t)(i * 8) * width, r + rr + i * 8 < r1 ? width - col : 0, is_b ? p.b_access : p.a_access, t[i]);
-                    };
-                    fetch(w, v[0]);
-                    ok = __all_sync(QMLB_FULL_MASK, mbar_wait(bar(empty[s]), ((uint32_t)(it / p.stages) & 1u) ^ 1u, gave_up));
-                    if (!ok) break;
-                    const uint32_t a = sbase + (uint32_t)s * stage_bytes;
-                    auto put = [&](int slab, const float (&t)[8][4]) {
-                        const bool is_b = slab >= 8;
-                        const int col = (is_b ? slab - 8 : slab) * 16 + cg * 4;          // within the tile
-                        float sc[4], inv[4];
+                    for (int i = 0; i < 8; ++i) load4(src + (size_t)(i * 8) * width, i * 8 < rows && first + col < width, t[i]);
+                } else {
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            uint32_t m = 0;
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) m = max(m, magnitude(t[i][q]));
-#pragma unroll
-                            for (int o = 4; o < 32; o <<= 1) m = max(m, __shfl_xor_sync(QMLB_FULL_MASK, m, o));
-                            scales(m, sc[q], inv[q]);
-                        }
-                        if (rr == 0)
-                            *reinterpret_cast<float4 *>(scale + (size_t)slot * SCALE_FLOATS + (is_b ? 128 : 0) + col) = make_float4(inv[0], inv[1], inv[2], inv[3]);
-                        const uint32_t base = a + (is_b ? 2 * A_HALF : 0) + (uint32_t)(col >> 6) * 8192u, half = is_b ? p.b_half : A_HALF;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            uint32_t h0, h1, l0, l1;
-                            split2(t[i][0] * sc[0], t[i][1] * sc[1], h0, l0);
-                            split2(t[i][2] * sc[2], t[i][3] * sc[3], h1, l1);
-                            const uint32_t at = base + (uint32_t)(rr + i * 8) * 128u + ((uint32_t)((col & 63) * 2) ^ ((uint32_t)rr << 4));
-                            sts64(at, h0, h1);
-                            sts64(at + half, l0, l1);
-                        }
-                    };
-                    for (int q = w; q < slabs; q += 8) {
-                        if (q + 4 < slabs) fetch(q + 4, v[1]);
-                        put(q, v[0]);
-                        if (q + 8 < slabs) fetch(q + 8, v[0]);
-                        if (q + 4 < slabs) put(q + 4, v[1]);
-                    }
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bar(full[s]));
-                    slot = slot + 1 == slots ? 0 : slot + 1;
+                    for (int i = 0; i < 8; ++i) load4_narrow(src + (size_t)(i * 8) * width, i * 8 < rows ? width - first - col : 0, t[i]);
                 }
+            };
+            Cursor at{(int)blockIdx.x, 0, 0, 0, 0};
+            place(at);
+            fetch(at, a_in, at.k0, p.K, p.a_access, v[0]);
+            if (has_b) fetch(at, b_in, at.n0, p.out, p.b_access, v[1]);
+            int s = 0, slot = 0;
+            uint32_t phase = 1;
+            bool first = true;
+            float unit_of[4] = {1.f, 1.f, 1.f, 1.f};                  // present scales of this thread's columns of dy
+            auto largest = [&](const float2 (&t)[8][2], float (&m)[4]) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) m[q] = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    m[0] = fmaxf(m[0], fabsf(t[i][0].x));
+                    m[1] = fmaxf(m[1], fabsf(t[i][0].y));
+                    m[2] = fmaxf(m[2], fabsf(t[i][1].x));
+                    m[3] = fmaxf(m[3], fabsf(t[i][1].y));
+                }
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) m[q] = fmaxf(m[q], __shfl_xor_sync(QMLB_FULL_MASK, m[q], o));
+            };
+            auto store = [&](const float2 (&t)[8][2], const float (&sc)[4], uint32_t to, uint32_t half) {
+                to += (uint32_t)(col >> 6) * 8192u + (uint32_t)rr * 128u + ((uint32_t)((col & 63) * 2) ^ ((uint32_t)rr << 4));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    uint32_t h0, h1, l0, l1;
+                    split2(t[i][0], make_float2(sc[0], sc[1]), h0, l0);
+                    split2(t[i][1], make_float2(sc[2], sc[3]), h1, l1);
+                    sts64(to + (uint32_t)i * 1024u, h0, h1);
+                    sts64(to + half + (uint32_t)i * 1024u, l0, l1);
+                }
+            };
+            while (at.unit < total) {
+                if (!(ok = __all_sync(QMLB_FULL_MASK, mbar_wait(bar(empty[s]), phase, gave_up)))) break;
+                const uint32_t stage = sbase + (uint32_t)s * stage_bytes;
+                float *mine = scale + (size_t)slot * SLOT;
+                Cursor next = at;
+                const bool begins = advance(next);
+                float m[4], sc[4], inv[4];
+                largest(v[0], m);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) scales(m[q], 268, sc[q], inv[q]);
+                if (rr == 0) *reinterpret_cast<float4 *>(mine + col) = make_float4(inv[0], inv[1], inv[2], inv[3]);
+                store(v[0], sc, stage, A_HALF);
+                fetch(next, a_in, next.k0, p.K, p.a_access, v[0]);
+                bool changed = false;
+                if (has_b) {
+                    // The sums of a column of dy are kept in its unit: the scale of the part's first stretch, with room for values up to
+                    // 32 times larger.  A stretch that needs more changes the unit, and the sums with it.
+                    float ratio[4];
+                    largest(v[1], m);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        float now, inverse;
+                        scales(m[q], 264, now, inverse);
+                        const float had = unit_of[q];
+                        const bool keep = !first && m[q] * had < 60000.f;
+                        ratio[q] = 1.f;
+                        if (!first && !keep) {
+                            ratio[q] = __uint_as_float((uint32_t)max((int)(__float_as_uint(now) >> 23) - (int)(__float_as_uint(had) >> 23) + 127, 0) << 23);
+                            changed = true;
+                        }
+                        unit_of[q] = keep ? had : now;
+                        inv[q] = __uint_as_float((254u << 23) - __float_as_uint(unit_of[q]));
+                    }
+                    if (rr == 0) {
+                        *reinterpret_cast<float4 *>(mine + 128 + col) = make_float4(inv[0], inv[1], inv[2], inv[3]);
+                        *reinterpret_cast<float4 *>(mine + RATIO + col) = make_float4(ratio[0], ratio[1], ratio[2], ratio[3]);
+                    }
+                    store(v[1], unit_of, stage + 2 * A_HALF, p.b_half);
+                    fetch(next, b_in, next.n0, p.out, p.b_access, v[1]);
+                }
+                changed = __any_sync(QMLB_FULL_MASK, changed);
+                if (lane == 0) mine[FLAGS + w] = changed ? 1.f : 0.f;
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(full[s]));
+                slot = slot + 1 == slots ? 0 : slot + 1;
+                if (++s == p.stages) { s = 0; phase ^= 1u; }
+                at = next;
+                first = begins;
             }
         }
         if (!ok) failed = 1;
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::R_FOLD));
         const int quarter = warp & 3, h = (warp - FOLD_WARP) >> 2, half = p.NT / 2;       // rows and columns of this warp
         unsigned char *mine = epi + (warp - FOLD_WARP) * 2048;
         const uint32_t lane_field = (uint32_t)(quarter * 32) << 16;
@@ -323,35 +476,46 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
             int g, part, r0, r1, k0, nt;
             locate(unit, g, part, r0, r1, k0, nt);
             const int chunks = chunks_of(r0, r1);
-            float acc[128];
+            float2 acc[HALF / 2];
 #pragma unroll
-            for (int i = 0; i < 128; ++i) acc[i] = 0.f;
+            for (int i = 0; i < HALF / 2; ++i) acc[i] = make_float2(0.f, 0.f);
             for (int c = 0; c < chunks && ok; ++c, ++it) {
-                const int buf = it & 1;
-                ok = __all_sync(QMLB_FULL_MASK, mbar_wait(bar(acc_full[buf]), (uint32_t)(it >> 1) & 1u, gave_up));
+                const int buf = it % NACC;
+                ok = __all_sync(QMLB_FULL_MASK, mbar_wait(bar(acc_full[buf]), (uint32_t)(it / NACC) & 1u, gave_up));
                 if (!ok) break;
                 fence_after();
-                const float *sc = scale + (size_t)slot * SCALE_FLOATS;
-                const float mine_scale = sc[quarter * 32 + lane];
-                const float *cols = sc + 128 + h * half;
-                const uint32_t from = tmem + (uint32_t)buf * BUF_COLS + lane_field + (uint32_t)(h * half);
+                const float *sc = scale + (size_t)slot * SLOT;
+                const float row_scale = sc[quarter * 32 + lane];
+                const float2 rs = make_float2(row_scale, row_scale);
+                bool changed = false;
+                if (GRAD) {
+                    const float4 f = *reinterpret_cast<const float4 *>(sc + FLAGS), e = *reinterpret_cast<const float4 *>(sc + FLAGS + 4);
+                    changed = f.x + f.y + f.z + f.w + e.x + e.y + e.z + e.w != 0.f;
+                }
+                if (GRAD && changed) {              // columns whose unit changes with this chunk
+                    const float *ratio = sc + RATIO + h * half;
 #pragma unroll
-                for (int cc = 0; cc < 128; cc += 8) {
+                    for (int cc = 0; cc < HALF; cc += 4) {
+                        if (cc < half) {
+                            const float4 f = *reinterpret_cast<const float4 *>(ratio + cc);
+                            acc[cc / 2] = __fmul2_rn(acc[cc / 2], make_float2(f.x, f.y));
+                            acc[cc / 2 + 1] = __fmul2_rn(acc[cc / 2 + 1], make_float2(f.z, f.w));
+                        }
+                    }
+                }
+                const uint32_t from = tmem + (uint32_t)buf * NT_MAX + lane_field + (uint32_t)(h * half);
+                // 16 columns at a time, the next 16 on their way from tensor memory meanwhile
+                uint32_t t[2][16];
+                tmem_ld16(from, t[0]);
+#pragma unroll
+                for (int cc = 0; cc < HALF; cc += 16) {
                     if (cc < half) {
-                        uint32_t t[8];
-                        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                                     : "=r"(t[0]), "=r"(t[1]), "=r"(t[2]), "=r"(t[3]), "=r"(t[4]), "=r"(t[5]), "=r"(t[6]), "=r"(t[7])
-                                     : "r"(from + (uint32_t)cc));
-                        const float4 f0 = *reinterpret_cast<const float4 *>(cols + cc), f1 = *reinterpret_cast<const float4 *>(cols + cc + 4);
                         tmem_ld_wait();
-                        acc[cc] = fmaf(__uint_as_float(t[0]), f0.x * mine_scale, acc[cc]);
-                        acc[cc + 1] = fmaf(__uint_as_float(t[1]), f0.y * mine_scale, acc[cc + 1]);
-                        acc[cc + 2] = fmaf(__uint_as_float(t[2]), f0.z * mine_scale, acc[cc + 2]);
-                        acc[cc + 3] = fmaf(__uint_as_float(t[3]), f0.w * mine_scale, acc[cc + 3]);
-                        acc[cc + 4] = fmaf(__uint_as_float(t[4]), f1.x * mine_scale, acc[cc + 4]);
-                        acc[cc + 5] = fmaf(__uint_as_float(t[5]), f1.y * mine_scale, acc[cc + 5]);
-                        acc[cc + 6] = fmaf(__uint_as_float(t[6]), f1.z * mine_scale, acc[cc + 6]);
-                        acc[cc + 7] = fmaf(__uint_as_float(t[7]), f1.w * mine_scale, acc[cc + 7]);
+                        if (cc + 16 < half) tmem_ld16(from + (uint32_t)cc + 16u, t[(cc / 16 + 1) & 1]);
+                        const uint32_t(&u)[16] = t[(cc / 16) & 1];
+#pragma unroll
+                        for (int q = 0; q < 8; ++q)
+                            acc[cc / 2 + q] = __ffma2_rn(make_float2(__uint_as_float(u[q * 2]), __uint_as_float(u[q * 2 + 1])), rs, acc[cc / 2 + q]);
                     }
                 }
                 fence_before();
@@ -362,8 +526,10 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
             if (!ok) {
                 failed = 1;                                     // at once: the other roles stop waiting
 #pragma unroll
-                for (int i = 0; i < 128; ++i) acc[i] = __int_as_float(0x7fc00000);
+                for (int i = 0; i < HALF / 2; ++i) acc[i] = make_float2(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
             }
+            // undo the columns' scales (of the last chunk; every chunk carries them)
+            const float *cols = scale + (size_t)(slot == 0 ? slots - 1 : slot - 1) * SLOT + 128 + h * half;
             // where the tile goes: rows of y, of dW, or of a part
             const int col0 = nt * p.NT + h * half;
             float *to;
@@ -392,28 +558,30 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
             }
             width = min(width, half);
 #pragma unroll
-            for (int cc = 0; cc < 128; cc += 16) {
+            for (int cc = 0; cc < HALF; cc += 16) {
                 if (cc < half) {
                     // 32 rows x 16 columns through shared memory: 64-byte pieces of rows
 #pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        *reinterpret_cast<float4 *>(mine + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) =
-                            make_float4(acc[cc + q * 4], acc[cc + q * 4 + 1], acc[cc + q * 4 + 2], acc[cc + q * 4 + 3]);
+                    for (int q = 0; q < 4; ++q) {
+                        const float4 f = *reinterpret_cast<const float4 *>(cols + cc + q * 4);
+                        const float2 lo = __fmul2_rn(acc[cc / 2 + q * 2], make_float2(f.x, f.y)), hi = __fmul2_rn(acc[cc / 2 + q * 2 + 1], make_float2(f.z, f.w));
+                        *reinterpret_cast<float4 *>(mine + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) = make_float4(lo.x, lo.y, hi.x, hi.y);
+                    }
                     __syncwarp();
-                    const int cols = min(16, width - cc);
+                    const int left = min(16, width - cc);
                     if (access == 16) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int r = i * 8 + (lane >> 2), q = lane & 3;
                             const float4 t = *reinterpret_cast<const float4 *>(mine + r * 64 + ((q ^ ((r >> 1) & 3)) << 4));
-                            if (r < rows && q * 4 < cols) *reinterpret_cast<float4 *>(to + (size_t)r * row_floats + cc + q * 4) = t;
+                            if (r < rows && q * 4 < left) *reinterpret_cast<float4 *>(to + (size_t)r * row_floats + cc + q * 4) = t;
                         }
                     } else {
 #pragma unroll 4
                         for (int i = 0; i < 16; ++i) {
                             const int r = i * 2 + (lane >> 4), q = lane & 15;
                             const float t = *reinterpret_cast<const float *>(mine + r * 64 + (((q >> 2) ^ ((r >> 1) & 3)) << 4) + (q & 3) * 4);
-                            if (r < rows && q < cols) to[(size_t)r * row_floats + cc + q] = t;
+                            if (r < rows && q < left) to[(size_t)r * row_floats + cc + q] = t;
                         }
                     }
                     __syncwarp();
@@ -430,58 +598,69 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
 }
 
 // Images of the matrices: per group, column tile and stretch of 64 along the depth NT lines of 64 high parts and NT lines of
-// low parts, swizzled as the kernel's shared memory wants them, and NT inverse scales.  One block: 64 columns of one stretch.
+// low parts, swizzled as the kernel's shared memory wants them, and NT inverse scales (one per column for the whole depth, so
+// that they are undone once per tile).  One block: 16 columns of one group, read twice (the second time from the cache).
 template <bool TRANS>
 __global__ void __launch_bounds__(256)
 pack_kernel(const float *__restrict__ W, Shape p, int N, unsigned char *__restrict__ packed, float *__restrict__ pack_scales) {
-    __shared__ uint32_t most[4][64];
-    const int g = blockIdx.z, c = blockIdx.x;
-    const int kq = TRANS ? threadIdx.x & 3 : threadIdx.x >> 6, cl = TRANS ? threadIdx.x >> 2 : threadIdx.x & 63;
-    const int col = blockIdx.y * 64 + cl;
+    __shared__ float most[16][17];
+    const int g = blockIdx.y;
+    // neighbouring threads read neighbouring addresses: along the columns, or along the depth of the transposed matrix
+    const int cl = TRANS ? threadIdx.x >> 4 : threadIdx.x & 15, kl = TRANS ? threadIdx.x & 15 : threadIdx.x >> 4;
+    const int col = blockIdx.x * 16 + cl;
     const float *Wg = W + (size_t)g * p.K * p.out;
-    float v[16];
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const int k = c * BK + kq * 16 + i;
-        v[i] = (col < p.out && k < p.K) ? (TRANS ? Wg[(size_t)col * N + k] : Wg[(size_t)k * N + col]) : 0.f;
-        m = max(m, magnitude(v[i]));
+    const float *base = TRANS ? Wg + (size_t)col * N : Wg + col;
+    const size_t step = TRANS ? 1 : (size_t)N;
+    float m = 0.f;
+    if (col < p.out) {
+#pragma unroll 8
+        for (int k = kl; k < p.K; k += 16) m = fmaxf(m, fabsf(base[(size_t)k * step]));
     }
-    most[kq][cl] = m;
+    most[cl][kl] = m;
     __syncthreads();
-    m = max(max(most[0][cl], most[1][cl]), max(most[2][cl], most[3][cl]));
-    if (col >= p.ntiles * p.NT) return;
-    float s, inv;
-    scales(m, s, inv);
-    const int tile = col / p.NT, in = col - tile * p.NT;
-    const size_t image = ((size_t)(g * p.ntiles + tile)) * p.nchunks + c;
-    if (kq == 0) pack_scales[image * p.NT + in] = inv;
-    unsigned char *line = packed + image * (2 * p.b_half) + (size_t)in * 128;
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
+    for (int i = 0; i < 16; ++i) m = fmaxf(m, most[cl][i]);
+    float s, inv;
+    scales(m, 268, s, inv);
+    const int tile = col / p.NT, in = col - tile * p.NT;               // the grid covers whole tiles
+    const size_t image = (size_t)(g * p.ntiles + tile) * p.nchunks;
+    for (int c0 = 0; c0 < p.nchunks; c0 += 2) {                        // two stretches: 16 threads of 8 values per column
+        const int c = c0 + (kl >> 3), k0 = c0 * BK + kl * 8;
+        if (c >= p.nchunks) continue;
+        float2 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i].x = (col < p.out && k0 + i * 2 < p.K) ? base[(size_t)(k0 + i * 2) * step] : 0.f;
+            v[i].y = (col < p.out && k0 + i * 2 + 1 < p.K) ? base[(size_t)(k0 + i * 2 + 1) * step] : 0.f;
+        }
         uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) split2(v[q * 8 + i * 2] * s, v[q * 8 + i * 2 + 1] * s, hi[i], lo[i]);
-        const int at = ((kq * 2 + q) ^ (in & 7)) << 4;
-        *reinterpret_cast<uint4 *>(line + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4 *>(line + p.b_half + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        for (int i = 0; i < 4; ++i) split2(v[i], make_float2(s, s), hi[i], lo[i]);
+        unsigned char *line = packed + (image + c) * (2 * p.b_half) + (size_t)in * 128 + (((kl & 7) ^ (in & 7)) << 4);
+        *reinterpret_cast<uint4 *>(line) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4 *>(line + p.b_half) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if ((kl & 7) == 0) pack_scales[(image + c) * p.NT + in] = inv;
     }
 }
 
-// shared memory of a block, or the largest column tile that fits
-size_t smem_of(const Shape &p, int arrays) {
-    return (size_t)p.stages * (2 * A_HALF + 2 * p.b_half) + (size_t)(p.stages + 2) * SCALE_FLOATS * 4 + EPI + (size_t)arrays * (p.G + 1) * 4 + 1024;
+template <bool GRAD>
+size_t smem_of(const Shape &p) {
+    using C = Config<GRAD>;
+    return (size_t)p.stages * (2 * A_HALF + 2 * p.b_half) + (size_t)(p.stages + C::ACCS + 1) * C::SLOT * 4 + EPI + (size_t)(GRAD ? 3 : 2) * (p.G + 1) * 4 + 1024;
 }
 
-void tile_columns(Shape &p, int out, bool grad, int arrays) {
-    for (int limit = 256;; limit -= 64) {                      // many groups leave less shared memory for the stages
-        const int nt = (out + limit - 1) / limit;
+// Columns per tile and stages.  Many groups leave less shared memory for the stages: then the tiles get narrower.
+template <bool GRAD>
+void tile_columns(Shape &p, int out) {
+    const size_t limit = SMEM_LIMIT - 512;
+    for (int widest = Config<GRAD>::NT;; widest -= 64) {
+        const int nt = (out + widest - 1) / widest;
         p.NT = ((out + nt - 1) / nt + 15) / 16 * 16;
         p.ntiles = (out + p.NT - 1) / p.NT;
-        p.b_half = grad ? (uint32_t)((p.NT + 63) / 64) * 8192u : (uint32_t)p.NT * 128u;
+        p.b_half = GRAD ? (uint32_t)((p.NT + 63) / 64) * 8192u : (uint32_t)p.NT * 128u;
         p.stages = MAXST;
-        while (p.stages > 2 && smem_of(p, arrays) > SMEM_LIMIT - 512) --p.stages;
-        if (smem_of(p, arrays) <= SMEM_LIMIT - 512 || limit == 64) return;
+        while (p.stages > 2 && smem_of<GRAD>(p) > limit) --p.stages;
+        if (smem_of<GRAD>(p) <= limit || widest == 64) return;
     }
 }
 
@@ -493,7 +672,7 @@ Shape product_shape(size_t n, int G, int K, int N, int transpose) {
     p.K = transpose ? N : K;
     p.out = transpose ? K : N;
     p.nchunks = (p.K + BK - 1) / BK;
-    tile_columns(p, p.out, false, 2);
+    tile_columns<false>(p, p.out);
     return p;
 }
 
@@ -515,13 +694,13 @@ int grouped_pair(const float *x, const float *W, const int *start, size_t n, int
     unsigned char *packed = static_cast<unsigned char *>(workspace);
     const size_t images = (size_t)G * p.ntiles * p.nchunks;
     float *pack_scales = reinterpret_cast<float *>(packed + images * (2 * p.b_half));
-    const dim3 pg((unsigned)p.nchunks, (unsigned)((p.ntiles * p.NT + 63) / 64), (unsigned)G);
+    const dim3 pg((unsigned)(p.ntiles * p.NT / 16), (unsigned)G);
     if (transpose) pack_kernel<true><<<pg, 256, 0, st>>>(W, p, N, packed, pack_scales);
     else pack_kernel<false><<<pg, 256, 0, st>>>(W, p, N, packed, pack_scales);
     const long units = ((long)((n + BM - 1) / BM) + G) * p.ntiles;
-    const size_t smem = smem_of(p, 2);
+    const size_t smem = smem_of<false>(p);
     if (int rc = ensure_smem(pair_kernel<false>, smem, "qmlb_grouped_matmul")) return rc;
-    pair_kernel<false><<<(unsigned)(units < 148 ? units : 148), NTHREADS, smem, st>>>(x, nullptr, packed, pack_scales, start, p, out, nullptr);
+    pair_kernel<false><<<(unsigned)(units < 148 ? units : 148), Config<false>::THREADS, smem, st>>>(x, nullptr, packed, pack_scales, start, p, out, nullptr);
     return check_launch("qmlb_grouped_matmul");
 }
 
@@ -533,17 +712,17 @@ int grouped_wgrad_pair(const float *x, const float *dy, const int *start, size_t
     p.G = G;
     p.K = K;
     p.out = N;
-    tile_columns(p, N, true, 3);
+    tile_columns<true>(p, N);
     p.ktiles = (K + BM - 1) / BM;
     p.split = wgrad_split(n, G, p.ktiles, p.ntiles);
     p.a_access = access_bytes((size_t)K * 4, 4, x);
     p.b_access = access_bytes((size_t)N * 4, 4, dy);
     p.out_access = access_bytes((size_t)N * 4, 4, dW);
     const long units = ((long)(n / p.split) + G) * p.ktiles * p.ntiles;
-    const size_t smem = smem_of(p, 3);
+    const size_t smem = smem_of<true>(p);
     float *partial = static_cast<float *>(workspace);
     if (int rc = ensure_smem(pair_kernel<true>, smem, "qmlb_grouped_matmul_wgrad")) return rc;
-    pair_kernel<true><<<(unsigned)(units < 148 ? units : 148), NTHREADS, smem, st>>>(x, dy, nullptr, nullptr, start, p, dW, partial);
+    pair_kernel<true><<<(unsigned)(units < 148 ? units : 148), Config<true>::THREADS, smem, st>>>(x, dy, nullptr, nullptr, start, p, dW, partial);
     return wgrad_join(dW, QMLB_F32, start, n, G, K, N, p.split, p.ntiles * p.NT, partial, st);
 }
 
@@ -551,7 +730,7 @@ size_t grouped_wgrad_pair_workspace(size_t n, int G, int K, int N) {
     Shape p;
     memset(&p, 0, sizeof(p));
     p.G = G;
-    tile_columns(p, N, true, 3);
+    tile_columns<true>(p, N);
     return wgrad_slots(n, G, wgrad_split(n, G, (K + BM - 1) / BM, p.ntiles)) * K * p.ntiles * p.NT * 4 + 256;
 }
 

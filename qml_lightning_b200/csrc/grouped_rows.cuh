@@ -91,30 +91,33 @@ __device__ __forceinline__ void stage_row(unsigned char *tile, int lane, const u
 }
 
 // LINES lines of 128 bytes (64 elements) of consecutive rows into a swizzled box, W bytes per access (2: through registers),
-// by `threads` threads.  Rows from `end` on and bytes behind the row's end become zeros.
-template <int W>
-__device__ __forceinline__ void load_lines(const unsigned char *in, size_t row_bytes, int row0, int end, size_t byte0, uint32_t dst, int lines, int t,
-                                           int threads) {
-    constexpr int PER_ROW = 128 / W;
+// by THREADS threads.  Rows from `end` on and bytes behind the row's end become zeros.
+template <int W, int LINES, int THREADS>
+__device__ __forceinline__ void load_lines(const unsigned char *in, size_t row_bytes, int row0, int end, size_t byte0, uint32_t dst, int t) {
+    constexpr int PER_ROW = 128 / W, ROWS = THREADS / PER_ROW;       // rows per round
+    static_assert(THREADS % PER_ROW == 0 && LINES % ROWS == 0, "whole rounds");
+    const int r0 = t / PER_ROW, c = (t % PER_ROW) * W;
+    const bool in_row = byte0 + c < row_bytes;
+    const unsigned char *src = in + (size_t)(row0 + r0) * row_bytes + byte0 + c;
 #pragma unroll 8
-    for (int i = t; i < lines * PER_ROW; i += threads) {
-        const int r = i / PER_ROW, c = (i % PER_ROW) * W;
-        const bool wanted = row0 + r < end && byte0 + c < row_bytes;
-        const unsigned char *src = wanted ? in + (size_t)(row0 + r) * row_bytes + byte0 + c : in;
+    for (int i = 0; i < LINES / ROWS; ++i) {
+        const int r = r0 + i * ROWS;
+        const bool wanted = in_row && row0 + r < end;
         const uint32_t to = dst + (uint32_t)r * 128u + ((uint32_t)c ^ ((uint32_t)(r & 7) << 4));      // the 128-byte swizzle
         if (W >= 4) {
-            cp_async<W >= 4 ? W : 4>(to, src, wanted);
+            cp_async<W >= 4 ? W : 4>(to, wanted ? src : in, wanted);
         } else {
             const uint16_t v = wanted ? *reinterpret_cast<const uint16_t *>(src) : (uint16_t)0;
             asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(v) : "memory");
         }
+        src += (size_t)ROWS * row_bytes;
     }
 }
-__device__ __forceinline__ void load_box(const unsigned char *in, size_t row_bytes, int row0, int end, size_t byte0, uint32_t dst, int lines, int t,
-                                         int threads, int access) {
-    if (access >= 8) load_lines<8>(in, row_bytes, row0, end, byte0, dst, lines, t, threads);
-    else if (access == 4) load_lines<4>(in, row_bytes, row0, end, byte0, dst, lines, t, threads);
-    else load_lines<2>(in, row_bytes, row0, end, byte0, dst, lines, t, threads);
+template <int LINES, int THREADS>
+__device__ __forceinline__ void load_box(const unsigned char *in, size_t row_bytes, int row0, int end, size_t byte0, uint32_t dst, int t, int access) {
+    if (access >= 8) load_lines<8, LINES, THREADS>(in, row_bytes, row0, end, byte0, dst, t);
+    else if (access == 4) load_lines<4, LINES, THREADS>(in, row_bytes, row0, end, byte0, dst, t);
+    else load_lines<2, LINES, THREADS>(in, row_bytes, row0, end, byte0, dst, t);
 }
 
 }  // namespace tc

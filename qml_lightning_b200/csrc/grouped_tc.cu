@@ -10,7 +10,7 @@
 // The matrices are read where they are: their rows run along N, which makes them an operand whose lines run along N in the
 // forward product and along K in the transposed one; the instruction takes both.  A row tile may reach over the end of its
 // group: those rows are read and multiplied (rows do not mix) and not stored.
-// Rows whose address is no multiple of 16 bytes (odd widths, offset views) cannot be fetched by TMA; then warps 8-11 bring
+// Rows whose address is no multiple of 16 bytes (odd widths, offset views) cannot be fetched by TMA; then warps 8-15 bring
 // them with cp.async of 8 or 4 bytes, or 2-byte loads, into the same swizzled stages.
 // Every wait is bounded; a block that gives up fills its remaining tiles with NaN and counts the event (qmlb_tc_timeouts).
 #include "grouped_tc.cuh"
@@ -24,8 +24,8 @@ using namespace qmlb::tc;
 
 constexpr int BM = 128;                          // rows per tile
 constexpr uint32_t A_BYTES = BM * BK * 2;
-constexpr int TMA_WARP = 0, MMA_WARP = 1, EPI_WARP = 4, LOAD_WARP = 8;
-constexpr int NTHREADS = 256, NTHREADS_LOADED = 384;
+constexpr int TMA_WARP = 0, MMA_WARP = 1, EPI_WARP = 4, LOAD_WARP = 8, LOAD_WARPS = 8;
+constexpr int NTHREADS = 256, NTHREADS_LOADED = NTHREADS + LOAD_WARPS * 32;
 
 __device__ int g_timeouts = 0;
 
@@ -59,7 +59,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
 
     if (tid == 0) {
         for (int s = 0; s < p.stages; ++s) {
-            mbar_init(bar(full[s]), LOADED ? 5 : 1);        // the TMA issuer, and the four loading warps
+            mbar_init(bar(full[s]), LOADED ? 1 + LOAD_WARPS : 1);        // the TMA issuer, and the loading warps
             mbar_init(bar(empty[s]), 1);
         }
         for (int i = 0; i < 2; ++i) { mbar_init(bar(acc_full[i]), 1); mbar_init(bar(acc_free[i]), 4); }
@@ -122,13 +122,13 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
                 w = w && mbar_wait(bar(full[s]), (uint32_t)(it / p.stages) & 1u, gave_up);
                 if (!__all_sync(QMLB_FULL_MASK, w)) { ok = false; break; }
                 fence_after();
-                if (lane == 0) {
-                    const uint32_t a = sbase + (uint32_t)s * stage_bytes;
-                    const uint32_t al = desc_lo(a, 16), bl = desc_lo(a + A_BYTES, TRANS ? 16 : 8192);
-                    constexpr uint32_t b_step = TRANS ? 2u : 128u;          // 16 deep: 32 bytes along the lines, or 16 lines
+                const uint32_t a = sbase + (uint32_t)s * stage_bytes, d = tmem + (uint32_t)buf * BUF_COLS;
+                const uint32_t al = desc_lo(a, 16), bl = desc_lo(a + A_BYTES, TRANS ? 16 : 8192);
+                constexpr uint32_t b_step = TRANS ? 2u : 128u;              // 16 deep: 32 bytes along the lines, or 16 lines
+                if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < BK / 16; ++k)
-                        mma_f16(tmem + (uint32_t)buf * BUF_COLS, al + k * 2u, DESC_HI_SW128, bl + k * b_step, DESC_HI_SW128, idesc, (c | k) ? 1u : 0u);
+                        mma_f16(d, al + k * 2u, DESC_HI_SW128, bl + k * b_step, DESC_HI_SW128, idesc, (c | k) ? 1u : 0u);
                     mma_commit(bar(empty[s]));
                     if (c == p.nchunks - 1) mma_commit(bar(acc_full[buf]));
                 }
@@ -209,7 +209,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
                 ok = __all_sync(QMLB_FULL_MASK, mbar_wait(bar(empty[s]), ((uint32_t)(it / p.stages) & 1u) ^ 1u, gave_up));
                 if (!ok) break;
                 const uint32_t a = sbase + (uint32_t)s * stage_bytes;
-                load_box(src, row_bytes, row0, p.n, (size_t)c * BK * 2, a, BM, t, 128, p.in_access);
+                load_box<BM, LOAD_WARPS * 32>(src, row_bytes, row0, p.n, (size_t)c * BK * 2, a, t, p.in_access);
                 cp_async_commit();
                 if (it >= AHEAD) {
                     cp_async_wait<AHEAD>();

@@ -6,8 +6,7 @@
 // the depth; tcgen05.mma takes them that way and nothing is transposed.  A unit of work is one tile of 128 columns of x by
 // NT columns of dy over at most `split` rows of one group.  Groups of one part are finished by their unit; the parts of the
 // others go to scratch in 32 bits and a second kernel adds them in order, so the result never depends on scheduling.
-// The split is chosen on the host from sizes alone: about one unit per SM when the tiles are few, several when they are many.
-// It is at most 16,384 rows, because the tensor core truncates when it adds: 1,024 additions are off by 3e-5 on average, far
+// The split is chosen on the host from sizes alone (wgrad_split).  It is at most 16,384 rows, because the tensor core truncates when it adds: 1,024 additions are off by 3e-5 on average, far
 // below the half step of the result.
 // Roles as in the forward product.  The last slice of a part may hold rows of the next group: the issuing warp overwrites
 // the lines up to the next multiple of 16 rows with zeros and leaves the other multiples out.
@@ -136,10 +135,13 @@ wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
                     __syncwarp();
                 }
                 fence_after();
-                if (lane == 0) {
-                    const uint32_t al = desc_lo(a, BOX), bl = desc_lo(a + 2 * BOX, BOX);
-                    for (int k = 0; k < steps; ++k)
-                        mma_f16(tmem + (uint32_t)buf * BUF_COLS, al + k * 128u, DESC_HI_SW128, bl + k * 128u, DESC_HI_SW128, idesc, (r > r0 || k) ? 1u : 0u);
+                const uint32_t al = desc_lo(a, BOX), bl = desc_lo(a + 2 * BOX, BOX), d = tmem + (uint32_t)buf * BUF_COLS;
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < BK / 16; ++k) {
+                        if (k >= steps) break;
+                        mma_f16(d, al + k * 128u, DESC_HI_SW128, bl + k * 128u, DESC_HI_SW128, idesc, (r > r0 || k) ? 1u : 0u);
+                    }
                     mma_commit(bar(empty[s]));
                     if (r + BK >= r1) mma_commit(bar(acc_full[buf]));
                 }
@@ -233,10 +235,10 @@ wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
                 const uint32_t a = sbase + (uint32_t)s * stage_bytes, b = a + 2 * BOX;
                 if (!tma_x)
                     for (int q = 0; q < xb; ++q)
-                        load_box(xs, (size_t)p.K * 2, r, r1, (size_t)(k0 + q * 64) * 2, a + (uint32_t)q * BOX, BK, t, LOAD_WARPS * 32, p.x_access);
+                        load_box<BK, LOAD_WARPS * 32>(xs, (size_t)p.K * 2, r, r1, (size_t)(k0 + q * 64) * 2, a + (uint32_t)q * BOX, t, p.x_access);
                 if (!tma_dy)
                     for (int q = 0; q < db; ++q)
-                        load_box(ds, (size_t)p.N * 2, r, r1, (size_t)(n0 + q * 64) * 2, b + (uint32_t)q * BOX, BK, t, LOAD_WARPS * 32, p.dy_access);
+                        load_box<BK, LOAD_WARPS * 32>(ds, (size_t)p.N * 2, r, r1, (size_t)(n0 + q * 64) * 2, b + (uint32_t)q * BOX, t, p.dy_access);
                 cp_async_commit();
                 if (it >= AHEAD) {
                     cp_async_wait<AHEAD>();
@@ -349,15 +351,18 @@ int run(const void *x, const void *dy, const int *start, size_t n, int G, int K,
 
 namespace qmlb {
 
-// Rows per part.  Few tiles: (n / split + G) * tiles units, one for every SM, so that all end together; many: three or more
-// units per SM.  No fewer than 256 rows: a part costs two passes over its tile in 32 bits.
+// Rows per part, for the shortest time of 148 SMs that take (n / split + G) * tiles units in turn.  Two bounds of that time, in
+// rows: whole rounds of units, and the even share plus one unit.  A unit costs its rows and about 384 more (its first loads, its
+// store, and a part's way through scratch).  Between 256 and 16,384 rows.
 int wgrad_split(size_t n, int G, int ktiles, int ntiles) {
-    const long tiles = (long)ktiles * ntiles, units = tiles * G;
-    const double sms = 148.0;
-    double split = units * 2 <= 148 ? (double)n * tiles / (sms - units) : (double)n * tiles / (sms * 3);
-    if (split < 256) split = 256;
-    if (split > 16384) split = 16384;
-    return ((int)split + BK - 1) / BK * BK;
+    const double tiles = (double)ktiles * ntiles, sms = 148.0, cost = 384.0;
+    double best = 0.0, least = -1.0;
+    for (double s = 256.0; s <= 16384.0; s *= 1.1892071) {          // four steps per doubling
+        const double units = ((double)n / s + G) * tiles, rounds = (double)(long)((units + sms - 1) / sms);
+        const double whole = rounds * (s + cost), share = (n * tiles + units * cost) / sms + s, t = whole < share ? whole : share;
+        if (least < 0.0 || t < least) { least = t; best = s; }
+    }
+    return ((int)best + BK - 1) / BK * BK;
 }
 
 // parts of groups of several parts: a group of r > split rows has at most 2 r / split

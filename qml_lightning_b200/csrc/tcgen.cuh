@@ -55,6 +55,14 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap *map, int
 }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
+// One lane of a converged warp.  Unlike a test of the lane number this leaves the branch uniform for the compiler, which then
+// keeps descriptors in uniform registers: an instruction is issued every few cycles instead of every hundred.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
 // cp.async of BYTES (4, 8 or 16) bytes; a source that is not wanted is replaced by zeros and not read
 template <int BYTES>
 __device__ __forceinline__ void cp_async(uint32_t dst, const void *src, bool wanted) {
