@@ -48,6 +48,7 @@ struct Config {
     // units change with this chunk, and a flag per loading warp that says whether any does
     static constexpr int RATIO = 128 + NT, FLAGS = RATIO + NT, SLOT = GRAD ? FLAGS + 8 : 128 + NT;
 };
+constexpr int PART_COST = 384;                    // of a part of a sum through scratch, in rows
 constexpr int AHEAD = 4;                          // stretches by which rows are asked into L2 in front of their loads
 constexpr uint32_t EPI = 8 * 2048;                // 32 rows x 16 columns per folding warp
 
@@ -570,18 +571,26 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
                     __syncwarp();
                     const int left = min(16, width - cc);
                     if (access == 16) {
+                        float *at = to + (size_t)(lane >> 2) * row_floats + cc + (lane & 3) * 4;
+                        uint4 t[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const int r = i * 8 + (lane >> 2), q = lane & 3;
-                            const float4 t = *reinterpret_cast<const float4 *>(mine + r * 64 + ((q ^ ((r >> 1) & 3)) << 4));
-                            if (r < rows && q * 4 < left) *reinterpret_cast<float4 *>(to + (size_t)r * row_floats + cc + q * 4) = t;
+                            const int r = i * 8 + (lane >> 2);
+                            t[i] = *reinterpret_cast<const uint4 *>(mine + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            store_if(at, t[i], i * 8 + (lane >> 2) < rows && (lane & 3) * 4 < left);
+                            at += 8 * row_floats;
                         }
                     } else {
+                        float *at = to + (size_t)(lane >> 4) * row_floats + cc + (lane & 15);
 #pragma unroll 4
                         for (int i = 0; i < 16; ++i) {
                             const int r = i * 2 + (lane >> 4), q = lane & 15;
-                            const float t = *reinterpret_cast<const float *>(mine + r * 64 + (((q >> 2) ^ ((r >> 1) & 3)) << 4) + (q & 3) * 4);
-                            if (r < rows && q < left) to[(size_t)r * row_floats + cc + q] = t;
+                            const uint32_t t = *reinterpret_cast<const uint32_t *>(mine + r * 64 + (((q >> 2) ^ ((r >> 1) & 3)) << 4) + (q & 3) * 4);
+                            store_if(at, t, r < rows && q < left);
+                            at += 2 * row_floats;
                         }
                     }
                     __syncwarp();
@@ -714,7 +723,7 @@ int grouped_wgrad_pair(const float *x, const float *dy, const int *start, size_t
     p.out = N;
     tile_columns<true>(p, N);
     p.ktiles = (K + BM - 1) / BM;
-    p.split = wgrad_split(n, G, p.ktiles, p.ntiles);
+    p.split = wgrad_split(n, G, p.ktiles, p.ntiles, PART_COST);
     p.a_access = access_bytes((size_t)K * 4, 4, x);
     p.b_access = access_bytes((size_t)N * 4, 4, dy);
     p.out_access = access_bytes((size_t)N * 4, 4, dW);
@@ -731,7 +740,7 @@ size_t grouped_wgrad_pair_workspace(size_t n, int G, int K, int N) {
     memset(&p, 0, sizeof(p));
     p.G = G;
     tile_columns<true>(p, N);
-    return wgrad_slots(n, G, wgrad_split(n, G, (K + BM - 1) / BM, p.ntiles)) * K * p.ntiles * p.NT * 4 + 256;
+    return wgrad_slots(n, G, wgrad_split(n, G, (K + BM - 1) / BM, p.ntiles, PART_COST)) * K * p.ntiles * p.NT * 4 + 256;
 }
 
 int grouped_pair_timeouts() {

@@ -59,16 +59,49 @@ __device__ __forceinline__ void read_groups(const Groups &s, const int *__restri
     __syncthreads();
 }
 
+// Predicated global stores: without a branch the loads in front of them are issued together.
+__device__ __forceinline__ void store_if(void *p, uint4 v, bool wanted) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t@p st.global.v4.b32 [%0], {%1, %2, %3, %4};\n\t}" ::"l"(__cvta_generic_to_global(p)),
+                 "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w), "r"((int)wanted)
+                 : "memory");
+}
+__device__ __forceinline__ void store_if(void *p, uint2 v, bool wanted) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\t@p st.global.v2.b32 [%0], {%1, %2};\n\t}" ::"l"(__cvta_generic_to_global(p)), "r"(v.x),
+                 "r"(v.y), "r"((int)wanted)
+                 : "memory");
+}
+__device__ __forceinline__ void store_if(void *p, uint32_t v, bool wanted) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p st.global.b32 [%0], %1;\n\t}" ::"l"(__cvta_generic_to_global(p)), "r"(v), "r"((int)wanted)
+                 : "memory");
+}
+__device__ __forceinline__ void store_if(void *p, uint16_t v, bool wanted) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p st.global.b16 [%0], %1;\n\t}" ::"l"(__cvta_generic_to_global(p)), "h"(v), "r"((int)wanted)
+                 : "memory");
+}
+
 // Store one warp's tile (32 rows of up to 128 bytes) from shared memory, W bytes per access.
 template <int W>
 __device__ __forceinline__ void store_rows(const unsigned char *tile, unsigned char *out, size_t row_bytes, int rows, int bytes, int lane) {
-    constexpr int PER_ROW = 128 / W;
-#pragma unroll 4
-    for (int i = lane; i < 32 * PER_ROW; i += 32) {
-        const int r = i / PER_ROW, c = (i % PER_ROW) * W;
-        if (r < rows && c < bytes)
-            *reinterpret_cast<typename Word<W>::type *>(out + (size_t)r * row_bytes + c) =
-                *reinterpret_cast<const typename Word<W>::type *>(tile + r * STAGE_ROW + c);
+    constexpr int PER_ROW = 128 / W;                                 // accesses per row
+    constexpr int LANES = PER_ROW < 32 ? PER_ROW : 32, ROWS = 32 / LANES, ACROSS = PER_ROW / LANES, BATCH = 8;
+    using V = typename Word<W>::type;
+    const int r0 = lane / LANES, c0 = (lane % LANES) * W;
+#pragma unroll
+    for (int a = 0; a < ACROSS; ++a) {
+        const int c = c0 + a * LANES * W;
+        unsigned char *to = out + (size_t)r0 * row_bytes + c;
+        const unsigned char *from = tile + r0 * STAGE_ROW + c;
+#pragma unroll 1
+        for (int b = 0; b < 32 / ROWS; b += BATCH) {
+            V t[BATCH];
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) t[i] = *reinterpret_cast<const V *>(from + (size_t)((b + i) * ROWS) * STAGE_ROW);
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                store_if(to, t[i], r0 + (b + i) * ROWS < rows && c < bytes);
+                to += (size_t)ROWS * row_bytes;
+            }
+        }
     }
 }
 __device__ __forceinline__ void store_tile(const unsigned char *tile, unsigned char *out, size_t row_bytes, int rows, int bytes, int lane, int access) {

@@ -25,7 +25,7 @@ int grouped_wgrad_pair(const float *x, const float *dy, const int *start, size_t
 int grouped_pair_timeouts();
 
 // sums over rows in parts: rows per part, parts that go to scratch, and their sum
-int wgrad_split(size_t n, int G, int ktiles, int ntiles);
+int wgrad_split(size_t n, int G, int ktiles, int ntiles, int part_cost);
 size_t wgrad_slots(size_t n, int G, int split);
 int wgrad_join(void *dW, int dtype, const int *start, size_t n, int G, int K, int N, int split, int row, const float *partial, cudaStream_t st);
 

@@ -309,7 +309,7 @@ Shape make_shape(size_t n, int G, int K, int N) {
     p.ntiles = (N + p.NT - 1) / p.NT;
     p.ktiles = (K + BM - 1) / BM;
     p.b_boxes = (uint32_t)((p.NT + 63) / 64);
-    p.split = qmlb::wgrad_split(n, G, p.ktiles, p.ntiles);
+    p.split = qmlb::wgrad_split(n, G, p.ktiles, p.ntiles, 1536);
     return p;
 }
 
@@ -352,13 +352,15 @@ int run(const void *x, const void *dy, const int *start, size_t n, int G, int K,
 namespace qmlb {
 
 // Rows per part, for the shortest time of 148 SMs that take (n / split + G) * tiles units in turn.  Two bounds of that time, in
-// rows: whole rounds of units, and the even share plus one unit.  A unit costs its rows and about 384 more (its first loads, its
-// store, and a part's way through scratch).  Between 256 and 16,384 rows.
-int wgrad_split(size_t n, int G, int ktiles, int ntiles) {
-    const double tiles = (double)ktiles * ntiles, sms = 148.0, cost = 384.0;
+// rows: whole rounds of units, and the even share plus one unit.  A unit costs its rows, 256 more for its first loads and its
+// store, and `part_cost` more when it is a part of a group and goes through scratch in 32 bits (groups have n / G rows on
+// average).  Between 256 and 16,384 rows.
+int wgrad_split(size_t n, int G, int ktiles, int ntiles, int part_cost) {
+    const double tiles = (double)ktiles * ntiles, sms = 148.0;
     double best = 0.0, least = -1.0;
     for (double s = 256.0; s <= 16384.0; s *= 1.1892071) {          // four steps per doubling
-        const double units = ((double)n / s + G) * tiles, rounds = (double)(long)((units + sms - 1) / sms);
+        const double units = ((double)n / s + G) * tiles, rounds = (double)(long)((units + sms - 1) / sms), parts = (double)n / (G * s);
+        const double cost = 256.0 + part_cost * (parts < 1.0 ? parts : 1.0);
         const double whole = rounds * (s + cost), share = (n * tiles + units * cost) / sms + s, t = whole < share ? whole : share;
         if (least < 0.0 || t < least) { least = t; best = s; }
     }
