@@ -10,8 +10,9 @@ namespace tc {
 
 constexpr int BK = 64;                           // depth per stage: one 128-byte line of 16-bit elements
 constexpr int MAX_STAGES = 8;
-constexpr int STAGE_ROW = 144;                   // bytes per row of a warp's epilogue tile: 128 bytes, padded against bank conflicts
-constexpr uint32_t EPI_BYTES = 4 * 32 * STAGE_ROW;
+constexpr int EPI_WARPS = 8;                     // warps that drain an accumulator: two per quarter of its rows
+constexpr int EPI_TILE = 2048;                   // a warp's epilogue tile: 32 rows of 64 bytes
+constexpr uint32_t EPI_BYTES = EPI_WARPS * EPI_TILE;
 constexpr uint32_t TMEM_COLS = 512, BUF_COLS = 256;
 constexpr size_t SMEM_LIMIT = 227 * 1024;
 
@@ -79,28 +80,26 @@ __device__ __forceinline__ void store_if(void *p, uint16_t v, bool wanted) {
                  : "memory");
 }
 
-// Store one warp's tile (32 rows of up to 128 bytes) from shared memory, W bytes per access.
+// Byte `c` of row `r` in a warp's epilogue tile: 16-byte pieces in an order that changes every two rows, so that neither the
+// writes by rows nor the reads along rows collide in the banks.
+__device__ __forceinline__ int tile_at(int r, int c) { return r * 64 + (((c >> 4) ^ ((r >> 1) & 3)) << 4) + (c & 15); }
+
+// Store one warp's tile (32 rows of up to 64 bytes) from shared memory, W bytes per access.
 template <int W>
 __device__ __forceinline__ void store_rows(const unsigned char *tile, unsigned char *out, size_t row_bytes, int rows, int bytes, int lane) {
-    constexpr int PER_ROW = 128 / W;                                 // accesses per row
-    constexpr int LANES = PER_ROW < 32 ? PER_ROW : 32, ROWS = 32 / LANES, ACROSS = PER_ROW / LANES, BATCH = 8;
+    constexpr int LANES = 64 / W, ROWS = 32 / LANES, BATCH = 32 / ROWS < 8 ? 32 / ROWS : 8;      // lanes per row, rows per access
     using V = typename Word<W>::type;
-    const int r0 = lane / LANES, c0 = (lane % LANES) * W;
-#pragma unroll
-    for (int a = 0; a < ACROSS; ++a) {
-        const int c = c0 + a * LANES * W;
-        unsigned char *to = out + (size_t)r0 * row_bytes + c;
-        const unsigned char *from = tile + r0 * STAGE_ROW + c;
+    const int r0 = lane / LANES, c = (lane % LANES) * W;
+    unsigned char *to = out + (size_t)r0 * row_bytes + c;
 #pragma unroll 1
-        for (int b = 0; b < 32 / ROWS; b += BATCH) {
-            V t[BATCH];
+    for (int b = 0; b < 32 / ROWS; b += BATCH) {
+        V t[BATCH];
 #pragma unroll
-            for (int i = 0; i < BATCH; ++i) t[i] = *reinterpret_cast<const V *>(from + (size_t)((b + i) * ROWS) * STAGE_ROW);
+        for (int i = 0; i < BATCH; ++i) t[i] = *reinterpret_cast<const V *>(tile + tile_at(r0 + (b + i) * ROWS, c));
 #pragma unroll
-            for (int i = 0; i < BATCH; ++i) {
-                store_if(to, t[i], r0 + (b + i) * ROWS < rows && c < bytes);
-                to += (size_t)ROWS * row_bytes;
-            }
+        for (int i = 0; i < BATCH; ++i) {
+            store_if(to, t[i], r0 + (b + i) * ROWS < rows && c < bytes);
+            to += (size_t)ROWS * row_bytes;
         }
     }
 }
@@ -111,16 +110,22 @@ __device__ __forceinline__ void store_tile(const unsigned char *tile, unsigned c
     else store_rows<2>(tile, out, row_bytes, rows, bytes, lane);
 }
 
-// 32 registers of 64 accumulator columns of this thread's row -> result type -> the warp's tile
+// 32 accumulator columns of this thread's row, rounded to the result type, into the warp's tile
 template <typename T>
-__device__ __forceinline__ void stage_row(unsigned char *tile, int lane, const uint32_t (&v)[64]) {
+__device__ __forceinline__ void stage_row(unsigned char *tile, int lane, const uint32_t (&v)[32]) {
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
+    for (int u = 0; u < 4; ++u) {
         Pack<T, 8> k;
 #pragma unroll
         for (int q = 0; q < 8; ++q) k.item[q] = from_f32<T>(__uint_as_float(v[u * 8 + q]));
-        *reinterpret_cast<uint4 *>(tile + lane * STAGE_ROW + u * 16) = k.word;
+        *reinterpret_cast<uint4 *>(tile + tile_at(lane, u * 16)) = k.word;
     }
+}
+// 16 of them as they are
+__device__ __forceinline__ void stage_row_f32(unsigned char *tile, int lane, const uint32_t *v) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        *reinterpret_cast<uint4 *>(tile + tile_at(lane, u * 16)) = make_uint4(v[u * 4], v[u * 4 + 1], v[u * 4 + 2], v[u * 4 + 3]);
 }
 
 // LINES lines of 128 bytes (64 elements) of consecutive rows into a swizzled box, W bytes per access (2: through registers),

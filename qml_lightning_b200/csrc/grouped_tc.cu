@@ -4,13 +4,13 @@
 //
 // One persistent block per SM walks tiles of 128 rows of one group by NT columns, column tiles fastest so that the row
 // tile that neighbours share stays in L2.  Roles: warp 0 fetches 64-deep slices of both operands by TMA into a ring of
-// stages, warp 1 issues tcgen05.mma (M = 128, N = NT, K = 16) into one of two tensor-memory accumulators, warps 4-7 drain
-// the other one: 32 bits to the result type, through a padded shared-memory tile, out in whole 128-byte lines.  Warps 2-3
+// stages, warp 1 issues tcgen05.mma (M = 128, N = NT, K = 16) into one of two tensor-memory accumulators, warps 4-11 drain
+// the other one: 32 bits to the result type, through a padded shared-memory tile, out in pieces of 64 bytes.  Warps 2-3
 // write the zero rows outside the groups.
 // The matrices are read where they are: their rows run along N, which makes them an operand whose lines run along N in the
 // forward product and along K in the transposed one; the instruction takes both.  A row tile may reach over the end of its
 // group: those rows are read and multiplied (rows do not mix) and not stored.
-// Rows whose address is no multiple of 16 bytes (odd widths, offset views) cannot be fetched by TMA; then warps 8-15 bring
+// Rows whose address is no multiple of 16 bytes (odd widths, offset views) cannot be fetched by TMA; then warps 12-19 bring
 // them with cp.async of 8 or 4 bytes, or 2-byte loads, into the same swizzled stages.
 // Every wait is bounded; a block that gives up fills its remaining tiles with NaN and counts the event (qmlb_tc_timeouts).
 #include "grouped_tc.cuh"
@@ -24,8 +24,8 @@ using namespace qmlb::tc;
 
 constexpr int BM = 128;                          // rows per tile
 constexpr uint32_t A_BYTES = BM * BK * 2;
-constexpr int TMA_WARP = 0, MMA_WARP = 1, EPI_WARP = 4, LOAD_WARP = 8, LOAD_WARPS = 8;
-constexpr int NTHREADS = 256, NTHREADS_LOADED = NTHREADS + LOAD_WARPS * 32;
+constexpr int TMA_WARP = 0, MMA_WARP = 1, EPI_WARP = 4, LOAD_WARP = EPI_WARP + EPI_WARPS, LOAD_WARPS = 8;
+constexpr int NTHREADS = LOAD_WARP * 32, NTHREADS_LOADED = NTHREADS + LOAD_WARPS * 32;
 
 __device__ int g_timeouts = 0;
 
@@ -62,7 +62,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
             mbar_init(bar(full[s]), LOADED ? 1 + LOAD_WARPS : 1);        // the TMA issuer, and the loading warps
             mbar_init(bar(empty[s]), 1);
         }
-        for (int i = 0; i < 2; ++i) { mbar_init(bar(acc_full[i]), 1); mbar_init(bar(acc_free[i]), 4); }
+        for (int i = 0; i < 2; ++i) { mbar_init(bar(acc_full[i]), 1); mbar_init(bar(acc_free[i]), EPI_WARPS); }
         mbar_init(bar(done), 1);
         failed = 0;
         mbar_init_fence();
@@ -148,8 +148,9 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
             for (int c = lane; c < p.out; c += 32) row[c] = qmlb::from_f32<T>(0.f);
         }
     } else if (warp < LOAD_WARP) {
-        const int quarter = warp & 3;
-        unsigned char *mine = epi + quarter * 32 * STAGE_ROW;
+        // warps w and w + 4 share a quarter of the rows and take every other 32 columns
+        const int quarter = warp & 3, c_first = ((warp - EPI_WARP) >> 2) * 32;
+        unsigned char *mine = epi + (warp - EPI_WARP) * EPI_TILE;
         const size_t row_bytes = (size_t)p.out * 2;
         int j = 0;
         bool ok = true;
@@ -164,12 +165,16 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
             if (!ok) failed = 1;                                // at once: the other roles stop waiting
             fence_after();
             const uint32_t from = tmem + (uint32_t)buf * BUF_COLS + ((uint32_t)(quarter * 32) << 16);
-            for (int c = 0; c < p.NT; c += 64) {
-                uint32_t v[64];
+            if (ok && c_first >= p.NT) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(acc_free[buf]));
+            }
+            for (int c = c_first; c < p.NT; c += 64) {
+                uint32_t v[32];
                 const int left = p.NT - c;
                 if (ok) {
 #pragma unroll
-                    for (int u = 0; u < 4; ++u)
+                    for (int u = 0; u < 2; ++u)
                         if (u * 16 < left) tmem_ld16(from + (uint32_t)(c + u * 16), v + u * 16);
                     tmem_ld_wait();
                     if (c + 64 >= p.NT) {                       // the accumulator is free once it sits in registers
@@ -179,11 +184,11 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
                     }
                 } else {
 #pragma unroll
-                    for (int u = 0; u < 64; ++u) v[u] = 0x7fc00000u;
+                    for (int u = 0; u < 32; ++u) v[u] = 0x7fc00000u;
                 }
                 stage_row<T>(mine, lane, v);
                 __syncwarp();
-                const int bytes = min(min(64, left), p.out - col0 - c) * 2;
+                const int bytes = min(min(32, left), p.out - col0 - c) * 2;
                 unsigned char *to = reinterpret_cast<unsigned char *>(out) + (size_t)row * row_bytes + (size_t)(col0 + c) * 2;
                 store_tile(mine, to, row_bytes, rows, bytes, lane, p.out_access);
                 __syncwarp();

@@ -23,8 +23,8 @@ using namespace qmlb::tc;
 
 constexpr int BM = 128;
 constexpr uint32_t BOX = 8192;                   // 64 rows x 64 columns
-constexpr int TMA_WARP = 0, MMA_WARP = 1, EPI_WARP = 4, LOAD_WARP = 8, LOAD_WARPS = 8;
-constexpr int NTHREADS = 256, NTHREADS_LOADED = NTHREADS + LOAD_WARPS * 32;
+constexpr int TMA_WARP = 0, MMA_WARP = 1, EPI_WARP = 4, LOAD_WARP = EPI_WARP + EPI_WARPS, LOAD_WARPS = 8;
+constexpr int NTHREADS = LOAD_WARP * 32, NTHREADS_LOADED = NTHREADS + LOAD_WARPS * 32;
 
 __device__ int g_timeouts = 0;
 
@@ -62,7 +62,7 @@ wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
             mbar_init(bar(full[s]), LOADED ? 1 + LOAD_WARPS : 1);
             mbar_init(bar(empty[s]), 1);
         }
-        for (int i = 0; i < 2; ++i) { mbar_init(bar(acc_full[i]), 1); mbar_init(bar(acc_free[i]), 4); }
+        for (int i = 0; i < 2; ++i) { mbar_init(bar(acc_full[i]), 1); mbar_init(bar(acc_free[i]), EPI_WARPS); }
         mbar_init(bar(done), 1);
         failed = 0;
         mbar_init_fence();
@@ -153,8 +153,9 @@ wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
         __syncwarp();
         for (int tries = 0; tries < WAIT_LIMIT && !mbar_try(bar(done), 0u); ++tries) {}
     } else if (warp >= EPI_WARP && warp < LOAD_WARP) {
-        const int quarter = warp & 3;
-        unsigned char *mine = epi + quarter * 32 * STAGE_ROW;
+        // warps w and w + 4 share a quarter of the rows and take every other 32 columns
+        const int quarter = warp & 3, c_first = ((warp - EPI_WARP) >> 2) * 32;
+        unsigned char *mine = epi + (warp - EPI_WARP) * EPI_TILE;
         int j = 0;
         bool ok = true;
         for (int unit = blockIdx.x; unit < total; unit += gridDim.x, ++j) {
@@ -169,12 +170,16 @@ wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
             if (!ok) failed = 1;
             fence_after();
             const uint32_t from = tmem + (uint32_t)buf * BUF_COLS + ((uint32_t)(quarter * 32) << 16);
-            for (int c = 0; c < p.NT; c += 64) {
-                uint32_t v[64];
+            if (ok && c_first >= p.NT) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(acc_free[buf]));
+            }
+            for (int c = c_first; c < p.NT; c += 64) {
+                uint32_t v[32];
                 const int left = min(p.NT - c, p.N - n0 - c);
                 if (ok) {
 #pragma unroll
-                    for (int u = 0; u < 4; ++u)
+                    for (int u = 0; u < 2; ++u)
                         if (u * 16 < left) tmem_ld16(from + (uint32_t)(c + u * 16), v + u * 16);
                     tmem_ld_wait();
                     if (c + 64 >= p.NT) {
@@ -184,7 +189,7 @@ wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
                     }
                 } else {
 #pragma unroll
-                    for (int u = 0; u < 64; ++u) v[u] = 0x7fc00000u;
+                    for (int u = 0; u < 32; ++u) v[u] = 0x7fc00000u;
                 }
                 if (left <= 0) continue;
                 if (whole) {
@@ -192,7 +197,7 @@ wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
                     __syncwarp();
                     const size_t row_bytes = (size_t)p.N * 2;
                     unsigned char *to = reinterpret_cast<unsigned char *>(dW) + ((size_t)g * p.K + row) * row_bytes + (size_t)(n0 + c) * 2;
-                    store_tile(mine, to, row_bytes, rows, min(64, left) * 2, lane, p.out_access);
+                    store_tile(mine, to, row_bytes, rows, min(32, left) * 2, lane, p.out_access);
                     __syncwarp();
                 } else {
                     // part of a sum: 32 bits, [slot][K][ntiles * NT]
@@ -200,14 +205,11 @@ wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
                     unsigned char *to = reinterpret_cast<unsigned char *>(partial) + (slot * p.K + row) * row_bytes + (size_t)(n0 + c) * 4;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                        for (int u = 0; u < 8; ++u)
-                            *reinterpret_cast<uint4 *>(mine + lane * STAGE_ROW + u * 16) =
-                                make_uint4(v[h * 32 + u * 4], v[h * 32 + u * 4 + 1], v[h * 32 + u * 4 + 2], v[h * 32 + u * 4 + 3]);
+                        stage_row_f32(mine, lane, v + h * 16);
                         __syncwarp();
                         // columns up to the tile's padding are written: the tile has room for them
-                        const int cols = min(32, p.NT - c - h * 32);
-                        if (cols > 0) store_rows<16>(mine, to + h * 128, row_bytes, rows, cols * 4, lane);
+                        const int cols = min(16, p.NT - c - h * 16);
+                        if (cols > 0) store_rows<16>(mine, to + h * 64, row_bytes, rows, cols * 4, lane);
                         __syncwarp();
                     }
                 }
