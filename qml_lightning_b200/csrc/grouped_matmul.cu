@@ -6,114 +6,85 @@
 //
 // Rows in front of the first and behind the last group give zero rows.  The group bounds live on the device and are
 // clamped to [0, n], so the host never waits for them and no value of theirs leads outside the tensors.
-// 64 x 64 tiles of FFMA products with 32-bit sums; any size, alignment and element type.
+// This file: the entry points, and FFMA kernels for few rows (any size, alignment and element type), where a product is bound by
+// reading the matrices and by latency; everything else goes to the tensor cores (grouped_tc.cu, grouped_wgrad_tc.cu for 16-bit
+// rows, grouped_pair_tc.cu for float32).
 #include "grouped_tc.cuh"
 #include "typed.cuh"
 
 namespace {
 
-constexpr int BM = 64, BN = 64, BK = 16, PAD = 4;
+constexpr int BM = 64, BN = 64, BK = 16, PAD = 4;      // tile of the gradient kernel
 constexpr int MAX_GROUPS = 1024;
 
 __device__ __forceinline__ int clamped(const int *start, int g, int n) { return min(max(start[g], 0), n); }
 
-// tile number -> group and rows; false behind the last tile.  All threads of the block take part.
-__device__ bool find_tile(const int *__restrict__ start, int G, int n, int tile, int *sh, int &g, int &row0, int &row1) {
-    if (threadIdx.x < 32) {
-        const int lane = threadIdx.x;
-        int before = 0, found = 0;
-        for (int g0 = 0; g0 < G && !found; g0 += 32) {
-            int s = 0, e = 0;
-            if (g0 + lane < G) {
-                s = clamped(start, g0 + lane, n);
-                e = max(clamped(start, g0 + lane + 1, n), s);
-            }
-            const int t = (e - s + BM - 1) / BM;
-            int inc = t;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(QMLB_FULL_MASK, inc, o);
-                if (lane >= o) inc += v;
-            }
-            const bool here = tile >= before + inc - t && tile < before + inc;
-            const unsigned m = __ballot_sync(QMLB_FULL_MASK, here);
-            if (here) {
-                sh[1] = g0 + lane;
-                sh[2] = s + (tile - (before + inc - t)) * BM;
-                sh[3] = e;
-            }
-            found = m != 0;
-            before += __shfl_sync(QMLB_FULL_MASK, inc, 31);
-        }
-        if (lane == 0) sh[0] = found;
-    }
-    __syncthreads();
-    g = sh[1];
-    row0 = sh[2];
-    row1 = sh[3];
-    return sh[0] != 0;
-}
-
+// Few rows: a block takes 32 columns of one group's result.  Lanes are columns, the warps split the depth, and every thread
+// keeps ROWS sums, so a matrix is read once per ROWS rows, in whole lines; the warps' sums meet in shared memory.  A transposed
+// matrix passes through a padded tile per warp.  What counts is latency: all loads of a stretch of the depth, rows and matrix,
+// are in flight before the first is used (addresses are clamped instead of tested).
+constexpr int ROWS = 8;
 template <typename T, bool TRANS>
-__global__ void __launch_bounds__(256)
-product_kernel(const T *__restrict__ x, const T *__restrict__ W, const int *__restrict__ start, int G, int n, int K, int N, int w_cols,
-               T *__restrict__ y) {
-    __shared__ __align__(16) float As[BK][BM + PAD];
-    __shared__ __align__(16) float Bs[BK][BN + PAD];
-    __shared__ int sh[4];
-    int g, row0, row1;
-    const int col0 = blockIdx.y * BN, tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    // zero rows outside the groups: every block takes its share
-    {
+__global__ void __launch_bounds__(TRANS ? 256 : 512)
+few_rows_kernel(const T *__restrict__ x, const T *__restrict__ W, const int *__restrict__ start, int G, int n, int K, int N, int w_cols,
+                T *__restrict__ y) {
+    constexpr int WARPS = TRANS ? 8 : 16, THREADS = WARPS * 32, DEPTH = WARPS * 32, PER = 32;      // each warp: 32 of the depth
+    __shared__ __align__(16) float xs[DEPTH][ROWS];
+    __shared__ float turn[TRANS ? WARPS : 1][32][TRANS ? 33 : 1];
+    float(*sums)[ROWS][32] = reinterpret_cast<float(*)[ROWS][32]>(&xs[0][0]);      // [WARPS][ROWS][32], once the depth is through
+    static_assert(WARPS * 32 <= DEPTH, "the sums fit over the rows");
+    const int g = blockIdx.y, col0 = blockIdx.x * 32, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = col0 + lane;
+    const int s = clamped(start, g, n), e = clamped(start, g + 1, n);
+    if (g == 0 && blockIdx.z == 0) {                       // zero rows outside the groups
         const int first = clamped(start, 0, n), last = max(clamped(start, G, n), first);
-        for (int r = blockIdx.x * 4 + (tid >> 6); r < n; r += gridDim.x * 4) {
-            if (r >= first && r < last) continue;
-            const int c = col0 + (tid & 63);
-            if (c < N) y[(size_t)r * N + c] = qmlb::from_f32<T>(0.f);
-        }
+        for (int r = warp; r < n; r += WARPS)
+            if ((r < first || r >= last) && c < N) y[(size_t)r * N + c] = qmlb::from_f32<T>(0.f);
     }
-    if (!find_tile(start, G, n, blockIdx.x, sh, g, row0, row1)) return;
     const T *Wg = W + (size_t)g * K * N;
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < K; k0 += BK) {
-        {
-            const int r = tid >> 2, kk = (tid & 3) * 4;
+    for (int r0 = s + blockIdx.z * ROWS; r0 < e; r0 += gridDim.z * ROWS) {
+        float acc[ROWS];
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                As[kk + q][r] = (row0 + r < row1 && k0 + kk + q < K) ? qmlb::to_f32(x[(size_t)(row0 + r) * K + k0 + kk + q]) : 0.f;
-        }
-        if (!TRANS) {
-            const int k = tid >> 4, c = (tid & 15) * 4;
+        for (int i = 0; i < ROWS; ++i) acc[i] = 0.f;
+        for (int k0 = 0; k0 < K; k0 += DEPTH) {
+            const int ka = k0 + warp * PER, m = min(PER, K - ka);              // this warp's part of the depth (m may be negative)
+            T w[PER];
+            if (!TRANS) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                Bs[k][c + q] = (k0 + k < K && col0 + c + q < N) ? qmlb::to_f32(Wg[(size_t)(k0 + k) * w_cols + col0 + c + q]) : 0.f;
-        } else {
-            const int c = tid >> 2, kk = (tid & 3) * 4;
+                for (int i = 0; i < PER; ++i) w[i] = Wg[(size_t)min(ka + i, K - 1) * w_cols + min(c, N - 1)];
+            } else {
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                Bs[kk + q][c] = (k0 + kk + q < K && col0 + c < N) ? qmlb::to_f32(Wg[(size_t)(col0 + c) * w_cols + k0 + kk + q]) : 0.f;
+                for (int i = 0; i < PER; ++i) w[i] = Wg[(size_t)min(col0 + i, N - 1) * w_cols + min(ka + lane, K - 1)];
+            }
+            T v[ROWS * DEPTH / THREADS];                                       // one k per thread, ROWS rows
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) v[i] = x[(size_t)min(r0 + i, e - 1) * K + min(k0 + (int)threadIdx.x, K - 1)];
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) xs[threadIdx.x][i] = k0 + (int)threadIdx.x < K ? qmlb::to_f32(v[i]) : 0.f;
+            if (TRANS) {
+#pragma unroll
+                for (int i = 0; i < PER; ++i) turn[warp][i][lane] = qmlb::to_f32(w[i]);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const float u = i < m ? (TRANS ? turn[warp][lane][i] : qmlb::to_f32(w[i])) : 0.f;      // behind the depth both are zero
+                const float4 a = *reinterpret_cast<const float4 *>(&xs[warp * PER + i][0]), b = *reinterpret_cast<const float4 *>(&xs[warp * PER + i][4]);
+                acc[0] = fmaf(a.x, u, acc[0]); acc[1] = fmaf(a.y, u, acc[1]); acc[2] = fmaf(a.z, u, acc[2]); acc[3] = fmaf(a.w, u, acc[3]);
+                acc[4] = fmaf(b.x, u, acc[4]); acc[5] = fmaf(b.y, u, acc[5]); acc[6] = fmaf(b.z, u, acc[6]); acc[7] = fmaf(b.w, u, acc[7]);
+            }
         }
         __syncthreads();
 #pragma unroll
-        for (int kk = 0; kk < BK; ++kk) {
-            const float4 a = *reinterpret_cast<const float4 *>(&As[kk][ty * 4]);
-            const float4 b = *reinterpret_cast<const float4 *>(&Bs[kk][tx * 4]);
-            const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+        for (int i = 0; i < ROWS; ++i) sums[warp][i][lane] = acc[i];
+        __syncthreads();
+        if (warp < ROWS) {                                   // one row per warp
+            float t = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(av[i], bv[j], acc[i][j]);
+            for (int q = 0; q < WARPS; ++q) t += sums[q][warp][lane];
+            if (r0 + warp < e && c < N) y[(size_t)(r0 + warp) * N + c] = qmlb::from_f32<T>(t);
         }
         __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = row0 + ty * 4 + i;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int c = col0 + tx * 4 + j;
-            if (r < row1 && c < N) y[(size_t)r * N + c] = qmlb::from_f32<T>(acc[i][j]);
-        }
     }
 }
 
@@ -158,14 +129,15 @@ wgrad_kernel(const T *__restrict__ x, const T *__restrict__ dy, const int *__res
 }
 
 template <typename T>
-int run_product(const void *x, const void *W, const int *start, int G, int n, int K, int N, int transpose, void *y, cudaStream_t st) {
+int run_few_rows(const void *x, const void *W, const int *start, int G, int n, int K, int N, int transpose, void *y, cudaStream_t st) {
     const int in = transpose ? N : K, out = transpose ? K : N;
-    // every group adds at most one partly filled tile
-    dim3 grid((unsigned)((n + BM - 1) / BM + G), (unsigned)((out + BN - 1) / BN));
+    // blocks that share a group's rows: for twice the average group; the rest of a larger group takes turns
+    const int turns = (2 * n / G + ROWS - 1) / ROWS, z = turns < 1 ? 1 : turns > 16 ? 16 : turns;
+    const dim3 grid((unsigned)((out + 31) / 32), (unsigned)G, (unsigned)z);
     if (transpose)
-        product_kernel<T, true><<<grid, 256, 0, st>>>(static_cast<const T *>(x), static_cast<const T *>(W), start, G, n, in, out, N, static_cast<T *>(y));
+        few_rows_kernel<T, true><<<grid, 256, 0, st>>>(static_cast<const T *>(x), static_cast<const T *>(W), start, G, n, in, out, N, static_cast<T *>(y));
     else
-        product_kernel<T, false><<<grid, 256, 0, st>>>(static_cast<const T *>(x), static_cast<const T *>(W), start, G, n, in, out, N, static_cast<T *>(y));
+        few_rows_kernel<T, false><<<grid, 512, 0, st>>>(static_cast<const T *>(x), static_cast<const T *>(W), start, G, n, in, out, N, static_cast<T *>(y));
     return qmlb::check_launch("qmlb_grouped_matmul");
 }
 
@@ -176,13 +148,22 @@ int run_wgrad(const void *x, const void *dy, const int *start, int G, int n, int
     return qmlb::check_launch("qmlb_grouped_matmul_wgrad");
 }
 
-bool few_rows(size_t n) { return n < 256; }
+// Few rows or many.  Measured (float32, B200): the FFMA kernel takes 8 us and 2 n K N operations at 10 TFLOP/s, the tensor-core
+// path 24 us and 12 bytes per matrix element for the images; equal at n = 9 G + 8e7 / (K N).  (3 groups, 336 x 256: 8 against
+// 26 us at n = 64, 29 against 28 us at n = 1,024; 32 groups, 1,024 x 1,024: 74 against 107 us at n = 256, 127 against 109 us at
+// n = 512.)  Beyond 2,048 rows a block would walk too many of them.
+bool few_rows(size_t n, int G, int K, int N) { return n <= 2048 && (double)n <= 9.0 * G + 8e7 / ((double)K * N); }
+// Gradient of the matrices.  float32: 16 against 18 us at n = 256, 27 against 23 us at n = 512 (3 groups, 336 x 256).  16-bit: 6 to
+// 10 against 16 us (which are mostly launches) while the result is small; 57 against 34 us for 32 groups, 1,024 x 1,024.
+bool few_rows_grad(size_t n, int G, int K, int N, int dtype) {
+    return dtype == QMLB_F32 ? n < 256 : n <= 128 && (double)G * K * N <= 4e6;
+}
 
 }  // namespace
 
 extern "C" size_t qmlb_grouped_matmul_workspace_bytes(size_t n, int ngroups, int K, int N, int dtype, int transpose) {
     if (n == 0 || ngroups <= 0 || K <= 0 || N <= 0) return 256;
-    if (dtype == QMLB_F32) return few_rows(n) ? 256 : qmlb::grouped_pair_workspace(n, ngroups, K, N, transpose);
+    if (dtype == QMLB_F32) return few_rows(n, ngroups, K, N) ? 256 : qmlb::grouped_pair_workspace(n, ngroups, K, N, transpose);
     return qmlb::grouped_tc_workspace(ngroups, K, N);
 }
 
@@ -195,7 +176,7 @@ extern "C" int qmlb_grouped_matmul(const void *x, const void *W, const int *grou
     QMLB_REQUIRE(n < ((size_t)1 << 31) - (1 << 20), "qmlb_grouped_matmul: too many rows");
     if (n == 0) return QMLB_OK;
     cudaStream_t st = qmlb::as_stream(stream);
-    if (dtype == QMLB_F32 && few_rows(n)) return run_product<float>(x, W, group_start, ngroups, (int)n, K, N, transpose, out, st);
+    if (dtype == QMLB_F32 && few_rows(n, ngroups, K, N)) return run_few_rows<float>(x, W, group_start, ngroups, (int)n, K, N, transpose, out, st);
     QMLB_REQUIRE(workspace && workspace_bytes >= qmlb_grouped_matmul_workspace_bytes(n, ngroups, K, N, dtype, transpose),
                  "qmlb_grouped_matmul: workspace too small");
     QMLB_REQUIRE(((uintptr_t)workspace & 255) == 0, "qmlb_grouped_matmul: workspace must be 256-byte aligned");
@@ -207,7 +188,8 @@ extern "C" int qmlb_grouped_matmul(const void *x, const void *W, const int *grou
 
 extern "C" size_t qmlb_grouped_matmul_wgrad_workspace_bytes(size_t n, int ngroups, int K, int N, int dtype) {
     if (n == 0 || ngroups <= 0 || K <= 0 || N <= 0) return 256;
-    if (dtype == QMLB_F32) return few_rows(n) ? 256 : qmlb::grouped_wgrad_pair_workspace(n, ngroups, K, N);
+    if (few_rows_grad(n, ngroups, K, N, dtype)) return 256;
+    if (dtype == QMLB_F32) return qmlb::grouped_wgrad_pair_workspace(n, ngroups, K, N);
     return qmlb::grouped_wgrad_tc_workspace(n, ngroups, K, N);
 }
 
@@ -224,7 +206,11 @@ extern "C" int qmlb_grouped_matmul_wgrad(const void *x, const void *dy, const in
         if (cudaMemsetAsync(dW, 0, (size_t)ngroups * K * N * es, st) != cudaSuccess) return qmlb::check_launch("qmlb_grouped_matmul_wgrad(memset)");
         return QMLB_OK;
     }
-    if (dtype == QMLB_F32 && few_rows(n)) return run_wgrad<float>(x, dy, group_start, ngroups, (int)n, K, N, dW, st);
+    if (few_rows_grad(n, ngroups, K, N, dtype)) {
+        if (dtype == QMLB_F32) return run_wgrad<float>(x, dy, group_start, ngroups, (int)n, K, N, dW, st);
+        if (dtype == QMLB_F16) return run_wgrad<__half>(x, dy, group_start, ngroups, (int)n, K, N, dW, st);
+        return run_wgrad<__nv_bfloat16>(x, dy, group_start, ngroups, (int)n, K, N, dW, st);
+    }
     QMLB_REQUIRE(workspace && workspace_bytes >= qmlb_grouped_matmul_wgrad_workspace_bytes(n, ngroups, K, N, dtype),
                  "qmlb_grouped_matmul_wgrad: workspace too small");
     QMLB_REQUIRE(((uintptr_t)workspace & 255) == 0, "qmlb_grouped_matmul_wgrad: workspace must be 256-byte aligned");
