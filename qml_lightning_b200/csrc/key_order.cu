@@ -9,10 +9,14 @@
 //   3. scatter   : every block ranks its keys again (the same order, so the result never depends on scheduling) and
 //                  writes position and key to base(digit) + counts[digit][block] + rank
 // Rank inside a block: each warp owns a contiguous run of its keys; the lanes that hold the same digit find one another
-// with one ballot per digit bit, and the warp's running count per digit stays in shared memory.  What bounds a pass is
+// by ballots or a match, and the warp's running count per digit stays in shared memory.  What bounds a pass is
 // latency and the scattered writes, not arithmetic: 8 + 8 bytes per key and pass.
-// With one pass the digit totals are the group sizes; with more, group_start comes from a binary search per key in the
-// sorted keys.
+// With one pass the digit totals are the group sizes; with more, group_start is read off the sorted keys.
+// Up to CLUSTER_KEYS keys take one launch of one thread-block cluster: the same passes, with the digit totals read from the
+// neighbours' shared memory and cluster barriers between the steps.  (Separate launches took 20 us for one pass and 57 us for two
+// whatever the number of keys; most of it the launches and the few busy SMs.)
+#include <cooperative_groups.h>
+
 #include "typed.cuh"
 
 namespace {
@@ -34,16 +38,35 @@ __device__ __forceinline__ uint32_t clamp_key(K k, uint32_t nkeys) {
     return (k >= 0 && (unsigned long long)k < (unsigned long long)nkeys) ? (uint32_t)k : nkeys;
 }
 
-// lanes whose value agrees with mine in the lowest `nbits` bits (all lanes of the warp take part; lanes with
-// `in` = false match nobody that has it true)
+// lanes that hold the same digit as mine (all lanes of the warp take part; lanes with `in` = false match nobody that has it
+// true).  Few digits: one match instruction, whose time grows with the number of distinct values; many: one ballot per bit.
 __device__ __forceinline__ unsigned same_digit(uint32_t d, int nbits, bool in) {
+    if (nbits <= 4) return __match_any_sync(QMLB_FULL_MASK, in ? d : 0xffffffffu);
     unsigned m = __ballot_sync(QMLB_FULL_MASK, in);
     if (!in) m = ~m;
-    for (int b = 0; b < nbits; ++b) {
-        const unsigned v = __ballot_sync(QMLB_FULL_MASK, (d >> b) & 1u);
-        m &= ((d >> b) & 1u) ? v : ~v;
+#pragma unroll
+    for (int b = 0; b < RADIX_BITS; ++b) {
+        if (b >= nbits) break;
+        const bool one = (d >> b) & 1u;
+        const unsigned v = __ballot_sync(QMLB_FULL_MASK, one);
+        m &= one ? v : ~v;
     }
     return m;
+}
+
+// group_start[v] = first position whose sorted key is not below v, for the v that the 32 positions p0 .. p0 + 31 answer: those
+// above the key in front of them and not above their last one (positions behind the end count as the key nkeys).  `key`: the key
+// of position p0 + lane, `front`: the key of position p0 - 1, or -1.  All lanes of the warp take part; writes are whole lines.
+__device__ __forceinline__ void write_starts(uint32_t key, int64_t front, uint32_t p0, int *__restrict__ group_start) {
+    const uint32_t last = __shfl_sync(QMLB_FULL_MASK, key, 31);
+    for (int64_t v0 = front + 1; v0 <= (int64_t)last; v0 += 32) {
+        const uint32_t v = (uint32_t)v0 + (threadIdx.x & 31);
+        int below = 0;                                           // lanes with a smaller key
+#pragma unroll
+        for (int step = 16; step; step >>= 1)
+            if (__shfl_sync(QMLB_FULL_MASK, key, below + step - 1) < v) below += step;
+        if (v <= last) group_start[v] = (int)(p0 + below);
+    }
 }
 
 // FIRST: keys come from the caller's tensor; else from the pairs of the previous pass
@@ -56,12 +79,16 @@ histogram_kernel(const K *__restrict__ keys, const uint32_t *__restrict__ pair_k
     for (int d = threadIdx.x; d < nd; d += THREADS) hist[d] = 0;
     __syncthreads();
     const uint32_t base = blockIdx.x * (uint32_t)TILE;
-#pragma unroll 4
+    uint32_t key[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {                // addresses are clamped instead of tested: all loads are in flight together
+        const uint32_t in = min(base + i * THREADS + threadIdx.x, n - 1);
+        key[i] = FIRST ? clamp_key(keys[in], nkeys) : pair_keys[in];
+    }
+#pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        const uint32_t at = base + i * THREADS + threadIdx.x;
-        const bool in = at < n;
-        uint32_t d = 0;
-        if (in) d = ((FIRST ? clamp_key(keys[at], nkeys) : pair_keys[at]) >> shift) & (uint32_t)(nd - 1);
+        const bool in = base + i * THREADS + threadIdx.x < n;
+        const uint32_t d = (key[i] >> shift) & (uint32_t)(nd - 1);
         // few distinct digits: one shared-memory add per distinct digit and warp instead of 32 colliding ones
         const unsigned m = same_digit(d, nbits, in);
         if (in && (threadIdx.x & 31) == __ffs(m) - 1) atomicAdd(&hist[d], (uint32_t)__popc(m));
@@ -82,14 +109,15 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t *warp_sums
     __syncthreads();
     if (lane == 31) warp_sums[warp] = inc;
     __syncthreads();
-    uint32_t before = 0, all = 0;
-    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) {
-        const uint32_t s = warp_sums[w];
-        if (w < warp) before += s;
-        all += s;
+    const uint32_t own = lane < (int)(blockDim.x >> 5) ? warp_sums[lane] : 0;      // every warp adds the warps' sums up
+    uint32_t upto = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t t = __shfl_up_sync(QMLB_FULL_MASK, upto, o);
+        if (lane >= o) upto += t;
     }
-    *sum = all;
-    return before + inc - v;
+    *sum = __shfl_sync(QMLB_FULL_MASK, upto, 31);
+    return __shfl_sync(QMLB_FULL_MASK, upto - own, warp) + inc - v;
 }
 
 __global__ void __launch_bounds__(THREADS)
@@ -139,13 +167,9 @@ scatter_kernel(const K *__restrict__ keys, const uint32_t *__restrict__ pair_key
     uint32_t *mine = run + warp * nd;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        const uint32_t at = w0 + i * 32 + lane;
-        key[i] = 0;
-        pos[i] = at;
-        if (at < n) {
-            key[i] = FIRST ? clamp_key(keys[at], nkeys) : pair_keys[at];
-            if (!FIRST) pos[i] = pair_pos[at];
-        }
+        const uint32_t at = w0 + i * 32 + lane, in = min(at, n - 1);
+        key[i] = FIRST ? clamp_key(keys[in], nkeys) : pair_keys[in];
+        pos[i] = FIRST ? at : pair_pos[in];
     }
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
@@ -179,7 +203,16 @@ scatter_kernel(const K *__restrict__ keys, const uint32_t *__restrict__ pair_key
     }
 }
 
-// group_start[v] = first position whose sorted key is not below v
+// the same from all positions, 32 per warp
+__global__ void __launch_bounds__(THREADS)
+fill_kernel(const uint32_t *__restrict__ sorted, uint32_t n, uint32_t nkeys, int *__restrict__ group_start) {
+    const uint32_t p0 = (blockIdx.x * WARPS + (threadIdx.x >> 5)) * 32, p = p0 + (threadIdx.x & 31);
+    if (p0 > n) return;
+    const uint32_t key = p < n ? sorted[p] : nkeys;
+    write_starts(key, p0 == 0 ? -1 : (int64_t)sorted[p0 - 1], p0, group_start);
+}
+
+// the same by a search per key: many more keys than positions would leave wide gaps to few warps
 __global__ void __launch_bounds__(THREADS)
 start_kernel(const uint32_t *__restrict__ sorted, uint32_t n, uint32_t nkeys, int *__restrict__ group_start) {
     for (uint32_t v = blockIdx.x * THREADS + threadIdx.x; v <= nkeys; v += gridDim.x * THREADS) {
@@ -194,6 +227,172 @@ start_kernel(const uint32_t *__restrict__ sorted, uint32_t n, uint32_t nkeys, in
 
 __global__ void empty_kernel(uint32_t nkeys, int *__restrict__ group_start) {
     for (uint32_t v = blockIdx.x * THREADS + threadIdx.x; v <= nkeys; v += gridDim.x * THREADS) group_start[v] = 0;
+}
+
+// ---- one cluster ----------------------------------------------------------------------------------------------------
+constexpr int C_THREADS = 1024, C_WARPS = 32, C_ITEMS = 8, C_BITS = 9, C_MAX = 8;
+constexpr uint32_t CLUSTER_KEYS = C_MAX * C_THREADS * C_ITEMS;      // 65,536
+
+// `items` keys per thread; pairs: scratch of two buffers of n keys and two of n positions
+template <typename K>
+__global__ void __launch_bounds__(C_THREADS)
+cluster_kernel(const K *__restrict__ keys, uint32_t n, uint32_t nkeys, int passes, int nbits, int items, int *__restrict__ order,
+               int *__restrict__ group_start, uint32_t *__restrict__ pairs, uint32_t row, int fill) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    extern __shared__ uint32_t sm[];
+    __shared__ uint32_t warp_sums[C_WARPS];
+    const int nd = 1 << nbits, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t *totals = sm;                                       // [2][nd], read by the other blocks (two: passes take turns)
+    uint32_t *base = sm + 2 * nd;                                // [nd] first place of this block's keys of a digit
+    uint32_t *inside = sm + 3 * nd;                              // [nd] the same within the block
+    uint16_t *run = reinterpret_cast<uint16_t *>(sm + 4 * nd);   // [C_WARPS][nd]
+    // Many digits: the block's keys are first put in order here and leave in runs of one digit; scattered one by one they would
+    // cost a store each on the few SMs of the cluster.
+    const bool gather = nbits > 5;
+    uint32_t *own_key = sm + 4 * nd + C_WARPS * nd / 2, *own_pos = own_key + C_THREADS * items;
+    const int rank_of_block = (int)cluster.block_rank(), blocks = (int)cluster.num_blocks();
+    const uint32_t w0 = ((uint32_t)rank_of_block * C_WARPS + warp) * (uint32_t)(32 * items);
+    uint32_t *bk[2] = {pairs, pairs + row}, *bp[2] = {pairs + 2 * row, pairs + 3 * row};
+    for (int pass = 0; pass < passes; ++pass) {
+        const bool first = pass == 0, last = pass == passes - 1;
+        const int shift = pass * nbits;
+        const uint32_t *ik = bk[(pass + 1) & 1], *ip = bp[(pass + 1) & 1];
+        uint32_t *ok = bk[pass & 1], *op = last ? reinterpret_cast<uint32_t *>(order) : bp[pass & 1];
+        uint32_t key[C_ITEMS], pos[C_ITEMS];
+        uint16_t rank[C_ITEMS];
+#pragma unroll
+        for (int i = 0; i < C_ITEMS; ++i) {
+            // addresses are clamped instead of tested: all loads are in flight together
+            const uint32_t at = w0 + i * 32 + lane, in = min(at, n - 1);
+            key[i] = first ? clamp_key(keys[in], nkeys) : ik[in];
+            pos[i] = first ? at : ip[in];
+        }
+        for (int i = threadIdx.x; i < C_WARPS * nd / 2; i += C_THREADS) reinterpret_cast<uint32_t *>(run)[i] = 0;
+        __syncthreads();
+        uint16_t *mine = run + warp * nd;
+#pragma unroll
+        for (int i = 0; i < C_ITEMS; ++i) {
+            if (i < items && w0 + i * 32 < n) {                  // the same for the whole warp
+                const bool in = w0 + i * 32 + lane < n;
+                const uint32_t d = (key[i] >> shift) & (uint32_t)(nd - 1);
+                const unsigned m = same_digit(d, nbits, in);
+                const uint32_t before = in ? mine[d] : 0;
+                __syncwarp();
+                rank[i] = (uint16_t)(before + __popc(m & ((1u << lane) - 1u)));
+                if (in && lane == __ffs(m) - 1) mine[d] = (uint16_t)(before + __popc(m));
+                __syncwarp();
+            }
+        }
+        __syncthreads();
+        uint32_t *tot = totals + (pass & 1) * nd;
+        if ((int)threadIdx.x < nd) {                             // warps' counts -> prefix over the warps, block total
+            const int d = threadIdx.x;
+            uint32_t sum = 0;
+            uint16_t c[C_WARPS];
+#pragma unroll
+            for (int w = 0; w < C_WARPS; ++w) c[w] = run[w * nd + d];
+#pragma unroll
+            for (int w = 0; w < C_WARPS; ++w) {
+                run[w * nd + d] = (uint16_t)sum;
+                sum += c[w];
+            }
+            tot[d] = sum;
+        }
+        cluster.sync();
+        uint32_t before = 0, all = 0;
+        if ((int)threadIdx.x < nd)
+        {
+            uint32_t t[C_MAX];
+#pragma unroll
+            for (int q = 0; q < C_MAX; ++q) t[q] = *cluster.map_shared_rank(tot + threadIdx.x, min(q, blocks - 1));
+#pragma unroll
+            for (int q = 0; q < C_MAX; ++q) {
+                if (q < rank_of_block) before += t[q];
+                if (q < blocks) all += t[q];
+            }
+        }
+        uint32_t whole;
+        const uint32_t start = block_prefix(all, warp_sums, &whole);
+        uint32_t local = 0;
+        if (gather) local = block_prefix((int)threadIdx.x < nd ? tot[threadIdx.x] : 0u, warp_sums, &whole);
+        if ((int)threadIdx.x < nd) {
+            base[threadIdx.x] = start + before - local;          // (modulo 2^32)
+            inside[threadIdx.x] = local;
+            if (passes == 1 && rank_of_block == 0 && threadIdx.x <= nkeys) group_start[threadIdx.x] = (int)start;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < C_ITEMS; ++i) {
+            if (i < items && w0 + i * 32 + lane < n) {
+                const uint32_t d = (key[i] >> shift) & (uint32_t)(nd - 1), to = (gather ? inside[d] : base[d]) + mine[d] + rank[i];
+                if (gather) {
+                    own_key[to] = key[i];
+                    own_pos[to] = pos[i];
+                } else {
+                    op[to] = pos[i];
+                    if (passes > 1) ok[to] = key[i];
+                }
+            }
+        }
+        if (gather) {
+            __syncthreads();
+            for (uint32_t i = threadIdx.x; i < whole; i += C_THREADS) {
+                const uint32_t k = own_key[i], to = base[(k >> shift) & (uint32_t)(nd - 1)] + i;
+                op[to] = own_pos[i];
+                if (passes > 1) ok[to] = k;
+            }
+        }
+        cluster.sync();                                          // pairs written; nobody reads a block's totals after it has left
+    }
+    if (!fill) return;
+    // group_start[v] = first position whose key is not below v: position p writes the v above its predecessor's key
+    const uint32_t *sorted = bk[(passes - 1) & 1];
+    uint32_t here[C_ITEMS], left[C_ITEMS];
+#pragma unroll
+    for (int i = 0; i < C_ITEMS; ++i) {
+        const uint32_t p0 = w0 + i * 32;
+        here[i] = sorted[min(p0 + lane, n - 1)];
+        left[i] = sorted[min(max(p0, 1u) - 1, n - 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < C_ITEMS; ++i) {
+        const uint32_t p0 = w0 + i * 32;
+        if (i < items && p0 <= n) write_starts(p0 + lane < n ? here[i] : nkeys, p0 == 0 ? -1 : (int64_t)left[i], p0, group_start);
+    }
+    if (w0 + (uint32_t)(32 * items) == n) write_starts(nkeys, sorted[n - 1], n, group_start);      // nobody's positions lie behind the end
+}
+
+template <typename K>
+int run_cluster(const K *keys, size_t n, int nkeys, int *order, int *group_start, unsigned char *scratch, cudaStream_t st) {
+    const int bits = bits_for((unsigned)nkeys), passes = (bits + C_BITS - 1) / C_BITS, nbits = (bits + passes - 1) / passes;
+    int blocks = 1;
+    while (blocks < C_MAX && (size_t)blocks * C_THREADS * 2 < n) blocks <<= 1;      // two keys per thread, then more
+    const int items = (int)((n + (size_t)blocks * C_THREADS - 1) / ((size_t)blocks * C_THREADS));
+    // many more keys than positions: the gaps are wide, and a search per key on all SMs fills them sooner
+    const bool fill = passes > 1 && (size_t)nkeys <= 16 * n;
+    const uint32_t row = (uint32_t)(((n * 4 + 255) & ~(size_t)255) / 4);
+    uint32_t *pairs = reinterpret_cast<uint32_t *>(scratch);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(C_THREADS);
+    cfg.dynamicSmemBytes = ((size_t)16 << nbits) + ((size_t)C_WARPS * 2 << nbits) + (nbits > 5 ? (size_t)8 * C_THREADS * items : 0);
+    if (int rc = qmlb::ensure_smem(cluster_kernel<K>, cfg.dynamicSmemBytes, "qmlb_group_by_key")) return rc;
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = (unsigned)blocks;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, cluster_kernel<K>, keys, (uint32_t)n, (uint32_t)nkeys, passes, nbits, items, order, group_start, pairs, row,
+                           (int)fill) != cudaSuccess)
+        return qmlb::check_launch("qmlb_group_by_key");
+    if (passes > 1 && !fill) {
+        const uint32_t sb = ((uint32_t)nkeys + THREADS) / THREADS;
+        start_kernel<<<sb < 1184 ? sb : 1184, THREADS, 0, st>>>(pairs + ((passes - 1) & 1) * row, (uint32_t)n, (uint32_t)nkeys, group_start);
+    }
+    return qmlb::check_launch("qmlb_group_by_key");
 }
 
 struct Plan {
@@ -246,7 +445,8 @@ int run_sort(const K *keys, size_t n, int nkeys, int *order, int *group_start, u
             scatter_kernel<K, false, true><<<p.blocks, THREADS, scat_smem, st>>>(keys, ik, ip, un, uk, shift, p.nbits, counts, totals, pk[i & 1],
                                                                                  pos_out, group_start);
             const uint32_t sb = (uk + THREADS) / THREADS;
-            start_kernel<<<sb < 1184 ? sb : 1184, THREADS, 0, st>>>(pk[i & 1], un, uk, group_start);
+            if ((size_t)nkeys <= 16 * n) fill_kernel<<<un / (WARPS * 32) + 1, THREADS, 0, st>>>(pk[i & 1], un, uk, group_start);
+            else start_kernel<<<sb < 1184 ? sb : 1184, THREADS, 0, st>>>(pk[i & 1], un, uk, group_start);
         } else {
             scatter_kernel<K, false, false><<<p.blocks, THREADS, scat_smem, st>>>(keys, ik, ip, un, uk, shift, p.nbits, counts, totals, pk[i & 1],
                                                                                   pp[i & 1], group_start);
@@ -259,6 +459,7 @@ int run_sort(const K *keys, size_t n, int nkeys, int *order, int *group_start, u
 
 extern "C" size_t qmlb_group_by_key_scratch_bytes(size_t n, int nkeys) {
     if (n == 0 || n >= (size_t)1 << 31 || nkeys <= 0 || nkeys == INT32_MAX) return 256;
+    if (n <= CLUSTER_KEYS) return 4 * ((n * 4 + 255) & ~(size_t)255) + 256;
     return make_plan(n, nkeys).bytes + 256;
 }
 
@@ -276,6 +477,9 @@ extern "C" int qmlb_group_by_key(const void *keys, int key_bits, size_t n, int n
     QMLB_REQUIRE(scratch_bytes >= qmlb_group_by_key_scratch_bytes(n, nkeys) - 256, "qmlb_group_by_key: scratch too small");
     QMLB_REQUIRE(((uintptr_t)scratch & 3) == 0, "qmlb_group_by_key: scratch must be 4-byte aligned");
     unsigned char *sc = static_cast<unsigned char *>(scratch);
+    if (n <= CLUSTER_KEYS)
+        return key_bits == 32 ? run_cluster(static_cast<const int32_t *>(keys), n, nkeys, order, group_start, sc, st)
+                              : run_cluster(static_cast<const int64_t *>(keys), n, nkeys, order, group_start, sc, st);
     return key_bits == 32 ? run_sort(static_cast<const int32_t *>(keys), n, nkeys, order, group_start, sc, st)
                           : run_sort(static_cast<const int64_t *>(keys), n, nkeys, order, group_start, sc, st);
 }
