@@ -23,9 +23,9 @@ namespace {
 
 constexpr int RADIX_BITS = 10;                 // widest digit
 constexpr int THREADS = 256, WARPS = THREADS / 32;
-constexpr int ITEMS = 16;                      // keys per thread
-constexpr int TILE = THREADS * ITEMS;          // keys per block
-constexpr int WARP_TILE = 32 * ITEMS;
+// keys per thread: few while the blocks do not fill the device
+constexpr int FEW = 4, MANY = 16;
+inline int items_for(size_t n) { return n < (size_t)148 * 8 * THREADS * FEW ? FEW : MANY; }
 
 __host__ __device__ inline int bits_for(unsigned nkeys) {   // digits of the values 0 .. nkeys (nkeys = "outside")
     int b = 1;
@@ -70,7 +70,7 @@ __device__ __forceinline__ void write_starts(uint32_t key, int64_t front, uint32
 }
 
 // FIRST: keys come from the caller's tensor; else from the pairs of the previous pass
-template <typename K, bool FIRST>
+template <typename K, bool FIRST, int ITEMS>
 __global__ void __launch_bounds__(THREADS)
 histogram_kernel(const K *__restrict__ keys, const uint32_t *__restrict__ pair_keys, uint32_t n, uint32_t nkeys, int shift, int nbits,
                  uint32_t *__restrict__ counts) {
@@ -78,7 +78,7 @@ histogram_kernel(const K *__restrict__ keys, const uint32_t *__restrict__ pair_k
     const int nd = 1 << nbits;
     for (int d = threadIdx.x; d < nd; d += THREADS) hist[d] = 0;
     __syncthreads();
-    const uint32_t base = blockIdx.x * (uint32_t)TILE;
+    const uint32_t base = blockIdx.x * (uint32_t)(THREADS * ITEMS);
     uint32_t key[ITEMS];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {                // addresses are clamped instead of tested: all loads are in flight together
@@ -137,7 +137,7 @@ scan_kernel(uint32_t *__restrict__ counts, uint32_t nblocks, uint32_t *__restric
 }
 
 // LAST: writes order[] (and, when START, group_start from the digit totals: one-pass sorts)
-template <typename K, bool FIRST, bool LAST>
+template <typename K, bool FIRST, bool LAST, int ITEMS>
 __global__ void __launch_bounds__(THREADS)
 scatter_kernel(const K *__restrict__ keys, const uint32_t *__restrict__ pair_keys, const uint32_t *__restrict__ pair_pos, uint32_t n,
                uint32_t nkeys, int shift, int nbits, const uint32_t *__restrict__ counts, const uint32_t *__restrict__ totals,
@@ -161,7 +161,7 @@ scatter_kernel(const K *__restrict__ keys, const uint32_t *__restrict__ pair_key
     }
     __syncthreads();
     // pass over the warp's run: digit and rank of every key
-    const uint32_t w0 = blockIdx.x * (uint32_t)TILE + warp * (uint32_t)WARP_TILE;
+    const uint32_t w0 = blockIdx.x * (uint32_t)(THREADS * ITEMS) + warp * (uint32_t)(32 * ITEMS);
     uint32_t key[ITEMS], pos[ITEMS];
     uint16_t rank[ITEMS];
     uint32_t *mine = run + warp * nd;
@@ -230,8 +230,8 @@ __global__ void empty_kernel(uint32_t nkeys, int *__restrict__ group_start) {
 }
 
 // ---- one cluster ----------------------------------------------------------------------------------------------------
-constexpr int C_THREADS = 1024, C_WARPS = 32, C_ITEMS = 8, C_BITS = 9, C_MAX = 8;
-constexpr uint32_t CLUSTER_KEYS = C_MAX * C_THREADS * C_ITEMS;      // 65,536
+constexpr int C_THREADS = 1024, C_WARPS = 32, C_ITEMS = 8, C_BITS = 9, C_MAX = 16;
+constexpr uint32_t CLUSTER_KEYS = C_MAX * C_THREADS * C_ITEMS;      // 131,072
 
 // `items` keys per thread; pairs: scratch of two buffers of n keys and two of n positions
 template <typename K>
@@ -367,7 +367,9 @@ template <typename K>
 int run_cluster(const K *keys, size_t n, int nkeys, int *order, int *group_start, unsigned char *scratch, cudaStream_t st) {
     const int bits = bits_for((unsigned)nkeys), passes = (bits + C_BITS - 1) / C_BITS, nbits = (bits + passes - 1) / passes;
     int blocks = 1;
-    while (blocks < C_MAX && (size_t)blocks * C_THREADS * 2 < n) blocks <<= 1;      // two keys per thread, then more
+    // two keys per thread, then more; sixteen blocks (more than every device promises) only where ranking counts
+    const int most = passes > 1 || n > (size_t)8 * C_THREADS * C_ITEMS ? C_MAX : 8;
+    while (blocks < most && (size_t)blocks * C_THREADS * 2 < n) blocks <<= 1;
     const int items = (int)((n + (size_t)blocks * C_THREADS - 1) / ((size_t)blocks * C_THREADS));
     // many more keys than positions: the gaps are wide, and a search per key on all SMs fills them sooner
     const bool fill = passes > 1 && (size_t)nkeys <= 16 * n;
@@ -377,6 +379,8 @@ int run_cluster(const K *keys, size_t n, int nkeys, int *order, int *group_start
     cfg.gridDim = dim3((unsigned)blocks);
     cfg.blockDim = dim3(C_THREADS);
     cfg.dynamicSmemBytes = ((size_t)16 << nbits) + ((size_t)C_WARPS * 2 << nbits) + (nbits > 5 ? (size_t)8 * C_THREADS * items : 0);
+    if (blocks > 8 && cudaFuncSetAttribute(cluster_kernel<K>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+        return qmlb::check_launch("qmlb_group_by_key(cluster size)");
     if (int rc = qmlb::ensure_smem(cluster_kernel<K>, cfg.dynamicSmemBytes, "qmlb_group_by_key")) return rc;
     cfg.stream = st;
     cudaLaunchAttribute at;
@@ -406,7 +410,8 @@ Plan make_plan(size_t n, int nkeys) {
     const int bits = bits_for((unsigned)nkeys);
     p.passes = (bits + RADIX_BITS - 1) / RADIX_BITS;
     p.nbits = (bits + p.passes - 1) / p.passes;
-    p.blocks = (uint32_t)((n + TILE - 1) / TILE);
+    const size_t tile = (size_t)THREADS * items_for(n);
+    p.blocks = (uint32_t)((n + tile - 1) / tile);
     auto round = [](size_t v) { return (v + 255) & ~(size_t)255; };
     const size_t row = round(n * 4);
     p.counts = 0;
@@ -418,7 +423,7 @@ Plan make_plan(size_t n, int nkeys) {
     return p;
 }
 
-template <typename K>
+template <typename K, int ITEMS>
 int run_sort(const K *keys, size_t n, int nkeys, int *order, int *group_start, unsigned char *scratch, cudaStream_t st) {
     const Plan p = make_plan(n, nkeys);
     uint32_t *counts = reinterpret_cast<uint32_t *>(scratch + p.counts), *totals = reinterpret_cast<uint32_t *>(scratch + p.totals);
@@ -432,27 +437,28 @@ int run_sort(const K *keys, size_t n, int nkeys, int *order, int *group_start, u
         const bool first = i == 0, last = i == p.passes - 1;
         const int shift = i * p.nbits;
         const uint32_t *ik = first ? nullptr : pk[(i - 1) & 1], *ip = first ? nullptr : pp[(i - 1) & 1];
-        if (first) histogram_kernel<K, true><<<p.blocks, THREADS, hist_smem, st>>>(keys, ik, un, uk, shift, p.nbits, counts);
-        else histogram_kernel<K, false><<<p.blocks, THREADS, hist_smem, st>>>(keys, ik, un, uk, shift, p.nbits, counts);
+        uint32_t *ok = pk[i & 1], *op = last ? pos_out : pp[i & 1];
+        auto histogram = first ? histogram_kernel<K, true, ITEMS> : histogram_kernel<K, false, ITEMS>;
+        auto scatter = first ? (last ? scatter_kernel<K, true, true, ITEMS> : scatter_kernel<K, true, false, ITEMS>)
+                             : (last ? scatter_kernel<K, false, true, ITEMS> : scatter_kernel<K, false, false, ITEMS>);
+        histogram<<<p.blocks, THREADS, hist_smem, st>>>(keys, ik, un, uk, shift, p.nbits, counts);
         scan_kernel<<<1 << p.nbits, THREADS, 0, st>>>(counts, p.blocks, totals);
-        if (first && last) {
-            scatter_kernel<K, true, true><<<p.blocks, THREADS, scat_smem, st>>>(keys, ik, ip, un, uk, shift, p.nbits, counts, totals, nullptr,
-                                                                                pos_out, group_start);
-        } else if (first) {
-            scatter_kernel<K, true, false><<<p.blocks, THREADS, scat_smem, st>>>(keys, ik, ip, un, uk, shift, p.nbits, counts, totals, pk[0],
-                                                                                 pp[0], group_start);
-        } else if (last) {
-            scatter_kernel<K, false, true><<<p.blocks, THREADS, scat_smem, st>>>(keys, ik, ip, un, uk, shift, p.nbits, counts, totals, pk[i & 1],
-                                                                                 pos_out, group_start);
+        scatter<<<p.blocks, THREADS, scat_smem, st>>>(keys, ik, ip, un, uk, shift, p.nbits, counts, totals, ok, op, group_start);
+        if (last && !first) {
             const uint32_t sb = (uk + THREADS) / THREADS;
-            if ((size_t)nkeys <= 16 * n) fill_kernel<<<un / (WARPS * 32) + 1, THREADS, 0, st>>>(pk[i & 1], un, uk, group_start);
-            else start_kernel<<<sb < 1184 ? sb : 1184, THREADS, 0, st>>>(pk[i & 1], un, uk, group_start);
-        } else {
-            scatter_kernel<K, false, false><<<p.blocks, THREADS, scat_smem, st>>>(keys, ik, ip, un, uk, shift, p.nbits, counts, totals, pk[i & 1],
-                                                                                  pp[i & 1], group_start);
+            if ((size_t)nkeys <= 16 * n) fill_kernel<<<un / (WARPS * 32) + 1, THREADS, 0, st>>>(ok, un, uk, group_start);
+            else start_kernel<<<sb < 1184 ? sb : 1184, THREADS, 0, st>>>(ok, un, uk, group_start);
         }
     }
     return qmlb::check_launch("qmlb_group_by_key");
+}
+
+template <typename K>
+int run(const void *keys, size_t n, int nkeys, int *order, int *group_start, unsigned char *scratch, cudaStream_t st) {
+    const K *k = static_cast<const K *>(keys);
+    if (n <= CLUSTER_KEYS) return run_cluster(k, n, nkeys, order, group_start, scratch, st);
+    return items_for(n) == FEW ? run_sort<K, FEW>(k, n, nkeys, order, group_start, scratch, st)
+                               : run_sort<K, MANY>(k, n, nkeys, order, group_start, scratch, st);
 }
 
 }  // namespace
@@ -477,9 +483,5 @@ extern "C" int qmlb_group_by_key(const void *keys, int key_bits, size_t n, int n
     QMLB_REQUIRE(scratch_bytes >= qmlb_group_by_key_scratch_bytes(n, nkeys) - 256, "qmlb_group_by_key: scratch too small");
     QMLB_REQUIRE(((uintptr_t)scratch & 3) == 0, "qmlb_group_by_key: scratch must be 4-byte aligned");
     unsigned char *sc = static_cast<unsigned char *>(scratch);
-    if (n <= CLUSTER_KEYS)
-        return key_bits == 32 ? run_cluster(static_cast<const int32_t *>(keys), n, nkeys, order, group_start, sc, st)
-                              : run_cluster(static_cast<const int64_t *>(keys), n, nkeys, order, group_start, sc, st);
-    return key_bits == 32 ? run_sort(static_cast<const int32_t *>(keys), n, nkeys, order, group_start, sc, st)
-                          : run_sort(static_cast<const int64_t *>(keys), n, nkeys, order, group_start, sc, st);
+    return key_bits == 32 ? run<int32_t>(keys, n, nkeys, order, group_start, sc, st) : run<int64_t>(keys, n, nkeys, order, group_start, sc, st);
 }
