@@ -48,7 +48,7 @@ lookup_kernel(const void *__restrict__ index, int bits, const T *__restrict__ ta
 // ---- gradient -----------------------------------------------------------------------------------------------------
 struct GradPlan {
     int vec, chunks;          // elements per access, accesses per row
-    int tc, r, run;           // column threads, row groups (tc * r = THREADS), positions per row group
+    int tc, r, run;           // column threads, row groups (tc * r <= THREADS), positions per row group
     int block;                // positions per block = r * run
     unsigned blocks, col_blocks, zero_blocks;
     size_t bytes;
@@ -59,17 +59,17 @@ GradPlan make_grad_plan(size_t n, int nkeys, int width, int dtype, const void *d
     const int es = qmlb::dtype_size(dtype);
     p.vec = qmlb::access_bytes((size_t)width * es, es, dout, dtable) / es;
     p.chunks = width / p.vec;
-    p.tc = 1;
-    while (p.tc < 64 && p.tc < p.chunks) p.tc <<= 1;
+    // all accesses of a row in one block where 128 threads suffice, in equal parts otherwise
+    p.col_blocks = (unsigned)((p.chunks + 127) / 128);
+    p.tc = (p.chunks + (int)p.col_blocks - 1) / (int)p.col_blocks;
     p.r = THREADS / p.tc;
-    p.col_blocks = (unsigned)((p.chunks + p.tc - 1) / p.tc);
-    // enough blocks to fill the device several times over, but runs long enough that the pieces stay few
+    // runs long enough that the pieces stay few and all blocks run at once, short enough that there is a block for every SM
     p.run = 8;
-    while (p.run < 64 && p.r * p.run < 2048 && n / ((size_t)p.r * p.run) * p.col_blocks > 148 * 16) p.run <<= 1;
+    while (p.run < 128 && p.r * p.run < 2048 && n / ((size_t)p.r * p.run) * p.col_blocks > 148 * 4) p.run <<= 1;
     p.block = p.r * p.run;
     p.blocks = (unsigned)((n + p.block - 1) / p.block);
-    // rows of keys that do not occur are zeroed by all blocks; a table much larger than n gets blocks for that alone
-    const size_t table_blocks = ((size_t)nkeys * width * es + 65535) / 65536;
+    // rows of keys that do not occur are zeroed by blocks of their own
+    const size_t table_blocks = ((size_t)nkeys + p.r * 16 - 1) / (p.r * 16);
     p.zero_blocks = (unsigned)(table_blocks < 148 * 8 ? table_blocks : 148 * 8);
     // per block: key of the tail, then head and tail pieces
     p.bytes = (((size_t)p.blocks * 4 + 255) & ~(size_t)255) + (size_t)p.blocks * 2 * width * 4 + 512;
@@ -89,7 +89,7 @@ __device__ __forceinline__ void store_scaled(T *p, const float (&v)[VEC], float 
 template <typename T, int VEC>
 __global__ void __launch_bounds__(THREADS)
 grad_kernel(const T *__restrict__ dout, const void *__restrict__ index, int bits, const int *__restrict__ order,
-            const int *__restrict__ start, unsigned n, int nkeys, int chunks, int tc, int run, float scale, T *__restrict__ dtable,
+            const int *__restrict__ start, unsigned n, int nkeys, int chunks, int tc, int run, unsigned blocks, float scale, T *__restrict__ dtable,
             int *__restrict__ tail_key, float *__restrict__ pieces) {
     extern __shared__ int sm[];
     const int r = THREADS / tc, block = r * run, width = chunks * VEC;
@@ -98,33 +98,49 @@ grad_kernel(const T *__restrict__ dout, const void *__restrict__ index, int bits
     const size_t p0 = (size_t)blockIdx.x * block;
     const int col = blockIdx.y * tc + threadIdx.x % tc;    // access within the row
     const int g = threadIdx.x / tc;
-    // zero rows of keys without positions
-    for (int64_t v = (int64_t)blockIdx.x * r + g; v < nkeys; v += (int64_t)gridDim.x * r) {
-        if (start[v] == start[v + 1] && col < chunks) {
-            float z[VEC];
+    if (blockIdx.x >= blocks) {                            // zero rows of keys without positions
+        if (g >= r || col >= chunks) return;
+        float z[VEC];
 #pragma unroll
-            for (int q = 0; q < VEC; ++q) z[q] = 0.f;
-            qmlb::store_f32<T, VEC>(dtable + ((size_t)v * chunks + col) * VEC, z);
-        }
-    }
-    if (p0 >= n) return;
-    // keys of the positions p0 - 1 .. p0 + block; a position without a valid row has key -1 and adds nothing
-    for (int i = (int)threadIdx.x - 1; i <= block; i += THREADS) {
-        const size_t p = p0 + i;                           // wraps to a huge value at i = -1, p0 = 0
-        int o = -1, k = -1;
-        if (p < n) {
-            o = order[p];
-            if (o >= 0 && (unsigned)o < n) {
-                const int64_t v = index_at(index, bits, (size_t)o);
-                if (v >= 0 && v < nkeys) k = (int)v;
+        for (int q = 0; q < VEC; ++q) z[q] = 0.f;
+        const int64_t step = (int64_t)(gridDim.x - blocks) * r;
+        for (int64_t v = (int64_t)(blockIdx.x - blocks) * r + g; v < nkeys; v += 4 * step) {
+            bool empty[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {                  // addresses are clamped instead of tested: all loads are in flight together
+                const int64_t at = v + i * step < nkeys ? v + i * step : nkeys - 1;
+                empty[i] = start[at] == start[at + 1];
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (v + i * step < nkeys && empty[i]) qmlb::store_f32<T, VEC>(dtable + ((size_t)(v + i * step) * chunks + col) * VEC, z);
         }
-        if (i >= 0 && i < block) ord[i] = o;
-        key[i] = k;
+        return;
+    }
+    // keys of the positions p0 - 1 .. p0 + block; a position without a valid row has key -1 and adds nothing
+    for (int i0 = (int)threadIdx.x - 1; i0 <= block; i0 += 4 * THREADS) {
+        int o[4], k[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t p = (int64_t)p0 + i0 + u * THREADS;
+            o[u] = order[p < 0 ? 0 : p < (int64_t)n ? p : (int64_t)n - 1];
+            if (p < 0 || p >= (int64_t)n || o[u] < 0 || (unsigned)o[u] >= n) o[u] = -1;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t v = index_at(index, bits, (size_t)max(o[u], 0));
+            k[u] = o[u] >= 0 && v >= 0 && v < nkeys ? (int)v : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = i0 + u * THREADS;
+            if (i >= 0 && i < block) ord[i] = max(o[u], 0);
+            if (i <= block) key[i] = k[u];
+        }
     }
     __syncthreads();
-    const bool active = col < chunks;
-    const int a = g * run, b = a + run;
+    const bool mine = g < r, active = mine && col < chunks;         // threads beyond r * tc only fetch keys
+    const int a = mine ? g * run : 0, b = mine ? a + run : 0;
     float acc[VEC];
 #pragma unroll
     for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
@@ -132,20 +148,18 @@ grad_kernel(const T *__restrict__ dout, const void *__restrict__ index, int bits
     // whole run is its head
     float *head = piece + ((size_t)(g * 2) * tc + threadIdx.x % tc) * VEC, *tail = head + (size_t)tc * VEC;
     bool from_before = key[a - 1] == key[a];
-    constexpr int U = 4;
+    constexpr int U = 8;
     for (int i = a; i < b; i += U) {
         float x[U][VEC];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-#pragma unroll
-            for (int q = 0; q < VEC; ++q) x[u][q] = 0.f;
-            if (active && key[i + u] >= 0) qmlb::load_f32<T, VEC>(dout + ((size_t)ord[i + u] * chunks + col) * VEC, x[u]);
+            qmlb::load_f32<T, VEC>(dout + ((size_t)ord[i + u] * chunks + (active ? col : 0)) * VEC, x[u]);      // always: see above
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-#pragma unroll
-            for (int q = 0; q < VEC; ++q) acc[q] += x[u][q];
             const int k = key[i + u];
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) acc[q] += k >= 0 ? x[u][q] : 0.f;
             const bool ends = key[i + u + 1] != k, last = i + u == b - 1;
             if (k >= 0 && (ends || last)) {
                 if (ends && !from_before) {
@@ -166,6 +180,7 @@ grad_kernel(const T *__restrict__ dout, const void *__restrict__ index, int bits
     __syncthreads();
     // join the pieces of the block: the group whose run holds the beginning of a key (or group 0, for the key that began
     // before the block) adds the heads that follow
+    if (!mine) return;
     const int ka = key[a], kb = key[b - 1];
     const bool whole = ka == kb;                                    // one key fills the run
     const bool opens = kb >= 0 && key[b] == kb && !(whole && key[a - 1] == ka);   // a key begins here and goes on
@@ -215,35 +230,63 @@ grad_kernel(const T *__restrict__ dout, const void *__restrict__ index, int bits
     }
 }
 
-// Keys that cross block borders: block b whose tail opens such a key adds the heads of the blocks behind it, in order.
-// JOIN_LANES row lanes of 32 column threads each take every JOIN_LANES-th piece.
-constexpr int JOIN_LANES = 8;
-template <typename T>
-__global__ void __launch_bounds__(32 * JOIN_LANES)
+// Keys that cross block borders: block b whose tail opens such a key adds the heads of the blocks behind it, in an order that
+// depends on their number alone.  Few pieces: every thread adds its columns.  Many (one key may hold most positions): JOIN_LANES
+// row lanes of 32 column threads take every JOIN_LANES-th piece, and blockIdx.y shares the columns.
+constexpr int JOIN_LANES = 16, JOIN_THREADS = 32 * JOIN_LANES;
+template <typename T, int VEC>
+__global__ void __launch_bounds__(JOIN_THREADS)
 join_kernel(const int *__restrict__ tail_key, const float *__restrict__ pieces, const int *__restrict__ start, unsigned blocks, int block,
             int width, float scale, T *__restrict__ dtable) {
-    __shared__ float part[JOIN_LANES][32];
+    __shared__ float part[JOIN_LANES][32 * VEC];
     const unsigned b = blockIdx.x;
     const int k = tail_key[b];
     if (k < 0) return;
     const int end = start[k + 1];                                   // one past the key's last position
     unsigned last = end > 0 ? (unsigned)(end - 1) / (unsigned)block : 0u;
     if (last >= blocks) last = blocks - 1;
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    for (int c0 = blockIdx.y * 32; c0 < width; c0 += gridDim.y * 32) {
-        const int c = c0 + lane;
-        float s = 0.f;
-        if (c < width) {
+    auto load = [&](unsigned j, int c, float (&v)[VEC]) { qmlb::load_f32<float, VEC>(pieces + ((size_t)j * 2 + (j == b)) * width + c, v); };
+    auto store = [&](int c, const float (&s)[VEC]) {
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) dtable[(size_t)k * width + c + q] = qmlb::from_f32<T>(s[q] * scale);
+    };
+    if (last < b + JOIN_LANES) {
+        if (blockIdx.y) return;
+        for (int c = (int)threadIdx.x * VEC; c < width; c += JOIN_THREADS * VEC) {
+            float s[VEC], v[VEC];
+            load(b, c, s);
 #pragma unroll 4
-            for (unsigned j = b + (unsigned)w; j <= last; j += JOIN_LANES) s += pieces[((size_t)j * 2 + (j == b)) * width + c];
+            for (unsigned j = b + 1; j <= last; ++j) {
+                load(j, c, v);
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) s[q] += v[q];
+            }
+            store(c, s);
         }
-        part[w][lane] = s;
+        return;
+    }
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    for (int c0 = blockIdx.y * 32 * VEC; c0 < width; c0 += gridDim.y * 32 * VEC) {
+        const int c = c0 + lane * VEC;
+        float s[VEC], v[VEC];
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) s[q] = 0.f;
+        if (c < width) {
+#pragma unroll 8
+            for (unsigned j = b + (unsigned)w; j <= last; j += JOIN_LANES) {
+                load(j, c, v);
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) s[q] += v[q];
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) part[w][lane * VEC + q] = s[q];
         __syncthreads();
-        if (w == 0 && c < width) {
+        for (int i = threadIdx.x; i < 32 * VEC; i += JOIN_THREADS) {
             float t = 0.f;
 #pragma unroll
-            for (int q = 0; q < JOIN_LANES; ++q) t += part[q][lane];
-            dtable[(size_t)k * width + c] = qmlb::from_f32<T>(t * scale);
+            for (int q = 0; q < JOIN_LANES; ++q) t += part[q][i];
+            if (c0 + i < width) dtable[(size_t)k * width + c0 + i] = qmlb::from_f32<T>(t * scale);
         }
         __syncthreads();
     }
@@ -276,13 +319,16 @@ int run_grad(const GradPlan &p, const T *dout, const void *index, int bits, cons
     int *tail_key = reinterpret_cast<int *>(scratch);
     float *pieces = reinterpret_cast<float *>(scratch + (((size_t)p.blocks * 4 + 255) & ~(size_t)255));
     const size_t smem = (size_t)((2 * p.block + 2 + 3) & ~3) * 4 + (size_t)p.r * 2 * p.tc * VEC * 4;
-    dim3 grid(p.blocks > p.zero_blocks ? p.blocks : p.zero_blocks, p.col_blocks);
+    dim3 grid(p.blocks + p.zero_blocks, p.col_blocks);
     if (int rc = qmlb::ensure_smem(grad_kernel<T, VEC>, smem, "qmlb_embedding_grad")) return rc;
-    grad_kernel<T, VEC><<<grid, THREADS, smem, st>>>(dout, index, bits, order, start, (unsigned)n, nkeys, p.chunks, p.tc, p.run, scale, dtable,
+    grad_kernel<T, VEC><<<grid, THREADS, smem, st>>>(dout, index, bits, order, start, (unsigned)n, nkeys, p.chunks, p.tc, p.run, p.blocks, scale, dtable,
                                                     tail_key, pieces);
     if (p.blocks > 1) {
-        const unsigned cb = (unsigned)((width + 31) / 32);
-        join_kernel<T><<<dim3(p.blocks - 1, cb < 8 ? cb : 8), 32 * JOIN_LANES, 0, st>>>(tail_key, pieces, start, p.blocks, p.block, width, scale, dtable);
+        const bool wide = (width & 3) == 0;
+        const unsigned cb = (unsigned)((width + (wide ? 127 : 31)) / (wide ? 128 : 32));
+        const dim3 jg(p.blocks - 1, cb < 4 ? cb : 4);
+        if (wide) join_kernel<T, 4><<<jg, JOIN_THREADS, 0, st>>>(tail_key, pieces, start, p.blocks, p.block, width, scale, dtable);
+        else join_kernel<T, 1><<<jg, JOIN_THREADS, 0, st>>>(tail_key, pieces, start, p.blocks, p.block, width, scale, dtable);
     }
     return qmlb::check_launch("qmlb_embedding_grad");
 }

@@ -3,7 +3,7 @@
 // the key nkeys: they come behind all groups, in their original order.
 //
 // Least-significant-digit radix sort with digits of at most RADIX_BITS bits, so up to 1,023 keys (every element or
-// species numbering) take ONE pass and 1,048,575 take two.  A pass over blocks of TILE keys:
+// species numbering) take ONE pass and 1,048,575 take two.  A pass over blocks of 1,024 or 4,096 keys:
 //   1. histogram : counts[digit][block]
 //   2. scan      : one block per digit turns its row into an exclusive prefix over the blocks and writes the digit's total
 //   3. scatter   : every block ranks its keys again (the same order, so the result never depends on scheduling) and
