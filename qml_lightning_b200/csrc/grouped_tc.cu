@@ -59,7 +59,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
 
     if (tid == 0) {
         for (int s = 0; s < p.stages; ++s) {
-            mbar_init(bar(full[s]), LOADED ? 1 + LOAD_WARPS : 1);        // the TMA issuer, and the loading warps
+            mbar_init(bar(full[s]), LOADED ? 1 + LOAD_WARPS * 32 : 1);        // the TMA issuer, and the loading threads
             mbar_init(bar(empty[s]), 1);
         }
         for (int i = 0; i < 2; ++i) { mbar_init(bar(acc_full[i]), 1); mbar_init(bar(acc_free[i]), EPI_WARPS); }
@@ -121,6 +121,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
                 const int s = it % p.stages;
                 w = w && mbar_wait(bar(full[s]), (uint32_t)(it / p.stages) & 1u, gave_up);
                 if (!__all_sync(QMLB_FULL_MASK, w)) { ok = false; break; }
+                if (LOADED) fence_async_smem();                     // copies and stores of the loading threads, as seen through the barrier
                 fence_after();
                 const uint32_t a = sbase + (uint32_t)s * stage_bytes, d = tmem + (uint32_t)buf * BUF_COLS;
                 const uint32_t al = desc_lo(a, 16), bl = desc_lo(a + A_BYTES, TRANS ? 16 : 8192);
@@ -198,14 +199,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
         const int t = tid - LOAD_WARP * 32;
         const unsigned char *src = reinterpret_cast<const unsigned char *>(in);
         const size_t row_bytes = (size_t)p.K * 2;
-        constexpr int AHEAD = 2;                                // stages whose copies are in flight behind the newest
         int it = 0;
         bool ok = true;
-        auto publish = [&](int i) {                             // this thread's copies of stage i have landed
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(full[i % p.stages]));
-        };
         for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
             int g, row0, row1;
             locate(tile, g, row0, row1);
@@ -215,15 +210,15 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
                 if (!ok) break;
                 const uint32_t a = sbase + (uint32_t)s * stage_bytes;
                 load_box<BM, LOAD_WARPS * 32>(src, row_bytes, row0, p.n, (size_t)c * BK * 2, a, t, p.in_access);
-                cp_async_commit();
-                if (it >= AHEAD) {
-                    cp_async_wait<AHEAD>();
-                    publish(it - AHEAD);
+                if (p.in_access >= 4) {
+                    cp_async_arrive(bar(full[s]));              // when this thread's copies have landed
+                } else {                                        // plain stores among them
+                    cp_async_wait<0>();
+                    mbar_arrive(bar(full[s]));
                 }
             }
         }
-        cp_async_wait<0>();
-        for (int i = max(0, it - AHEAD); i < it; ++i) publish(i);
+        cp_async_wait<0>();                                     // no copy may be in flight when the block leaves
         if (!ok) failed = 1;
     }
     __syncwarp();

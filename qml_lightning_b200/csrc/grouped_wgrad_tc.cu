@@ -59,7 +59,7 @@ wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
 
     if (tid == 0) {
         for (int s = 0; s < p.stages; ++s) {
-            mbar_init(bar(full[s]), LOADED ? 1 + LOAD_WARPS : 1);
+            mbar_init(bar(full[s]), LOADED ? 1 + LOAD_WARPS * 32 : 1);
             mbar_init(bar(empty[s]), 1);
         }
         for (int i = 0; i < 2; ++i) { mbar_init(bar(acc_full[i]), 1); mbar_init(bar(acc_free[i]), EPI_WARPS); }
@@ -134,6 +134,7 @@ wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
                     fence_async_smem();
                     __syncwarp();
                 }
+                if (LOADED) fence_async_smem();                       // copies and stores of the loading threads, as seen through the barrier
                 fence_after();
                 const uint32_t al = desc_lo(a, BOX), bl = desc_lo(a + 2 * BOX, BOX), d = tmem + (uint32_t)buf * BUF_COLS;
                 if (elect_one()) {
@@ -218,14 +219,8 @@ wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
     } else if (LOADED && warp >= LOAD_WARP) {
         const int t = tid - LOAD_WARP * 32;
         const unsigned char *xs = reinterpret_cast<const unsigned char *>(x), *ds = reinterpret_cast<const unsigned char *>(dy);
-        constexpr int AHEAD = 2;
         int it = 0;
         bool ok = true;
-        auto publish = [&](int i) {
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(full[i % p.stages]));
-        };
         for (int unit = blockIdx.x; unit < total && ok; unit += gridDim.x) {
             int g, r0, r1, k0, n0;
             locate(unit, g, r0, r1, k0, n0);
@@ -241,15 +236,15 @@ wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
                 if (!tma_dy)
                     for (int q = 0; q < db; ++q)
                         load_box<BK, LOAD_WARPS * 32>(ds, (size_t)p.N * 2, r, r1, (size_t)(n0 + q * 64) * 2, b + (uint32_t)q * BOX, t, p.dy_access);
-                cp_async_commit();
-                if (it >= AHEAD) {
-                    cp_async_wait<AHEAD>();
-                    publish(it - AHEAD);
+                if (min(p.x_access, p.dy_access) >= 4) {
+                    cp_async_arrive(bar(full[s]));              // when this thread's copies have landed
+                } else {                                        // plain stores among them
+                    cp_async_wait<0>();
+                    mbar_arrive(bar(full[s]));
                 }
             }
         }
-        cp_async_wait<0>();
-        for (int i = max(0, it - AHEAD); i < it; ++i) publish(i);
+        cp_async_wait<0>();                                     // no copy may be in flight when the block leaves
         if (!ok) failed = 1;
     }
     __syncwarp();

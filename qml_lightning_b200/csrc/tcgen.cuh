@@ -73,8 +73,12 @@ __device__ __forceinline__ void cp_async(uint32_t dst, const void *src, bool wan
         asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(__cvta_generic_to_global(src)), "n"(BYTES), "r"(n) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// arrive on the barrier once this thread's copies so far have landed
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
 template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.commit_group;\n\tcp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // Shared-memory matrix descriptors with the 128-byte swizzle.  High word: offset between groups of eight 128-byte lines
 // (1,024 bytes), descriptor version 1, swizzle mode 2.  Low word: address, and offset between blocks of 64 elements along
