@@ -24,6 +24,11 @@ using namespace qmlb::tc;
 
 constexpr int BM = 128;                          // rows per tile
 constexpr uint32_t A_BYTES = BM * BK * 2;
+// Pairs of blocks fetch half of the matrix each, which pays when the sums are deep and the groups fill tiles of 256 rows.  Measured
+// (bf16): 65,536 rows of 8 groups, 2,048 x 2,048: 508 -> 474 us, transposed 443 -> 395; 210,000 rows, 1,024 deep, 256 columns: 126 ->
+// 116; but 256 deep, 784 columns (330,000 rows): 193 -> 238, and 336 deep, 256 columns (210,000 rows): 62 -> 70.
+constexpr int PAIR_DEPTH = 768;
+constexpr size_t PAIR_ROWS = 512;                // rows per group, on average
 constexpr int TMA_WARP = 0, MMA_WARP = 1, EPI_WARP = 4, LOAD_WARP = EPI_WARP + EPI_WARPS, LOAD_WARPS = 8;
 constexpr int NTHREADS = LOAD_WARP * 32, NTHREADS_LOADED = NTHREADS + LOAD_WARPS * 32;
 
@@ -38,7 +43,7 @@ struct Shape {
     int out_access;
 };
 
-template <typename T, bool TRANS, bool LOADED>
+template <typename T, bool TRANS, bool LOADED, bool PAIR>
 __global__ void __launch_bounds__(LOADED ? NTHREADS_LOADED : NTHREADS, 1)
 grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant__ CUtensorMap map_w, const T *__restrict__ in,
                const int *__restrict__ start, Shape p, T *__restrict__ out) {
@@ -56,29 +61,37 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
     gr.parts = gr.start + p.G + 1;
     gr.split = nullptr;
     auto bar = [](const uint64_t &b) { return smem_u32(&b); };
+    static_assert(!(LOADED && PAIR), "pairs fetch their rows by TMA");
+    constexpr int BLOCKS = PAIR ? 2 : 1, TILE_ROWS = BM * BLOCKS;
+    const uint32_t rank = PAIR ? cluster_rank() : 0;            // the even block of a pair issues
+    const int unit0 = blockIdx.x / BLOCKS, units = gridDim.x / BLOCKS;
 
     if (tid == 0) {
         for (int s = 0; s < p.stages; ++s) {
             mbar_init(bar(full[s]), LOADED ? 1 + LOAD_WARPS * 32 : 1);        // the TMA issuer, and the loading threads
             mbar_init(bar(empty[s]), 1);
         }
-        for (int i = 0; i < 2; ++i) { mbar_init(bar(acc_full[i]), 1); mbar_init(bar(acc_free[i]), EPI_WARPS); }
+        for (int i = 0; i < 2; ++i) { mbar_init(bar(acc_full[i]), 1); mbar_init(bar(acc_free[i]), EPI_WARPS * BLOCKS); }
         mbar_init(bar(done), 1);
         failed = 0;
         mbar_init_fence();
         if (!LOADED) prefetch_map(&map_in);
         prefetch_map(&map_w);
     }
-    if (warp == MMA_WARP) tmem_alloc(smem_u32(&tmem_slot), TMEM_COLS);
+    if (warp == MMA_WARP) {
+        if (PAIR) tmem_alloc_pair(smem_u32(&tmem_slot), TMEM_COLS);
+        else tmem_alloc(smem_u32(&tmem_slot), TMEM_COLS);
+    }
     fence_before();
-    read_groups(gr, start, p.G, p.n, BM);
+    read_groups(gr, start, p.G, p.n, TILE_ROWS);
+    if (PAIR) cluster_sync();                                   // both blocks' barriers are ready
     fence_after();
     const uint32_t tmem = tmem_slot;
     const int total = gr.parts[p.G] * p.ntiles;
     auto locate = [&](int tile, int &g, int &row0, int &row1) {
         const int mt = tile / p.ntiles;
         g = gr.find(p.G, mt);
-        row0 = gr.start[g] + (mt - gr.parts[g]) * BM;
+        row0 = gr.start[g] + (mt - gr.parts[g]) * TILE_ROWS + (int)rank * BM;
         row1 = gr.start[g + 1];
     };
     const volatile int *gave_up = &failed;
@@ -87,34 +100,48 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
         if (lane == 0) {
             int it = 0;
             bool ok = true;
-            for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+            for (int tile = unit0; tile < total && ok; tile += units) {
                 int g, row0, row1;
                 locate(tile, g, row0, row1);
                 const int col0 = (tile % p.ntiles) * p.NT;
-                // forward: boxes of 64 columns by 64 deep, as many as reach into the matrix; transposed: one box of NT rows
-                const int boxes = TRANS ? 1 : min((p.NT + 63) / 64, (p.out - col0 + 63) / 64);
-                const uint32_t bytes = (LOADED ? 0u : A_BYTES) + (TRANS ? p.b_bytes : (uint32_t)boxes * 8192u);
+                // Forward: boxes of 64 columns by 64 deep, as many as reach into the matrix; transposed: one box of the block's rows.
+                // The even block of a pair expects what both fetch.
+                const int own = p.NT / BLOCKS, bcol = col0 + (int)rank * own;
+                auto boxes_at = [&](int col) { return TRANS ? 1 : max(0, min((own + 63) / 64, (p.out - col + 63) / 64)); };
+                auto bytes_at = [&](int col) { return (LOADED ? 0u : A_BYTES) + (TRANS ? p.b_bytes : (uint32_t)boxes_at(col) * 8192u); };
+                const int boxes = boxes_at(bcol);
+                const uint32_t bytes = bytes_at(col0) + (PAIR ? bytes_at(col0 + own) : 0u);
                 for (int c = 0; c < p.nchunks; ++c, ++it) {
                     const int s = it % p.stages;
                     if (!mbar_wait(bar(empty[s]), ((uint32_t)(it / p.stages) & 1u) ^ 1u, gave_up)) { ok = false; break; }
                     const uint32_t a = sbase + (uint32_t)s * stage_bytes, b = a + A_BYTES;
-                    mbar_expect_tx(bar(full[s]), bytes);
-                    if (!LOADED) tma_2d(a, &map_in, c * BK, row0, bar(full[s]));
-                    if (TRANS) tma_3d(b, &map_w, c * BK, col0, g, bar(full[s]));
-                    else
-                        for (int j = 0; j < boxes; ++j) tma_3d(b + (uint32_t)j * 8192u, &map_w, col0 + j * 64, c * BK, g, bar(full[s]));
+                    if (rank == 0) mbar_expect_tx(bar(full[s]), bytes);
+                    if (PAIR) {
+                        const uint32_t to = map_rank(bar(full[s]), 0);
+                        tma_2d_pair(a, &map_in, c * BK, row0, to);
+                        if (TRANS) tma_3d_pair(b, &map_w, c * BK, bcol, g, to);
+                        else
+                            for (int j = 0; j < boxes; ++j) tma_3d_pair(b + (uint32_t)j * 8192u, &map_w, bcol + j * 64, c * BK, g, to);
+                    } else {
+                        if (!LOADED) tma_2d(a, &map_in, c * BK, row0, bar(full[s]));
+                        if (TRANS) tma_3d(b, &map_w, c * BK, bcol, g, bar(full[s]));
+                        else
+                            for (int j = 0; j < boxes; ++j) tma_3d(b + (uint32_t)j * 8192u, &map_w, bcol + j * 64, c * BK, g, bar(full[s]));
+                    }
                 }
             }
             if (!ok) failed = 1;
             // no copy may be in flight when the block leaves
-            for (int i = max(0, it - p.stages); i < it; ++i)
+            for (int i = max(0, it - p.stages); i < it && rank == 0; ++i)
                 for (int tries = 0; tries < WAIT_LIMIT && !mbar_try(bar(full[i % p.stages]), (uint32_t)(i / p.stages) & 1u); ++tries) {}
         }
+    } else if (warp == MMA_WARP && rank != 0) {
+        // the even block issues for both
     } else if (warp == MMA_WARP) {
-        const uint32_t idesc = instr_desc(sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value, false, !TRANS, BM, p.NT);
+        const uint32_t idesc = instr_desc(std::is_same<T, __nv_bfloat16>::value, false, !TRANS, TILE_ROWS, p.NT);
         int it = 0, j = 0;
         bool ok = true;
-        for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x, ++j) {
+        for (int tile = unit0; tile < total && ok; tile += units, ++j) {
             const int buf = j & 1;
             bool w = mbar_wait(bar(acc_free[buf]), ((uint32_t)(j >> 1) & 1u) ^ 1u, gave_up);
             for (int c = 0; c < p.nchunks; ++c, ++it) {
@@ -128,16 +155,25 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
                 constexpr uint32_t b_step = TRANS ? 2u : 128u;              // 16 deep: 32 bytes along the lines, or 16 lines
                 if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < BK / 16; ++k)
-                        mma_f16(d, al + k * 2u, DESC_HI_SW128, bl + k * b_step, DESC_HI_SW128, idesc, (c | k) ? 1u : 0u);
-                    mma_commit(bar(empty[s]));
-                    if (c == p.nchunks - 1) mma_commit(bar(acc_full[buf]));
+                    for (int k = 0; k < BK / 16; ++k) {
+                        if (PAIR) mma_f16_pair(d, al + k * 2u, DESC_HI_SW128, bl + k * b_step, DESC_HI_SW128, idesc, (c | k) ? 1u : 0u);
+                        else mma_f16(d, al + k * 2u, DESC_HI_SW128, bl + k * b_step, DESC_HI_SW128, idesc, (c | k) ? 1u : 0u);
+                    }
+                    if (PAIR) mma_commit_pair(bar(empty[s]));
+                    else mma_commit(bar(empty[s]));
+                    if (c == p.nchunks - 1) {
+                        if (PAIR) mma_commit_pair(bar(acc_full[buf]));
+                        else mma_commit(bar(acc_full[buf]));
+                    }
                 }
                 __syncwarp();
             }
         }
         if (!ok) failed = 1;
-        if (lane == 0) mma_commit(bar(done));                   // everything issued has left the tensor pipe
+        if (lane == 0) {
+            if (PAIR) mma_commit_pair(bar(done));
+            else mma_commit(bar(done));                         // everything issued has left the tensor pipe
+        }
         __syncwarp();
         for (int tries = 0; tries < WAIT_LIMIT && !mbar_try(bar(done), 0u); ++tries) {}
     } else if (warp < EPI_WARP) {
@@ -153,9 +189,13 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
         const int quarter = warp & 3, c_first = ((warp - EPI_WARP) >> 2) * 32;
         unsigned char *mine = epi + (warp - EPI_WARP) * EPI_TILE;
         const size_t row_bytes = (size_t)p.out * 2;
+        auto release = [&](int buf) {                           // to the block that issues
+            if (PAIR) mbar_arrive_cluster(map_rank(bar(acc_free[buf]), 0));
+            else mbar_arrive(bar(acc_free[buf]));
+        };
         int j = 0;
         bool ok = true;
-        for (int tile = blockIdx.x; tile < total; tile += gridDim.x, ++j) {
+        for (int tile = unit0; tile < total; tile += units, ++j) {
             const int buf = j & 1;
             int g, row0, row1;
             locate(tile, g, row0, row1);
@@ -168,7 +208,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
             const uint32_t from = tmem + (uint32_t)buf * BUF_COLS + ((uint32_t)(quarter * 32) << 16);
             if (ok && c_first >= p.NT) {
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar(acc_free[buf]));
+                if (lane == 0) release(buf);
             }
             for (int c = c_first; c < p.NT; c += 64) {
                 uint32_t v[32];
@@ -181,7 +221,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
                     if (c + 64 >= p.NT) {                       // the accumulator is free once it sits in registers
                         fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(bar(acc_free[buf]));
+                        if (lane == 0) release(buf);
                     }
                 } else {
 #pragma unroll
@@ -201,7 +241,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
         const size_t row_bytes = (size_t)p.K * 2;
         int it = 0;
         bool ok = true;
-        for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+        for (int tile = unit0; tile < total && ok; tile += units) {
             int g, row0, row1;
             locate(tile, g, row0, row1);
             for (int c = 0; c < p.nchunks; ++c, ++it) {
@@ -213,12 +253,12 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
                 if (p.in_access >= 4) {
                     cp_async_arrive(bar(full[s]));              // when this thread's copies have landed
                 } else {                                        // plain stores among them
-                    cp_async_wait<0>();
+                    cp_async_wait_all();
                     mbar_arrive(bar(full[s]));
                 }
             }
         }
-        cp_async_wait<0>();                                     // no copy may be in flight when the block leaves
+        cp_async_wait_all();                                     // no copy may be in flight when the block leaves
         if (!ok) failed = 1;
     }
     __syncwarp();
@@ -226,7 +266,11 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
     __syncthreads();
     fence_after();
     if (tid == 0 && failed) atomicAdd(&g_timeouts, 1);
-    if (warp == MMA_WARP) tmem_free(tmem, TMEM_COLS);
+    if (PAIR) cluster_sync();                                   // neither block leaves while the other's instructions may read it
+    if (warp == MMA_WARP) {
+        if (PAIR) tmem_free_pair(tmem, TMEM_COLS);
+        else tmem_free(tmem, TMEM_COLS);
+    }
 }
 
 // W [G][K][N] with rows that no 16-byte access can follow -> the same with rows padded to a multiple of 8 elements
@@ -243,12 +287,27 @@ pad_kernel(const T *__restrict__ W, size_t rows, int N, int Np, T *__restrict__ 
 
 bool needs_pad(const void *W, int N) { return ((uintptr_t)W & 15) != 0 || (N & 7) != 0; }
 
-template <typename T, bool TRANS, bool LOADED>
+template <typename T, bool TRANS, bool LOADED, bool PAIR>
 int launch(const CUtensorMap &mi, const CUtensorMap &mw, const T *in, const int *start, const Shape &p, int blocks, T *out, cudaStream_t st) {
     const size_t smem = (size_t)p.stages * (A_BYTES + p.b_bytes) + EPI_BYTES + (size_t)2 * (p.G + 1) * 4 + 1024;
-    auto kernel = grouped_kernel<T, TRANS, LOADED>;
+    auto kernel = grouped_kernel<T, TRANS, LOADED, PAIR>;
     if (int rc = qmlb::ensure_smem(kernel, smem, "qmlb_grouped_matmul")) return rc;
-    kernel<<<blocks, LOADED ? NTHREADS_LOADED : NTHREADS, smem, st>>>(mi, mw, in, start, p, out);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(LOADED ? NTHREADS_LOADED : NTHREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = PAIR ? 2 : 1;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, mi, mw, in, start, p, out);
+    if (e != cudaSuccess) {
+        qmlb::set_error("qmlb_grouped_matmul: %s", cudaGetErrorString(e));
+        return QMLB_ERR_CUDA;
+    }
     return qmlb::check_launch("qmlb_grouped_matmul");
 }
 
@@ -266,12 +325,16 @@ int run(const void *x, const void *W, const int *start, size_t n, int G, int K, 
     // Columns per tile: as many as one accumulator holds, so that the rows are read once, in equal parts; fewer when the row
     // tiles alone do not give every SM a tile.
     const long mtiles = (long)((n + BM - 1) / BM);
+    const bool loaded = p.in_access < 16, pair = !loaded && p.K >= PAIR_DEPTH && n / G >= PAIR_ROWS && mtiles * ((p.out + 255) / 256) >= 2 * 148;
+    const int blocks_per_tile = pair ? 2 : 1;
     long nt = (p.out + 255) / 256;
     const long wanted = (148 + mtiles - 1) / mtiles, most = (p.out + 63) / 64;
     if (nt < wanted) nt = wanted < most ? wanted : most;
-    p.NT = (int)(((p.out + nt - 1) / nt + 15) / 16 * 16);
+    const int unit = 16 * blocks_per_tile;                     // each block of a pair holds half of the columns
+    p.NT = (int)(((p.out + nt - 1) / nt + unit - 1) / unit * unit);
     p.ntiles = (p.out + p.NT - 1) / p.NT;
-    p.b_bytes = transpose ? (uint32_t)p.NT * 128u : (uint32_t)((p.NT + 63) / 64) * 8192u;
+    const int own = p.NT / blocks_per_tile;
+    p.b_bytes = transpose ? (uint32_t)own * 128u : (uint32_t)((own + 63) / 64) * 8192u;
     p.b_bytes = (p.b_bytes + 1023u) & ~1023u;
     const size_t fixed = EPI_BYTES + (size_t)2 * (G + 1) * 4 + 1024 + 512;
     p.stages = (int)((SMEM_LIMIT - fixed) / (A_BYTES + p.b_bytes));
@@ -286,19 +349,19 @@ int run(const void *x, const void *W, const int *start, size_t n, int G, int K, 
         Wp = workspace;
     }
     CUtensorMap mi, mw;
-    if (int rc = qmlb::encode_tiles(&mw, Wp, bf16, (uint64_t)N, (uint64_t)K, (uint64_t)G, (uint64_t)Np * 2, transpose ? (uint32_t)p.NT : 64u,
+    if (int rc = qmlb::encode_tiles(&mw, Wp, bf16, (uint64_t)N, (uint64_t)K, (uint64_t)G, (uint64_t)Np * 2, transpose ? (uint32_t)own : 64u,
                                     "qmlb_grouped_matmul"))
         return rc;
-    const bool loaded = p.in_access < 16;
     mi = mw;
     if (!loaded)
         if (int rc = qmlb::encode_tiles(&mi, x, bf16, (uint64_t)p.K, (uint64_t)n, 0, (uint64_t)p.K * 2, BM, "qmlb_grouped_matmul")) return rc;
-    const long tiles = (mtiles + G) * p.ntiles;
+    const long tiles = ((long)((n + BM * blocks_per_tile - 1) / (BM * blocks_per_tile)) + G) * p.ntiles * blocks_per_tile;
     const int blocks = (int)(tiles < 148 ? tiles : 148);
     const T *xi = static_cast<const T *>(x);
     T *o = static_cast<T *>(out);
-    if (transpose) return loaded ? launch<T, true, true>(mi, mw, xi, start, p, blocks, o, st) : launch<T, true, false>(mi, mw, xi, start, p, blocks, o, st);
-    return loaded ? launch<T, false, true>(mi, mw, xi, start, p, blocks, o, st) : launch<T, false, false>(mi, mw, xi, start, p, blocks, o, st);
+    if (loaded) return transpose ? launch<T, true, true, false>(mi, mw, xi, start, p, blocks, o, st) : launch<T, false, true, false>(mi, mw, xi, start, p, blocks, o, st);
+    if (pair) return transpose ? launch<T, true, false, true>(mi, mw, xi, start, p, blocks, o, st) : launch<T, false, false, true>(mi, mw, xi, start, p, blocks, o, st);
+    return transpose ? launch<T, true, false, false>(mi, mw, xi, start, p, blocks, o, st) : launch<T, false, false, false>(mi, mw, xi, start, p, blocks, o, st);
 }
 
 }  // namespace

@@ -239,12 +239,12 @@ wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
                 if (min(p.x_access, p.dy_access) >= 4) {
                     cp_async_arrive(bar(full[s]));              // when this thread's copies have landed
                 } else {                                        // plain stores among them
-                    cp_async_wait<0>();
+                    cp_async_wait_all();
                     mbar_arrive(bar(full[s]));
                 }
             }
         }
-        cp_async_wait<0>();                                     // no copy may be in flight when the block leaves
+        cp_async_wait_all();                                     // no copy may be in flight when the block leaves
         if (!ok) failed = 1;
     }
     __syncwarp();

@@ -229,6 +229,27 @@ def test_larger_grouped_products(K, N, sizes, front, dtype):
 
 
 @pytest.mark.parametrize('dtype', R.TYPES)
+@pytest.mark.parametrize('K,N,sizes', [(136, 256, [30000, 9001, 2]), (64, 520, [20011, 5]), (520, 72, [39000]), (264, 264, [1, 21000, 0, 257, 128]),
+                                       (48, 304, [38000, 255, 129]), (781, 40, [38001]),
+                                       (776, 264, [20500, 1, 300]), (40, 1032, [6000, 5999])])
+def test_products_of_large_groups(K, N, sizes, dtype):
+    """Groups of tens of thousands of rows, tiles that end anywhere in a group, columns that end anywhere in a tile."""
+    g = gen(K * 3 + N)
+    n = sum(sizes) + 200
+    start = R.start_of(sizes, DEV, 7)
+    x, dy, W = randn(g, n, K, dtype=dtype), randn(g, n, N, dtype=dtype), (randn(g, len(sizes), K, N) / K ** 0.5).to(dtype)
+    y, dx, dW = ops().grouped_matmul(x, W, start, False), ops().grouped_matmul(dy, W, start, True), ops().grouped_matmul_wgrad(x, dy, start)
+    for name, got, (exact, mag, *terms), m in (('y', y, R.product(x, W, start), K), ('dx', dx, R.product(dy, W, start, True), N),
+                                               ('dW', dW, R.wgrad(x, dy, start), 0)):
+        R.assert_within(got, exact, R.sum_bound(exact, mag, terms[0] if terms else m, dtype), name)
+        longest = int(terms[0].max()) if terms else m
+        assert R.relative(got, exact) < (longest ** 0.5 + 16) * R.U + R.half_step(dtype)
+    assert torch.equal(dW, ops().grouped_matmul_wgrad(x, dy, start)) and torch.equal(y, ops().grouped_matmul(x, W, start, False))
+    from qml_lightning_b200 import cabi
+    assert cabi.tc_timeouts() == 0
+
+
+@pytest.mark.parametrize('dtype', R.TYPES)
 def test_products_of_misaligned_tensors(dtype):
     g = gen(5)
     sizes, K, N = [70, 0, 200], 64, 128
