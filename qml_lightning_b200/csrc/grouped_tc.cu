@@ -10,11 +10,17 @@
 // The matrices are read where they are: their rows run along N, which makes them an operand whose lines run along N in the
 // forward product and along K in the transposed one; the instruction takes both.  A row tile may reach over the end of its
 // group: those rows are read and multiplied (rows do not mix) and not stored.
-// Rows whose address is no multiple of 16 bytes (odd widths, offset views) cannot be fetched by TMA; then warps 12-19 bring
-// them with cp.async of 8 or 4 bytes, or 2-byte loads, into the same swizzled stages.
+// Rows whose address is no multiple of 16 bytes (odd widths, offset views) cannot be fetched by TMA one after the other.  Forward:
+// every PERIOD-th row (2, 4 or 8) has the same offset from a 16-byte boundary, so a tile takes 128 rows of one offset, by a tensor
+// map that starts at the boundary; its sums begin `shift` elements early, against zero rows of the matrix (coordinates in front of
+// its first row), and the issuing warp overwrites what the rows bring there.  (780 deep, 330,001 rows: 231 us with cp.async of
+// 8 bytes, 177 us so; 781 deep: 664 us with 2-byte loads, 181 us so.)  Transposed, the matrix's lines would have to move along, so warps 12-19 bring the rows with cp.async of 8 or
+// 4 bytes, or 2-byte loads, into the same swizzled stages.
 // Every wait is bounded; a block that gives up fills its remaining tiles with NaN and counts the event (qmlb_tc_timeouts).
 #include "grouped_tc.cuh"
 #include "grouped_rows.cuh"
+
+#include <string.h>
 
 #include <type_traits>
 
@@ -41,11 +47,15 @@ struct Shape {
     uint32_t b_bytes;        // one stage of the matrix operand
     int in_access;           // widest access that can follow the rows of `in` (16: TMA), in bytes
     int out_access;
+    int period;              // rows that lie at the same offset from a 16-byte boundary: every period-th
+    int shift[8];            // that offset, in elements
 };
 
-template <typename T, bool TRANS, bool LOADED, bool PAIR>
+struct RowMaps { CUtensorMap map[8]; };          // one per offset
+
+template <typename T, bool TRANS, bool LOADED, bool PAIR, bool SHIFTED>
 __global__ void __launch_bounds__(LOADED ? NTHREADS_LOADED : NTHREADS, 1)
-grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant__ CUtensorMap map_w, const T *__restrict__ in,
+grouped_kernel(const __grid_constant__ RowMaps maps, const __grid_constant__ CUtensorMap map_w, const T *__restrict__ in,
                const int *__restrict__ start, Shape p, T *__restrict__ out) {
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_free[2], done;
@@ -61,7 +71,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
     gr.parts = gr.start + p.G + 1;
     gr.split = nullptr;
     auto bar = [](const uint64_t &b) { return smem_u32(&b); };
-    static_assert(!(LOADED && PAIR), "pairs fetch their rows by TMA");
+    static_assert(LOADED + PAIR + SHIFTED <= 1 && !(SHIFTED && TRANS) && !(LOADED && !TRANS), "one way to fetch rows");
+    const int period = SHIFTED ? p.period : 1;
     constexpr int BLOCKS = PAIR ? 2 : 1, TILE_ROWS = BM * BLOCKS;
     const uint32_t rank = PAIR ? cluster_rank() : 0;            // the even block of a pair issues
     const int unit0 = blockIdx.x / BLOCKS, units = gridDim.x / BLOCKS;
@@ -75,7 +86,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
         mbar_init(bar(done), 1);
         failed = 0;
         mbar_init_fence();
-        if (!LOADED) prefetch_map(&map_in);
+        if (!LOADED) prefetch_map(&maps.map[0]);
         prefetch_map(&map_w);
     }
     if (warp == MMA_WARP) {
@@ -83,17 +94,21 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
         else tmem_alloc(smem_u32(&tmem_slot), TMEM_COLS);
     }
     fence_before();
-    read_groups(gr, start, p.G, p.n, TILE_ROWS);
+    read_groups(gr, start, p.G, p.n, TILE_ROWS * period);
     if (PAIR) cluster_sync();                                   // both blocks' barriers are ready
     fence_after();
     const uint32_t tmem = tmem_slot;
-    const int total = gr.parts[p.G] * p.ntiles;
-    auto locate = [&](int tile, int &g, int &row0, int &row1) {
-        const int mt = tile / p.ntiles;
-        g = gr.find(p.G, mt);
-        row0 = gr.start[g] + (mt - gr.parts[g]) * TILE_ROWS + (int)rank * BM;
+    const int total = gr.parts[p.G] * p.ntiles * period;
+    // tile -> group, first row of this block (the others follow in steps of `period`), end of the group, column tile
+    auto locate = [&](int tile, int &g, int &row0, int &row1, int &col0) {
+        const int mt = tile / p.ntiles, part = mt / period;
+        col0 = (tile - mt * p.ntiles) * p.NT;
+        g = gr.find(p.G, part);
+        row0 = gr.start[g] + ((part - gr.parts[g]) * TILE_ROWS + (int)rank * BM) * period + (mt - part * period);
         row1 = gr.start[g + 1];
     };
+    auto shift_of = [&](int row) { return SHIFTED ? p.shift[row % period] : 0; };
+    auto chunks_of = [&](int row) { return SHIFTED ? (p.K + shift_of(row) + BK - 1) / BK : p.nchunks; };
     const volatile int *gave_up = &failed;
 
     if (warp == TMA_WARP) {
@@ -101,9 +116,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
             int it = 0;
             bool ok = true;
             for (int tile = unit0; tile < total && ok; tile += units) {
-                int g, row0, row1;
-                locate(tile, g, row0, row1);
-                const int col0 = (tile % p.ntiles) * p.NT;
+                int g, row0, row1, col0;
+                locate(tile, g, row0, row1, col0);
                 // Forward: boxes of 64 columns by 64 deep, as many as reach into the matrix; transposed: one box of the block's rows.
                 // The even block of a pair expects what both fetch.
                 const int own = p.NT / BLOCKS, bcol = col0 + (int)rank * own;
@@ -111,22 +125,24 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
                 auto bytes_at = [&](int col) { return (LOADED ? 0u : A_BYTES) + (TRANS ? p.b_bytes : (uint32_t)boxes_at(col) * 8192u); };
                 const int boxes = boxes_at(bcol);
                 const uint32_t bytes = bytes_at(col0) + (PAIR ? bytes_at(col0 + own) : 0u);
-                for (int c = 0; c < p.nchunks; ++c, ++it) {
+                const int chunks = chunks_of(row0), shift = shift_of(row0);
+                const CUtensorMap *rows_map = &maps.map[SHIFTED ? row0 % period : 0];
+                for (int c = 0; c < chunks; ++c, ++it) {
                     const int s = it % p.stages;
                     if (!mbar_wait(bar(empty[s]), ((uint32_t)(it / p.stages) & 1u) ^ 1u, gave_up)) { ok = false; break; }
                     const uint32_t a = sbase + (uint32_t)s * stage_bytes, b = a + A_BYTES;
                     if (rank == 0) mbar_expect_tx(bar(full[s]), bytes);
                     if (PAIR) {
                         const uint32_t to = map_rank(bar(full[s]), 0);
-                        tma_2d_pair(a, &map_in, c * BK, row0, to);
+                        tma_2d_pair(a, rows_map, c * BK, row0, to);
                         if (TRANS) tma_3d_pair(b, &map_w, c * BK, bcol, g, to);
                         else
                             for (int j = 0; j < boxes; ++j) tma_3d_pair(b + (uint32_t)j * 8192u, &map_w, bcol + j * 64, c * BK, g, to);
                     } else {
-                        if (!LOADED) tma_2d(a, &map_in, c * BK, row0, bar(full[s]));
+                        if (!LOADED) tma_2d(a, rows_map, c * BK, row0 / period, bar(full[s]));
                         if (TRANS) tma_3d(b, &map_w, c * BK, bcol, g, bar(full[s]));
                         else
-                            for (int j = 0; j < boxes; ++j) tma_3d(b + (uint32_t)j * 8192u, &map_w, bcol + j * 64, c * BK, g, bar(full[s]));
+                            for (int j = 0; j < boxes; ++j) tma_3d(b + (uint32_t)j * 8192u, &map_w, bcol + j * 64, c * BK - shift, g, bar(full[s]));
                     }
                 }
             }
@@ -143,11 +159,25 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
         bool ok = true;
         for (int tile = unit0; tile < total && ok; tile += units, ++j) {
             const int buf = j & 1;
+            int chunks = p.nchunks, shift = 0;
+            if (SHIFTED) {
+                int g, row0, row1, col0;
+                locate(tile, g, row0, row1, col0);
+                chunks = chunks_of(row0);
+                shift = shift_of(row0);
+            }
             bool w = mbar_wait(bar(acc_free[buf]), ((uint32_t)(j >> 1) & 1u) ^ 1u, gave_up);
-            for (int c = 0; c < p.nchunks; ++c, ++it) {
+            for (int c = 0; c < chunks; ++c, ++it) {
                 const int s = it % p.stages;
                 w = w && mbar_wait(bar(full[s]), (uint32_t)(it / p.stages) & 1u, gave_up);
                 if (!__all_sync(QMLB_FULL_MASK, w)) { ok = false; break; }
+                if (SHIFTED && c == 0 && shift) {                   // what lies in front of the rows is not theirs
+                    unsigned char *rows = sp + (size_t)s * stage_bytes;
+                    for (int r = lane; r < BM; r += 32)
+                        for (int i = 0; i < shift; ++i) *reinterpret_cast<uint16_t *>(rows + r * 128 + ((r & 7) << 4) + i * 2) = 0;
+                    fence_async_smem();
+                    __syncwarp();
+                }
                 if (LOADED) fence_async_smem();                     // copies and stores of the loading threads, as seen through the barrier
                 fence_after();
                 const uint32_t a = sbase + (uint32_t)s * stage_bytes, d = tmem + (uint32_t)buf * BUF_COLS;
@@ -161,7 +191,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
                     }
                     if (PAIR) mma_commit_pair(bar(empty[s]));
                     else mma_commit(bar(empty[s]));
-                    if (c == p.nchunks - 1) {
+                    if (c == chunks - 1) {
                         if (PAIR) mma_commit_pair(bar(acc_full[buf]));
                         else mma_commit(bar(acc_full[buf]));
                     }
@@ -188,7 +218,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
         // warps w and w + 4 share a quarter of the rows and take every other 32 columns
         const int quarter = warp & 3, c_first = ((warp - EPI_WARP) >> 2) * 32;
         unsigned char *mine = epi + (warp - EPI_WARP) * EPI_TILE;
-        const size_t row_bytes = (size_t)p.out * 2;
+        const size_t row_bytes = (size_t)p.out * 2, row_step = row_bytes * period;
         auto release = [&](int buf) {                           // to the block that issues
             if (PAIR) mbar_arrive_cluster(map_rank(bar(acc_free[buf]), 0));
             else mbar_arrive(bar(acc_free[buf]));
@@ -197,10 +227,10 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
         bool ok = true;
         for (int tile = unit0; tile < total; tile += units, ++j) {
             const int buf = j & 1;
-            int g, row0, row1;
-            locate(tile, g, row0, row1);
-            const int col0 = (tile % p.ntiles) * p.NT, row = row0 + quarter * 32;
-            const int rows = min(32, row1 - row);
+            int g, row0, row1, col0;
+            locate(tile, g, row0, row1, col0);
+            const int row = row0 + quarter * 32 * period;
+            const int rows = min(32, (row1 - row + period - 1) / period);
             ok = ok && mbar_wait(bar(acc_full[buf]), (uint32_t)(j >> 1) & 1u, gave_up);
             ok = __all_sync(QMLB_FULL_MASK, ok);
             if (!ok) failed = 1;                                // at once: the other roles stop waiting
@@ -231,7 +261,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
                 __syncwarp();
                 const int bytes = min(min(32, left), p.out - col0 - c) * 2;
                 unsigned char *to = reinterpret_cast<unsigned char *>(out) + (size_t)row * row_bytes + (size_t)(col0 + c) * 2;
-                store_tile(mine, to, row_bytes, rows, bytes, lane, p.out_access);
+                store_tile(mine, to, row_step, rows, bytes, lane, p.out_access);
                 __syncwarp();
             }
         }
@@ -242,8 +272,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap map_in, const __grid_constant
         int it = 0;
         bool ok = true;
         for (int tile = unit0; tile < total && ok; tile += units) {
-            int g, row0, row1;
-            locate(tile, g, row0, row1);
+            int g, row0, row1, col0;
+            locate(tile, g, row0, row1, col0);
             for (int c = 0; c < p.nchunks; ++c, ++it) {
                 const int s = it % p.stages;
                 ok = __all_sync(QMLB_FULL_MASK, mbar_wait(bar(empty[s]), ((uint32_t)(it / p.stages) & 1u) ^ 1u, gave_up));
@@ -287,10 +317,10 @@ pad_kernel(const T *__restrict__ W, size_t rows, int N, int Np, T *__restrict__ 
 
 bool needs_pad(const void *W, int N) { return ((uintptr_t)W & 15) != 0 || (N & 7) != 0; }
 
-template <typename T, bool TRANS, bool LOADED, bool PAIR>
-int launch(const CUtensorMap &mi, const CUtensorMap &mw, const T *in, const int *start, const Shape &p, int blocks, T *out, cudaStream_t st) {
+template <typename T, bool TRANS, bool LOADED, bool PAIR, bool SHIFTED>
+int launch(const RowMaps &mi, const CUtensorMap &mw, const T *in, const int *start, const Shape &p, int blocks, T *out, cudaStream_t st) {
     const size_t smem = (size_t)p.stages * (A_BYTES + p.b_bytes) + EPI_BYTES + (size_t)2 * (p.G + 1) * 4 + 1024;
-    auto kernel = grouped_kernel<T, TRANS, LOADED, PAIR>;
+    auto kernel = grouped_kernel<T, TRANS, LOADED, PAIR, SHIFTED>;
     if (int rc = qmlb::ensure_smem(kernel, smem, "qmlb_grouped_matmul")) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)blocks);
@@ -325,7 +355,7 @@ int run(const void *x, const void *W, const int *start, size_t n, int G, int K, 
     // Columns per tile: as many as one accumulator holds, so that the rows are read once, in equal parts; fewer when the row
     // tiles alone do not give every SM a tile.
     const long mtiles = (long)((n + BM - 1) / BM);
-    const bool loaded = p.in_access < 16, pair = !loaded && p.K >= PAIR_DEPTH && n / G >= PAIR_ROWS && mtiles * ((p.out + 255) / 256) >= 2 * 148;
+    const bool aligned = p.in_access == 16, shifted = !aligned && !transpose, loaded = !aligned && transpose, pair = aligned && p.K >= PAIR_DEPTH && n / G >= PAIR_ROWS && mtiles * ((p.out + 255) / 256) >= 2 * 148;
     const int blocks_per_tile = pair ? 2 : 1;
     long nt = (p.out + 255) / 256;
     const long wanted = (148 + mtiles - 1) / mtiles, most = (p.out + 63) / 64;
@@ -348,20 +378,42 @@ int run(const void *x, const void *W, const int *start, size_t n, int G, int K, 
         pad_kernel<T><<<(unsigned)(b < 2368 ? b : 2368), 256, 0, st>>>(static_cast<const T *>(W), (size_t)G * K, N, Np, static_cast<T *>(workspace));
         Wp = workspace;
     }
-    CUtensorMap mi, mw;
+    RowMaps mi;
+    CUtensorMap mw;
+    memset(&mi, 0, sizeof(mi));
     if (int rc = qmlb::encode_tiles(&mw, Wp, bf16, (uint64_t)N, (uint64_t)K, (uint64_t)G, (uint64_t)Np * 2, transpose ? (uint32_t)own : 64u,
                                     "qmlb_grouped_matmul"))
         return rc;
-    mi = mw;
-    if (!loaded)
-        if (int rc = qmlb::encode_tiles(&mi, x, bf16, (uint64_t)p.K, (uint64_t)n, 0, (uint64_t)p.K * 2, BM, "qmlb_grouped_matmul")) return rc;
-    const long tiles = ((long)((n + BM * blocks_per_tile - 1) / (BM * blocks_per_tile)) + G) * p.ntiles * blocks_per_tile;
+    const uint64_t row_bytes = (uint64_t)p.K * 2;
+    p.period = 1;
+    if (shifted) {
+        while ((row_bytes * p.period) & 15) p.period <<= 1;
+        if (p.period == 1) p.period = 2;                       // an offset view of aligned rows: a map's rows must not overlap
+    }
+    for (int q = 0; q < 8; ++q) {
+        const uintptr_t at = (uintptr_t)x + q * row_bytes;
+        p.shift[q] = (int)(at & 15) / 2;
+        if (loaded || q >= p.period) continue;
+        if ((uint64_t)q >= n) {                                // no such row: any valid map, nothing of it is stored
+            mi.map[q] = mi.map[0];
+            continue;
+        }
+        if (int rc = qmlb::encode_tiles(&mi.map[q], reinterpret_cast<const void *>(at & ~(uintptr_t)15), bf16, (uint64_t)(p.K + p.shift[q]),
+                                        (n - q + p.period - 1) / p.period, 0, row_bytes * p.period, BM, "qmlb_grouped_matmul"))
+            return rc;
+    }
+    const long rows_per_tile = (long)BM * blocks_per_tile * p.period;
+    const long tiles = ((long)((n + rows_per_tile - 1) / rows_per_tile) + G) * p.period * p.ntiles * blocks_per_tile;
     const int blocks = (int)(tiles < 148 ? tiles : 148);
     const T *xi = static_cast<const T *>(x);
     T *o = static_cast<T *>(out);
-    if (loaded) return transpose ? launch<T, true, true, false>(mi, mw, xi, start, p, blocks, o, st) : launch<T, false, true, false>(mi, mw, xi, start, p, blocks, o, st);
-    if (pair) return transpose ? launch<T, true, false, true>(mi, mw, xi, start, p, blocks, o, st) : launch<T, false, false, true>(mi, mw, xi, start, p, blocks, o, st);
-    return transpose ? launch<T, true, false, false>(mi, mw, xi, start, p, blocks, o, st) : launch<T, false, false, false>(mi, mw, xi, start, p, blocks, o, st);
+    if (loaded) return launch<T, true, true, false, false>(mi, mw, xi, start, p, blocks, o, st);
+    if (shifted) return launch<T, false, false, false, true>(mi, mw, xi, start, p, blocks, o, st);
+    if (pair)
+        return transpose ? launch<T, true, false, true, false>(mi, mw, xi, start, p, blocks, o, st)
+                         : launch<T, false, false, true, false>(mi, mw, xi, start, p, blocks, o, st);
+    return transpose ? launch<T, true, false, false, false>(mi, mw, xi, start, p, blocks, o, st)
+                     : launch<T, false, false, false, false>(mi, mw, xi, start, p, blocks, o, st);
 }
 
 }  // namespace

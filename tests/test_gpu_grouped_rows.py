@@ -284,22 +284,27 @@ def test_products_keep_magnitudes_apart(dtype):
     R.assert_within(y, exact, R.sum_bound(exact, mag, K, dtype), 'y')
 
 
-def test_values_that_are_not_finite_stay_in_their_rows():
+@pytest.mark.parametrize('K,N', [(64, 32), (63, 32), (60, 31), (66, 36)])
+def test_values_that_are_not_finite_stay_in_their_rows(K, N):
     g = gen(7)
     for dtype in R.TYPES:
-        x, W = randn(g, 300, 64, dtype=dtype), randn(g, 2, 64, 32, dtype=dtype)
-        start = R.start_of([130, 160], DEV)
-        x[5, 3], x[131, 60] = float('nan'), float('inf')
-        W[0, 0, 7] = float('inf')
-        y = ops().grouped_matmul(x, W, start, False)
-        bad = ~torch.isfinite(y)
-        assert bad[5].all() and bad[131].all() and bad[:130, 7].all()
-        bad[5], bad[131], bad[:130, 7] = False, False, False
-        assert not bad.any()
-        # a group's gradient is not touched by the rows of its neighbours
-        dy = randn(g, 300, 32, dtype=dtype)
-        dW = ops().grouped_matmul_wgrad(x[:, :], dy, R.start_of([5, 0, 100], DEV, 6))
-        assert torch.isfinite(dW).all()
+        for n in (300, 3000):
+            x, W = randn(g, n, K, dtype=dtype), randn(g, 2, K, N, dtype=dtype)
+            start = R.start_of([130, n - 140], DEV)
+            x[5], x[131, K - 2], x[n - 20, 0] = float('nan'), float('inf'), float('nan')
+            W[0, 0, 7] = float('inf')
+            y = ops().grouped_matmul(x, W, start, False)
+            bad = ~torch.isfinite(y)
+            assert bad[5].all() and bad[131].all() and bad[n - 20].all() and bad[:130, 7].all()
+            bad[5], bad[131], bad[n - 20], bad[:130, 7] = False, False, False, False
+            assert not bad.any()
+            dy = randn(g, n, N, dtype=dtype)
+            dy[77] = float('inf')
+            bad = ~torch.isfinite(ops().grouped_matmul(dy, randn(g, 2, K, N, dtype=dtype), start, True))
+            assert bad[77].all() and not bad[torch.arange(n, device=DEV) != 77].any()
+            # a group's gradient is not touched by the rows of its neighbours
+            dW = ops().grouped_matmul_wgrad(x, randn(g, n, N, dtype=dtype), R.start_of([5, 0, 100], DEV, 6))
+            assert torch.isfinite(dW).all()
 
 
 def test_bounds_outside_the_rows_are_clamped():
