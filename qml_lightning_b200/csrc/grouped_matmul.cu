@@ -25,7 +25,7 @@ __device__ __forceinline__ int clamped(const int *start, int g, int n) { return 
 // are in flight before the first is used (addresses are clamped instead of tested).
 constexpr int ROWS = 8;
 template <typename T, bool TRANS>
-__global__ void __launch_bounds__(TRANS ? 256 : 512)
+__global__ void __launch_bounds__(TRANS ? 256 : 512, TRANS ? 4 : 2)
 few_rows_kernel(const T *__restrict__ x, const T *__restrict__ W, const int *__restrict__ start, int G, int n, int K, int N, int w_cols,
                 T *__restrict__ y) {
     constexpr int WARPS = TRANS ? 8 : 16, THREADS = WARPS * 32, DEPTH = WARPS * 32, PER = 32;      // each warp: 32 of the depth

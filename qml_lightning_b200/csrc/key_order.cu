@@ -381,7 +381,8 @@ int run_cluster(const K *keys, size_t n, int nkeys, int *order, int *group_start
     cfg.dynamicSmemBytes = ((size_t)16 << nbits) + ((size_t)C_WARPS * 2 << nbits) + (nbits > 5 ? (size_t)8 * C_THREADS * items : 0);
     if (blocks > 8 && cudaFuncSetAttribute(cluster_kernel<K>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
         return qmlb::check_launch("qmlb_group_by_key(cluster size)");
-    if (int rc = qmlb::ensure_smem(cluster_kernel<K>, cfg.dynamicSmemBytes, "qmlb_group_by_key")) return rc;
+    // (1 KB more: the kernel's own variables count towards the 48 KB that need no opting in)
+    if (int rc = qmlb::ensure_smem(cluster_kernel<K>, cfg.dynamicSmemBytes + 1024, "qmlb_group_by_key")) return rc;
     cfg.stream = st;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeClusterDimension;

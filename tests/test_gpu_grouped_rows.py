@@ -33,8 +33,8 @@ def misaligned(t):
 
 
 # ---- order by key ---------------------------------------------------------------------------------------------------
-@pytest.mark.parametrize('nkeys', [1, 2, 3, 5, 31, 255, 1023, 1024, 50021, 1048575, 2100000])
-@pytest.mark.parametrize('n', [1, 2, 31, 33, 257, 4095, 4097, 8193, 70001])
+@pytest.mark.parametrize('nkeys', [1, 2, 3, 5, 31, 255, 300, 511, 1023, 1024, 50021, 1048575, 2100000])
+@pytest.mark.parametrize('n', [1, 2, 31, 33, 257, 1024, 1025, 4095, 4097, 8193, 70001])
 def test_order_is_stable(n, nkeys):
     g = gen(n * 7 + nkeys)
     for dtype in (torch.int32, torch.int64):
