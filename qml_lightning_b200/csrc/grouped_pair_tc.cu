@@ -202,7 +202,7 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
                 for (int c = 0; c < chunks; ++c, ++it) {
                     const int s = it % p.stages, buf = it % NACC;
                     bool w = mbar_wait(bar(acc_free[buf]), ((uint32_t)(it / NACC) & 1u) ^ 1u, gave_up);
-                    w = w && mbar_wait(bar(full[s]), (uint32_t)(it / p.stages) & 1u, gave_up);
+                    w = w && mbar_wait(bar(full[s]), (uint32_t)(it / p.stages) & 1u, gave_up, it ? WAIT_LIMIT : QMLB_TEST_FIRST_WAIT_POLLS);
                     if (!__all_sync(QMLB_FULL_MASK, w)) { ok = false; break; }
                     fence_after();
                     const int steps = min(BK / 16, (depth - c * BK + 15) / 16);

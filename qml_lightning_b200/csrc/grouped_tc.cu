@@ -169,7 +169,7 @@ grouped_kernel(const __grid_constant__ RowMaps maps, const __grid_constant__ CUt
             bool w = mbar_wait(bar(acc_free[buf]), ((uint32_t)(j >> 1) & 1u) ^ 1u, gave_up);
             for (int c = 0; c < chunks; ++c, ++it) {
                 const int s = it % p.stages;
-                w = w && mbar_wait(bar(full[s]), (uint32_t)(it / p.stages) & 1u, gave_up);
+                w = w && mbar_wait(bar(full[s]), (uint32_t)(it / p.stages) & 1u, gave_up, it ? WAIT_LIMIT : QMLB_TEST_FIRST_WAIT_POLLS);
                 if (!__all_sync(QMLB_FULL_MASK, w)) { ok = false; break; }
                 if (SHIFTED && c == 0 && shift) {                   // what lies in front of the rows is not theirs
                     unsigned char *rows = sp + (size_t)s * stage_bytes;

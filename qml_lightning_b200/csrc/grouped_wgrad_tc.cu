@@ -122,7 +122,7 @@ wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
             bool w = mbar_wait(bar(acc_free[buf]), ((uint32_t)(j >> 1) & 1u) ^ 1u, gave_up);
             for (int r = r0; r < r1; r += BK, ++it) {
                 const int s = it % p.stages;
-                w = w && mbar_wait(bar(full[s]), (uint32_t)(it / p.stages) & 1u, gave_up);
+                w = w && mbar_wait(bar(full[s]), (uint32_t)(it / p.stages) & 1u, gave_up, it ? WAIT_LIMIT : QMLB_TEST_FIRST_WAIT_POLLS);
                 if (!__all_sync(QMLB_FULL_MASK, w)) { ok = false; break; }
                 const uint32_t a = sbase + (uint32_t)s * stage_bytes;
                 const int valid = min(BK, r1 - r), steps = (valid + 15) >> 4;

@@ -10,6 +10,11 @@ namespace qmlb {
 namespace tc {
 
 constexpr int WAIT_LIMIT = 1 << 22;            // polls of one wait before a block gives up
+// Polls granted to the first wait for operands.  The failure-detection test builds the kernels with none, so that this one wait
+// runs out before anything was issued and the give-up path runs (NaN results, copies drained, tensor memory freed, event counted).
+#ifndef QMLB_TEST_FIRST_WAIT_POLLS
+#define QMLB_TEST_FIRST_WAIT_POLLS WAIT_LIMIT
+#endif
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
@@ -34,9 +39,8 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     return ok != 0;
 }
 // Bounded parity wait.  False when the limit is reached, or when another role of the block has given up.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const volatile int *failed) {
-    if (mbar_try(bar, parity)) return true;
-    for (int it = 0; it < WAIT_LIMIT; ++it) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const volatile int *failed, int limit = WAIT_LIMIT) {
+    for (int it = 0; it < limit; ++it) {
         if (mbar_try(bar, parity)) return true;
         if ((it & 255) == 255 && *failed) return false;
     }
