@@ -384,7 +384,8 @@ int qmlb_unpack_upper(const double *packed, int F, double *ZTZ, qmlb_stream_t st
  *   order i32[n]              positions of the keys by ascending key, equal keys in their original order; keys outside
  *                             [0, nkeys) (-1 for a padded slot) follow behind all groups, in their original order
  *   group_start i32[nkeys+1]  first position of every key; group_start[nkeys] = number of keys inside [0, nkeys)
- * n < 2^31, 0 < nkeys < 2^31 - 1.  scratch: qmlb_group_by_key_scratch_bytes bytes of device memory, 4-byte aligned. */
+ * n < 2^31, 0 < nkeys < 2^31 - 1.  scratch: qmlb_group_by_key_scratch_bytes bytes of device memory, 4-byte aligned (here and
+ * below a size of 0 means that none is needed and NULL will do). */
 size_t qmlb_group_by_key_scratch_bytes(size_t n, int nkeys);
 int qmlb_group_by_key(const void *keys, int key_bits, size_t n, int nkeys, int *order, int *group_start, void *scratch,
                       size_t scratch_bytes, qmlb_stream_t stream);

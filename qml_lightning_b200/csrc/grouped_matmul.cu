@@ -162,8 +162,8 @@ bool few_rows_grad(size_t n, int G, int K, int N, int dtype) {
 }  // namespace
 
 extern "C" size_t qmlb_grouped_matmul_workspace_bytes(size_t n, int ngroups, int K, int N, int dtype, int transpose) {
-    if (n == 0 || ngroups <= 0 || K <= 0 || N <= 0) return 256;
-    if (dtype == QMLB_F32) return few_rows(n, ngroups, K, N) ? 256 : qmlb::grouped_pair_workspace(n, ngroups, K, N, transpose);
+    if (n == 0 || ngroups <= 0 || K <= 0 || N <= 0) return 0;
+    if (dtype == QMLB_F32) return few_rows(n, ngroups, K, N) ? 0 : qmlb::grouped_pair_workspace(n, ngroups, K, N, transpose);
     return qmlb::grouped_tc_workspace(ngroups, K, N);
 }
 
@@ -187,8 +187,8 @@ extern "C" int qmlb_grouped_matmul(const void *x, const void *W, const int *grou
 }
 
 extern "C" size_t qmlb_grouped_matmul_wgrad_workspace_bytes(size_t n, int ngroups, int K, int N, int dtype) {
-    if (n == 0 || ngroups <= 0 || K <= 0 || N <= 0) return 256;
-    if (few_rows_grad(n, ngroups, K, N, dtype)) return 256;
+    if (n == 0 || ngroups <= 0 || K <= 0 || N <= 0) return 0;
+    if (few_rows_grad(n, ngroups, K, N, dtype)) return 0;
     if (dtype == QMLB_F32) return qmlb::grouped_wgrad_pair_workspace(n, ngroups, K, N);
     return qmlb::grouped_wgrad_tc_workspace(n, ngroups, K, N);
 }

@@ -256,8 +256,8 @@ wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
 }
 
 // Groups of several parts: their sum, in order.  Groups without rows: zeros.  blockIdx.y walks the groups; `row` is the
-// row length of the parts.
-template <typename T>
+// row length of the parts.  VEC columns per thread: four, or one where that leaves too few threads to hide the latency.
+template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
 join_kernel(const int *__restrict__ start, const float *__restrict__ partial, int n, int G, int K, int N, int split, size_t row, T *__restrict__ dW) {
     extern __shared__ int sm[];
@@ -266,32 +266,38 @@ join_kernel(const int *__restrict__ start, const float *__restrict__ partial, in
     gr.parts = sm + G + 1;
     gr.split = gr.parts + G + 1;
     read_groups(gr, start, G, n, split);
+    const unsigned per_row = ((unsigned)N + VEC - 1u) / VEC;
     for (int g = blockIdx.y; g < G; g += gridDim.y) {
         const int parts = gr.parts[g + 1] - gr.parts[g];
         if (parts == 1) continue;
-        const unsigned per_row = ((unsigned)N + 3u) / 4u;
         for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < (size_t)K * per_row; i += (size_t)gridDim.x * 256) {
-            const unsigned k = (unsigned)(i / per_row), c = (unsigned)(i - (size_t)k * per_row) * 4u;
+            const unsigned k = (unsigned)(i / per_row), c = (unsigned)(i - (size_t)k * per_row) * VEC;
             const float *src = partial + ((size_t)gr.split[g] * K + k) * row + c;
-            float s[4] = {0.f, 0.f, 0.f, 0.f};
+            float s[VEC], v[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) s[e] = 0.f;
 #pragma unroll 8
             for (int q = 0; q < parts; ++q) {
-                const float4 v = *reinterpret_cast<const float4 *>(src + (size_t)q * K * row);
-                s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
+                qmlb::load_f32<float, VEC>(src + (size_t)q * K * row, v);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) s[e] += v[e];
             }
             T *to = dW + ((size_t)g * K + k) * N + c;
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (c + q < (unsigned)N) to[q] = qmlb::from_f32<T>(s[q]);
+            for (int e = 0; e < VEC; ++e)
+                if (c + e < (unsigned)N) to[e] = qmlb::from_f32<T>(s[e]);
         }
     }
 }
 
 template <typename T>
 int join(T *dW, const int *start, size_t n, int G, int K, int N, int split, size_t row, const float *partial, cudaStream_t st) {
-    const size_t per = ((size_t)K * ((N + 3) / 4) + 255) / 256, most = (size_t)(148 * 8 + G - 1) / G;   // most groups need nothing when there are many
-    join_kernel<T><<<dim3((unsigned)(per < most ? per : most), (unsigned)G), 256, (size_t)3 * (G + 1) * 4, st>>>(start, partial, (int)n, G, K, N,
-                                                                                                                split, row, dW);
+    const bool small = (size_t)K * N < (size_t)148 * 2048 * 4;
+    const size_t per = ((size_t)K * (small ? N : (N + 3) / 4) + 255) / 256, most = (size_t)(148 * 8 + G - 1) / G;   // most groups need nothing when there are many
+    const dim3 grid((unsigned)(per < most ? per : most), (unsigned)G);
+    const size_t smem = (size_t)3 * (G + 1) * 4;
+    if (small) join_kernel<T, 1><<<grid, 256, smem, st>>>(start, partial, (int)n, G, K, N, split, row, dW);
+    else join_kernel<T, 4><<<grid, 256, smem, st>>>(start, partial, (int)n, G, K, N, split, row, dW);
     return qmlb::check_launch("qmlb_grouped_matmul_wgrad");
 }
 

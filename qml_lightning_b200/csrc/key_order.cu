@@ -465,14 +465,14 @@ int run(const void *keys, size_t n, int nkeys, int *order, int *group_start, uns
 }  // namespace
 
 extern "C" size_t qmlb_group_by_key_scratch_bytes(size_t n, int nkeys) {
-    if (n == 0 || n >= (size_t)1 << 31 || nkeys <= 0 || nkeys == INT32_MAX) return 256;
-    if (n <= CLUSTER_KEYS) return 4 * ((n * 4 + 255) & ~(size_t)255) + 256;
-    return make_plan(n, nkeys).bytes + 256;
+    if (n == 0 || n >= (size_t)1 << 31 || nkeys <= 0 || nkeys == INT32_MAX) return 0;
+    if (n <= CLUSTER_KEYS) return bits_for((unsigned)nkeys) <= C_BITS ? 0 : 4 * ((n * 4 + 255) & ~(size_t)255);
+    return make_plan(n, nkeys).bytes;
 }
 
 extern "C" int qmlb_group_by_key(const void *keys, int key_bits, size_t n, int nkeys, int *order, int *group_start, void *scratch,
                                  size_t scratch_bytes, qmlb_stream_t stream) {
-    QMLB_REQUIRE(group_start && ((keys && order && scratch) || n == 0), "qmlb_group_by_key: null tensor");
+    QMLB_REQUIRE(group_start && ((keys && order) || n == 0), "qmlb_group_by_key: null tensor");
     QMLB_REQUIRE(key_bits == 32 || key_bits == 64, "qmlb_group_by_key: keys must have 32 or 64 bits");
     QMLB_REQUIRE(n < (size_t)1 << 31, "qmlb_group_by_key: fewer than 2^31 keys supported");
     QMLB_REQUIRE(nkeys > 0 && nkeys < INT32_MAX, "qmlb_group_by_key: bad number of keys");
@@ -481,8 +481,9 @@ extern "C" int qmlb_group_by_key(const void *keys, int key_bits, size_t n, int n
         empty_kernel<<<((unsigned)nkeys + THREADS) / THREADS < 1184 ? ((unsigned)nkeys + THREADS) / THREADS : 1184, THREADS, 0, st>>>((uint32_t)nkeys, group_start);
         return qmlb::check_launch("qmlb_group_by_key");
     }
-    QMLB_REQUIRE(scratch_bytes >= qmlb_group_by_key_scratch_bytes(n, nkeys) - 256, "qmlb_group_by_key: scratch too small");
-    QMLB_REQUIRE(((uintptr_t)scratch & 3) == 0, "qmlb_group_by_key: scratch must be 4-byte aligned");
+    const size_t need = qmlb_group_by_key_scratch_bytes(n, nkeys);
+    QMLB_REQUIRE(need == 0 || (scratch && scratch_bytes >= need), "qmlb_group_by_key: scratch too small");
+    QMLB_REQUIRE(need == 0 || ((uintptr_t)scratch & 3) == 0, "qmlb_group_by_key: scratch must be 4-byte aligned");
     unsigned char *sc = static_cast<unsigned char *>(scratch);
     return key_bits == 32 ? run<int32_t>(keys, n, nkeys, order, group_start, sc, st) : run<int64_t>(keys, n, nkeys, order, group_start, sc, st);
 }

@@ -14,6 +14,7 @@
 // This file contains no device code: it only allocates tensors, picks the current stream and device, and forwards
 // raw pointers to libqmlb200.so.  Unlike upstream it honours the current CUDA stream and device of the inputs.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/all.h>
 #include <torch/script.h>
@@ -434,7 +435,12 @@ void on_device(const Tensor &t, const torch::Device &dev, const char *name) {
 bool differentiable(const Tensor &a) { return at::GradMode::is_enabled() && a.requires_grad(); }
 bool differentiable(const Tensor &a, const Tensor &b) { return at::GradMode::is_enabled() && (a.requires_grad() || b.requires_grad()); }
 
-Tensor bytes_on(const Tensor &like, size_t bytes) { return torch::empty({(int64_t)bytes}, like.options().dtype(torch::kUInt8).requires_grad(false)); }
+// Uninitialised tensor on the device of `like`, without a pass through the dispatcher: the smallest calls of these operators are
+// bound by the host.
+Tensor new_tensor(at::IntArrayRef sizes, const Tensor &like, at::ScalarType type) {
+    return Tensor(at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt));
+}
+Tensor bytes_on(const Tensor &like, size_t bytes) { return new_tensor({(int64_t)bytes}, like, torch::kUInt8); }
 
 std::tuple<Tensor, Tensor> group_by_key(const Tensor &keys, int64_t nkeys) {
     TORCH_CHECK(keys.is_cuda(), "keys must be a CUDA tensor");
@@ -444,10 +450,9 @@ std::tuple<Tensor, Tensor> group_by_key(const Tensor &keys, int64_t nkeys) {
     c10::cuda::CUDAGuard guard(keys.device());
     Tensor k = keys.contiguous();
     const size_t n = (size_t)k.numel();
-    Tensor order = torch::empty({(int64_t)n}, k.options().dtype(torch::kInt32));
-    Tensor start = torch::empty({nkeys + 1}, k.options().dtype(torch::kInt32));
+    Tensor order = new_tensor({(int64_t)n}, k, torch::kInt32), start = new_tensor({nkeys + 1}, k, torch::kInt32);
     const size_t bytes = qmlb_group_by_key_scratch_bytes(n, (int)nkeys);
-    Tensor scratch = bytes_on(k, bytes);
+    Tensor scratch = bytes > 0 ? bytes_on(k, bytes) : order;
     check(qmlb_group_by_key(k.data_ptr(), bits, n, (int)nkeys, order.data_ptr<int>(), start.data_ptr<int>(), scratch.data_ptr(), bytes,
                             current_stream()),
           "group_by_key");
@@ -467,9 +472,9 @@ Tensor embedding_call(const Tensor &indices, const Tensor &table, double scale) 
     TORCH_CHECK(table.size(1) < INT32_MAX, "embedding: table too wide");
     c10::cuda::CUDAGuard guard(table.device());
     Tensor idx = indices.contiguous(), t = table.contiguous();
-    std::vector<int64_t> shape = indices.sizes().vec();
+    at::DimVector shape(indices.sizes());
     shape.push_back(table.size(1));
-    Tensor out = torch::empty(shape, t.options().requires_grad(false));
+    Tensor out = new_tensor(shape, t, t.scalar_type());
     if (out.numel() == 0) return out;
     check(qmlb_embedding(idx.data_ptr(), bits, t.data_ptr(), dt, (size_t)idx.numel(), t.size(0), (int)t.size(1), (float)scale, out.data_ptr(),
                          current_stream()),
@@ -492,7 +497,7 @@ Tensor embedding_grad_call(const Tensor &grad, const Tensor &indices, const Tens
     TORCH_CHECK(width < INT32_MAX, "embedding_grad: table too wide");
     c10::cuda::CUDAGuard guard(grad.device());
     Tensor g = grad.contiguous(), idx = indices.contiguous(), ord = order.contiguous(), st = group_start.contiguous();
-    Tensor out = torch::empty({rows, width}, g.options().requires_grad(false));
+    Tensor out = new_tensor({rows, width}, g, g.scalar_type());
     if (out.numel() == 0) return out;
     const size_t bytes = qmlb_embedding_grad_scratch_bytes((size_t)n, (int)rows, (int)width);
     Tensor scratch = bytes_on(g, bytes);
@@ -569,11 +574,11 @@ Tensor grouped_matmul_call(const Tensor &x, const Tensor &W, const Tensor &group
     TORCH_CHECK(G < INT32_MAX && K < INT32_MAX && N < INT32_MAX, "grouped_matmul: W too large");
     c10::cuda::CUDAGuard guard(W.device());
     Tensor xc = x.contiguous(), Wc = W.contiguous(), st = bounds(group_start, W, G);
-    Tensor out = torch::empty({n, transpose ? K : N}, Wc.options().requires_grad(false));
+    Tensor out = new_tensor({n, transpose ? K : N}, Wc, Wc.scalar_type());
     if (out.numel() == 0) return out;
     if (x.size(1) == 0) return out.zero_();
     const size_t bytes = qmlb_grouped_matmul_workspace_bytes((size_t)n, (int)G, (int)K, (int)N, dt, transpose);
-    Tensor ws = bytes_on(xc, bytes);
+    Tensor ws = bytes > 0 ? bytes_on(xc, bytes) : out;
     check(qmlb_grouped_matmul(xc.data_ptr(), Wc.data_ptr(), st.data_ptr<int>(), dt, (size_t)n, (int)G, (int)K, (int)N, transpose, out.data_ptr(),
                               ws.data_ptr(), bytes, current_stream()),
           "grouped_matmul");
@@ -590,10 +595,10 @@ Tensor grouped_matmul_wgrad_call(const Tensor &x, const Tensor &dy, const Tensor
     Tensor xc = x.contiguous(), dyc = dy.contiguous(), st = bounds(group_start, x, -1);
     const int64_t G = st.numel() - 1, K = x.size(1), N = dy.size(1);
     TORCH_CHECK(G < INT32_MAX && K < INT32_MAX && N < INT32_MAX, "grouped_matmul_wgrad: sizes too large");
-    Tensor out = torch::empty({G, K, N}, xc.options().requires_grad(false));
+    Tensor out = new_tensor({G, K, N}, xc, xc.scalar_type());
     if (out.numel() == 0) return out;
     const size_t bytes = qmlb_grouped_matmul_wgrad_workspace_bytes((size_t)x.size(0), (int)G, (int)K, (int)N, dt);
-    Tensor ws = bytes_on(xc, bytes);
+    Tensor ws = bytes > 0 ? bytes_on(xc, bytes) : out;
     check(qmlb_grouped_matmul_wgrad(xc.data_ptr(), dyc.data_ptr(), st.data_ptr<int>(), dt, (size_t)x.size(0), (int)G, (int)K, (int)N, out.data_ptr(),
                                     ws.data_ptr(), bytes, current_stream()),
           "grouped_matmul_wgrad");

@@ -26,7 +26,8 @@ def test_c_entries_refuse_bad_arguments():
     refused(L.qmlb_group_by_key(DUMMY, 16, 5, 3, DUMMY, DUMMY, DUMMY, 1 << 20, None), b'32 or 64')
     refused(L.qmlb_group_by_key(DUMMY, 32, 1 << 31, 3, DUMMY, DUMMY, DUMMY, 1 << 20, None), b'2^31')
     refused(L.qmlb_group_by_key(DUMMY, 32, 5, 0, DUMMY, DUMMY, DUMMY, 1 << 20, None), b'number of keys')
-    refused(L.qmlb_group_by_key(DUMMY, 32, 100000, 3, DUMMY, DUMMY, DUMMY, 16, None), b'scratch')
+    refused(L.qmlb_group_by_key(DUMMY, 32, 200000, 3, DUMMY, DUMMY, DUMMY, 16, None), b'scratch')
+    refused(L.qmlb_group_by_key(DUMMY, 32, 1000, 3000, DUMMY, DUMMY, None, 0, None), b'scratch')
     refused(L.qmlb_embedding(None, 32, DUMMY, 0, 5, 3, 4, 1.0, DUMMY, None), b'null')
     refused(L.qmlb_embedding(DUMMY, 32, None, 0, 5, 3, 4, 1.0, DUMMY, None), b'null')
     refused(L.qmlb_embedding(DUMMY, 8, DUMMY, 0, 5, 3, 4, 1.0, DUMMY, None), b'32 or 64')
@@ -50,7 +51,8 @@ def test_c_entries_refuse_bad_arguments():
 
 def test_scratch_sizes_grow_with_the_work():
     L = lib()
-    assert L.qmlb_group_by_key_scratch_bytes(0, 5) >= 1
+    assert L.qmlb_group_by_key_scratch_bytes(0, 5) == 0 and L.qmlb_group_by_key_scratch_bytes(1000, 5) == 0      # one launch, no scratch
+    assert L.qmlb_grouped_matmul_workspace_bytes(21, 3, 336, 256, 0, 0) == 0 and L.qmlb_grouped_matmul_workspace_bytes(210000, 3, 336, 256, 0, 0) > 0
     assert L.qmlb_group_by_key_scratch_bytes(1 << 20, 5) < 8 << 20                 # one pass: counters only
     assert L.qmlb_group_by_key_scratch_bytes(1 << 20, 50000) >= 3 * 4 << 20        # two passes: pairs and sorted keys
     assert L.qmlb_embedding_grad_scratch_bytes(1 << 20, 100, 256) >= 2 * 256 * 4
