@@ -3,7 +3,7 @@
 // the key nkeys: they come behind all groups, in their original order.
 //
 // Least-significant-digit radix sort with digits of at most RADIX_BITS bits, so up to 1,023 keys (every element or
-// species numbering) take ONE pass and 1,048,575 take two.  A pass over blocks of 1,024 or 4,096 keys:
+// species numbering) take ONE pass and 1,048,575 take two.  A pass over blocks of 1,024 or 2,048 keys:
 //   1. histogram : counts[digit][block]
 //   2. scan      : one block per digit turns its row into an exclusive prefix over the blocks and writes the digit's total
 //   3. scatter   : every block ranks its keys again (the same order, so the result never depends on scheduling) and
@@ -23,8 +23,8 @@ namespace {
 
 constexpr int RADIX_BITS = 10;                 // widest digit
 constexpr int THREADS = 256, WARPS = THREADS / 32;
-// keys per thread: few while the blocks do not fill the device
-constexpr int FEW = 4, MANY = 16;
+// keys per thread: few while the blocks do not fill the device (3.3 million keys of 5: 32 us with 8, 36 with 16, 42 with 32)
+constexpr int FEW = 4, MANY = 8;
 inline int items_for(size_t n) { return n < (size_t)148 * 8 * THREADS * FEW ? FEW : MANY; }
 
 __host__ __device__ inline int bits_for(unsigned nkeys) {   // digits of the values 0 .. nkeys (nkeys = "outside")
@@ -120,12 +120,13 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t *warp_sums
     return __shfl_sync(QMLB_FULL_MASK, upto - own, warp) + inc - v;
 }
 
-__global__ void __launch_bounds__(THREADS)
+constexpr int SCAN_THREADS = 1024;
+__global__ void __launch_bounds__(SCAN_THREADS)
 scan_kernel(uint32_t *__restrict__ counts, uint32_t nblocks, uint32_t *__restrict__ totals) {
-    __shared__ uint32_t warp_sums[WARPS];
+    __shared__ uint32_t warp_sums[SCAN_THREADS / 32];
     uint32_t *row = counts + (size_t)blockIdx.x * nblocks;
     uint32_t carry = 0;
-    for (uint32_t b = 0; b < nblocks; b += THREADS) {
+    for (uint32_t b = 0; b < nblocks; b += SCAN_THREADS) {
         const uint32_t at = b + threadIdx.x;
         const uint32_t v = at < nblocks ? row[at] : 0;
         uint32_t sum;
@@ -443,7 +444,7 @@ int run_sort(const K *keys, size_t n, int nkeys, int *order, int *group_start, u
         auto scatter = first ? (last ? scatter_kernel<K, true, true, ITEMS> : scatter_kernel<K, true, false, ITEMS>)
                              : (last ? scatter_kernel<K, false, true, ITEMS> : scatter_kernel<K, false, false, ITEMS>);
         histogram<<<p.blocks, THREADS, hist_smem, st>>>(keys, ik, un, uk, shift, p.nbits, counts);
-        scan_kernel<<<1 << p.nbits, THREADS, 0, st>>>(counts, p.blocks, totals);
+        scan_kernel<<<1 << p.nbits, SCAN_THREADS, 0, st>>>(counts, p.blocks, totals);
         scatter<<<p.blocks, THREADS, scat_smem, st>>>(keys, ik, ip, un, uk, shift, p.nbits, counts, totals, ok, op, group_start);
         if (last && !first) {
             const uint32_t sb = (uk + THREADS) / THREADS;

@@ -46,7 +46,7 @@ def test_order_is_stable(n, nkeys):
 
 
 @pytest.mark.parametrize('n', [20000, 33000, 131072, 131073, 300000, 1234567])
-@pytest.mark.parametrize('nkeys', [5, 1000, 30011])
+@pytest.mark.parametrize('nkeys', [1, 2, 3, 5, 7, 8, 15, 16, 1000, 30011])
 def test_order_of_many_skewed_keys(n, nkeys):
     g = gen(n + nkeys)
     u = torch.rand(n, generator=g, device=DEV, dtype=torch.float64)
