@@ -34,9 +34,18 @@ int encode_tiles(CUtensorMap *map, const void *base, bool bf16, uint64_t cols, u
     }
     const cuuint64_t dims[3] = {cols, rows, planes}, strides[2] = {row_bytes, row_bytes * rows};
     const cuuint32_t box[3] = {64, box_rows, 1}, step[3] = {1, 1, 1};
-    const CUresult r = f(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, planes > 0 ? 3 : 2, const_cast<void *>(base),
-                         dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    auto encode = [&]() {
+        return f(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, planes > 0 ? 3 : 2, const_cast<void *>(base),
+                 dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = encode();
+    if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) {
+        // A thread whose first CUDA call this is (a backward pass runs in one): the encoder belongs to the driver, which does not bind
+        // the device's context by itself as the runtime's calls do.
+        int dev = 0;
+        if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+    }
     if (r != CUDA_SUCCESS) {
         set_error("%s: tensor map refused (code %d, %llu x %llu x %llu)", what, (int)r, (unsigned long long)cols, (unsigned long long)rows,
                   (unsigned long long)planes);

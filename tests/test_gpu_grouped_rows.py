@@ -470,6 +470,40 @@ def test_streams_run_apart():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize('dtype', R.TYPES)
+def test_first_call_of_a_thread(dtype):
+    """A backward pass runs in a thread of its own, whose first call to the device may be one of these."""
+    import threading
+    g = gen(30)
+    x, W, dy = randn(g, 3000, 64, dtype=dtype), randn(g, 2, 64, 48, dtype=dtype), randn(g, 3000, 48, dtype=dtype)
+    start = R.start_of([1000, 1900], DEV)
+    keys = torch.randint(0, 9, (3000,), generator=g, device=DEV)
+
+    def calls():
+        order, first = ops().group_by_key(keys, 9)
+        return [ops().grouped_matmul(x, W, start, False), ops().grouped_matmul(dy, W, start, True), ops().grouped_matmul_wgrad(x, dy, start), order,
+                ops().embedding(keys, x, 1.0), ops().embedding_grad(x, keys, order, first, 9, 1.0)]
+
+    want = calls()                                                    # the allocator has every block by now
+    for k in range(len(want)):
+        got, errors = [], []
+
+        def work(k=k):
+            try:
+                first = [lambda: ops().grouped_matmul(x, W, start, False), lambda: ops().grouped_matmul(dy, W, start, True),
+                         lambda: ops().grouped_matmul_wgrad(x, dy, start), lambda: ops().group_by_key(keys, 9)[0],
+                         lambda: ops().embedding(keys, x, 1.0), lambda: ops().embedding_grad(x, keys, want[3], ops().group_by_key(keys, 9)[1], 9, 1.0)][k]
+                got.append(first())
+                torch.cuda.synchronize()
+            except Exception as e:  # noqa: BLE001
+                errors.append(e)
+        t = threading.Thread(target=work)
+        t.start()
+        t.join()
+        assert not errors, errors
+        assert torch.equal(got[0], want[k])
+
+
 def test_captured_step_replays_on_new_inputs():
     """A whole step with its gradients in a CUDA graph; two graphs share nothing; no operator waits for the device."""
     g = gen(24)
