@@ -250,6 +250,31 @@ def test_products_of_large_groups(K, N, sizes, dtype):
 
 
 @pytest.mark.parametrize('dtype', R.TYPES)
+@pytest.mark.parametrize('K,N', [(20, 12), (336, 256), (1100, 520)])
+@pytest.mark.parametrize('sizes', [[0, 13, 0], [0, 200, 0], [0, 0, 2500, 0], [700, 0, 701, 0], [0, 9000, 0, 1], [0, 0]])
+def test_every_result_is_written(sizes, K, N, dtype):
+    """Whatever stood in the outputs and in the scratch, groups without rows have zero gradients, rows without a group zero rows."""
+    from qml_lightning_b200 import cabi
+    g = gen(K + len(sizes))
+    used, front = sum(sizes), 2
+    n = used + 5
+    start = R.start_of(sizes, DEV, front)
+    x, dy, W = randn(g, n, K, dtype=dtype), randn(g, n, N, dtype=dtype), (randn(g, len(sizes), K, N) / K ** 0.5).to(dtype)
+    nan = lambda *shape: torch.full(shape, float('nan'), dtype=dtype, device=DEV)
+    scratch = torch.full((1 << 24,), float('nan'), device=DEV)        # freed: what the calls below allocate comes from it
+    del scratch
+    dW = cabi.grouped_matmul_wgrad(x, dy, start, out=nan(len(sizes), K, N))
+    y = cabi.grouped_matmul(x, W, start, out=nan(n, N))
+    dx = cabi.grouped_matmul(dy, W, start, transpose=True, out=nan(n, K))
+    for i, rows in enumerate(sizes):
+        assert rows or (dW[i] == 0).all()
+    for t in (y, dx):
+        assert (t[:front] == 0).all() and (t[front + used:] == 0).all()
+    for got, (exact, mag, *terms), m in ((y, R.product(x, W, start), K), (dx, R.product(dy, W, start, True), N), (dW, R.wgrad(x, dy, start), 0)):
+        R.assert_within(got, exact, R.sum_bound(exact, mag, terms[0] if terms else m, dtype), f'{sizes} {K} {N}')
+
+
+@pytest.mark.parametrize('dtype', R.TYPES)
 def test_products_of_misaligned_tensors(dtype):
     g = gen(5)
     sizes, K, N = [70, 0, 200], 64, 128
