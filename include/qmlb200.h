@@ -405,7 +405,8 @@ int qmlb_embedding_grad(const void *dout, int dtype, const void *index, int inde
                         qmlb_stream_t stream);
 
 /* One matrix per group of rows.  W [ngroups, K, N]; the rows of group g are group_start[g] <= r < group_start[g+1]
- * (i32[ngroups+1], ascending; groups may be empty and of any size).
+ * (i32[ngroups+1], ascending; groups may be empty and of any size).  Bounds outside [0, n] are clamped; bounds that descend
+ * give rows of no meaning, but no access outside the tensors.  No output may overlap an input.
  *   transpose = 0: out [n, N], out[r] = x[r] . W[g]       x [n, K]
  *   transpose = 1: out [n, K], out[r] = x[r] . W[g]^T     x [n, N]   (gradient of the rows)
  * Rows in front of the first group or behind the last become zero rows.  32-bit sums, one rounding to `dtype`.

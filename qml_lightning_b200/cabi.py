@@ -639,11 +639,19 @@ def _together(first, **others):
             raise RuntimeError(f"{name} must be on {first.device}, got {t.device}")
 
 
-def _output(out, shape, dtype, device, name='out'):
+def _sizes(*sizes):
+    if max(sizes) >= 2 ** 31:                             # ctypes would cut them off without a word
+        raise RuntimeError(f"sizes below 2^31 supported, got {sizes}")
+
+
+def _output(out, shape, dtype, device, *inputs):
     if out is None:
         return torch.empty(shape, dtype=dtype, device=device)
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != device:
-        raise RuntimeError(f"{name} must be {dtype} {tuple(shape)} on {device}, got {out.dtype} {tuple(out.shape)} on {out.device}")
+        raise RuntimeError(f"out must be {dtype} {tuple(shape)} on {device}, got {out.dtype} {tuple(out.shape)} on {out.device}")
+    first, end = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
+    if any(t.data_ptr() < end and first < t.data_ptr() + t.numel() * t.element_size() for t in inputs):
+        raise RuntimeError("out must not overlap an input")
     return out
 
 
@@ -672,7 +680,8 @@ def embedding(indices, table, scale=1.0, out=None):
         raise RuntimeError("table must be [rows, width]")
     pi, pt = _p(indices, None, 'indices'), _p(table, None, 'table')
     _together(table, indices=indices)
-    out = _output(out, tuple(indices.shape) + (table.shape[1],), table.dtype, table.device)
+    _sizes(table.shape[1])
+    out = _output(out, tuple(indices.shape) + (table.shape[1],), table.dtype, table.device, indices, table)
     if out.numel():
         check(_lib.load().qmlb_embedding(pi, bits, pt, dtype, indices.numel(), table.shape[0], table.shape[1], float(scale),
                                          _p(out, None, 'out'), _stream(table.device)), 'qmlb_embedding')
@@ -691,7 +700,8 @@ def embedding_grad(grad, indices, order, group_start, scale=1.0, out=None):
     pg, pi = _p(grad, None, 'grad'), _p(indices, None, 'indices')
     po, ps = _p(order, torch.int32, 'order'), _p(group_start, torch.int32, 'group_start')
     _together(grad, indices=indices, order=order, group_start=group_start)
-    out = _output(out, (rows, width), grad.dtype, grad.device)
+    _sizes(rows, width)
+    out = _output(out, (rows, width), grad.dtype, grad.device, grad, indices, order, group_start)
     if out.numel():
         lib = _lib.load()
         nbytes = lib.qmlb_embedding_grad_scratch_bytes(n, rows, width)
@@ -715,7 +725,8 @@ def grouped_matmul(x, W, group_start, transpose=False, out=None):
         raise RuntimeError("group_start must have one entry per group and one more")
     px, pw, ps = _p(x, W.dtype, 'x'), _p(W, None, 'W'), _p(group_start, torch.int32, 'group_start')
     _together(W, x=x, group_start=group_start)
-    out = _output(out, (n, K if transpose else N), W.dtype, W.device)
+    _sizes(G, K, N)
+    out = _output(out, (n, K if transpose else N), W.dtype, W.device, x, W, group_start)
     if out.numel() == 0:
         return out
     if x.shape[1] == 0:
@@ -738,7 +749,8 @@ def grouped_matmul_wgrad(x, dy, group_start, out=None):
         raise RuntimeError("group_start must have one entry per group and one more")
     px, pd, ps = _p(x, None, 'x'), _p(dy, x.dtype, 'dy'), _p(group_start, torch.int32, 'group_start')
     _together(x, dy=dy, group_start=group_start)
-    out = _output(out, (G, K, N), x.dtype, x.device)
+    _sizes(G, K, N)
+    out = _output(out, (G, K, N), x.dtype, x.device, x, dy, group_start)
     if out.numel() == 0:
         return out
     lib = _lib.load()

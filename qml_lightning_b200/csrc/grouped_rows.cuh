@@ -32,10 +32,19 @@ struct Groups {              // in shared memory
     }
 };
 
-// Fill `start` (all threads) and `parts` (warp 0): a group of r rows has ceil(r / part_rows) parts.  Ends with a barrier.
+// Fill `start` (all threads) and `parts` (warp 0): a group of r rows has ceil(r / part_rows) parts.  Bounds that descend, which
+// no caller should pass, are raised to the largest before them: the groups never hold more than n rows, for which tiles and
+// scratch were counted.  Ends with a barrier.
 __device__ __forceinline__ void read_groups(const Groups &s, const int *__restrict__ start, int G, int n, int part_rows) {
     for (int g = threadIdx.x; g <= G; g += blockDim.x) s.start[g] = min(max(start[g], 0), n);
     __syncthreads();
+    bool down = false;
+    for (int g = threadIdx.x; g < G; g += blockDim.x) down |= s.start[g + 1] < s.start[g];
+    if (__syncthreads_or(down)) {
+        if (threadIdx.x == 0)
+            for (int g = 0; g < G; ++g) s.start[g + 1] = max(s.start[g + 1], s.start[g]);
+        __syncthreads();
+    }
     if (threadIdx.x < 32) {
         const int lane = threadIdx.x;
         for (int pass = 0; pass < (s.split ? 2 : 1); ++pass) {

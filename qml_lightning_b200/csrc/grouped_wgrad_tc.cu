@@ -6,8 +6,8 @@
 // the depth; tcgen05.mma takes them that way and nothing is transposed.  A unit of work is one tile of 128 columns of x by
 // NT columns of dy over at most `split` rows of one group.  Groups of one part are finished by their unit; the parts of the
 // others go to scratch in 32 bits and a second kernel adds them in order, so the result never depends on scheduling.
-// The split is chosen on the host from sizes alone (wgrad_split).  It is at most 16,384 rows, because the tensor core truncates when it adds: 1,024 additions are off by 3e-5 on average, far
-// below the half step of the result.
+// The split is chosen on the host from sizes alone (wgrad_split).  It is at most 16,384 rows, because the tensor core truncates
+// when it adds: 1,024 additions are off by 3e-5 on average, far below the half step of the result.
 // Roles as in the forward product.  The last slice of a part may hold rows of the next group: the issuing warp overwrites
 // the lines up to the next multiple of 16 rows with zeros and leaves the other multiples out.
 #include "grouped_rows.cuh"

@@ -345,6 +345,110 @@ def test_bounds_outside_the_rows_are_clamped():
             assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize('dtype', R.TYPES)
+@pytest.mark.parametrize('n,K,N', [(100, 24, 16), (5000, 136, 72), (40000, 64, 48)])
+def test_descending_bounds_stay_inside(n, K, N, dtype):
+    """Groups that overlap, if their bounds were taken as they are, hold many times n rows: tiles, scratch and results keep their
+    sizes, and what follows on the stream is right."""
+    from qml_lightning_b200 import _lib, cabi
+    g = gen(n)
+    groups = 64
+    x, dy, W = randn(g, n, K, dtype=dtype), randn(g, n, N, dtype=dtype), randn(g, groups, K, N, dtype=dtype)
+    start = torch.tensor([0, n] * (groups // 2) + [0], dtype=torch.int32, device=DEV)
+    code, lib, stream = cabi._DTYPES[dtype], _lib.load(), torch.cuda.current_stream().cuda_stream
+    guard = 1 << 20
+
+    def call(name, a, b, out_numel, *tail):
+        nbytes = getattr(lib, name + '_workspace_bytes')(n, groups, K, N, code, *tail)
+        ws = torch.full((nbytes + guard,), 85, dtype=torch.uint8, device=DEV)
+        out = torch.full((out_numel + guard,), 3.0, dtype=dtype, device=DEV)
+        assert getattr(lib, name)(a.data_ptr(), b.data_ptr(), start.data_ptr(), code, n, groups, K, N, *tail, out.data_ptr(), ws.data_ptr(),
+                                  nbytes, stream) == 0
+        assert (ws[nbytes:] == 85).all() and (out[out_numel:] == 3).all()
+
+    call('qmlb_grouped_matmul', x, W, n * N, 0)
+    call('qmlb_grouped_matmul', dy, W, n * K, 1)
+    call('qmlb_grouped_matmul_wgrad', x, dy, groups * K * N)
+    start = R.start_of([n // 3, 0, n // 2] + [0] * (groups - 3), DEV)
+    exact, mag, terms = R.wgrad(x, dy, start)
+    R.assert_within(ops().grouped_matmul_wgrad(x, dy, start), exact, R.sum_bound(exact, mag, terms, dtype), 'dW')
+    assert cabi.tc_timeouts() == 0
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('n,K,N', [(2200001, 1000, 24), (2200003, 24, 1000)])
+def test_products_beyond_32_bit_offsets(n, K, N, dtype):
+    """Rows and results of 2.2e9 elements: groups at both ends, compared with the products of their rows alone."""
+    g = gen(11)
+    x, dy = torch.zeros(n, K, dtype=dtype, device=DEV), torch.zeros(n, N, dtype=dtype, device=DEV)
+    W = (randn(g, 3, K, N) / K ** 0.5).to(dtype)
+    start = R.start_of([300, n - 300 - 700, 693], DEV)
+    parts = [(0, 300), (n - 700, n - 7)]
+    for a, b in parts:
+        x[a:b], dy[a:b] = randn(g, b - a, K, dtype=dtype), randn(g, b - a, N, dtype=dtype)
+    dW = ops().grouped_matmul_wgrad(x, dy, start)
+    assert (dW[1] == 0).all()
+    for (a, b), e in zip(parts, (0, 2)):
+        exact, mag, terms = R.wgrad(x[a:b], dy[a:b], R.start_of([b - a], DEV))
+        R.assert_within(dW[e:e + 1], exact, R.sum_bound(exact, mag, terms, dtype), f'dW {e}')
+    for transpose, rows, depth in ((False, x, K), (True, dy, N)):
+        out = ops().grouped_matmul(rows, W, start, transpose)
+        for (a, b), e in zip(parts, (0, 2)):
+            exact, mag = R.product(rows[a:b], W[e:e + 1], R.start_of([b - a], DEV), transpose)
+            R.assert_within(out[a:b], exact, R.sum_bound(exact, mag, depth, dtype), f'{transpose} {e}')
+        assert int(out[300:n - 700].count_nonzero()) == 0 and int(out[n - 7:].count_nonzero()) == 0
+        del out
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_matrices_beyond_32_bit_offsets(dtype):
+    """1,024 matrices of 2.2e9 elements together, rows for the first and the last."""
+    g = gen(12)
+    G, K, N = 1024, 1050, 2056
+    W = torch.zeros(G, K, N, dtype=dtype, device=DEV)
+    W[0], W[-1] = randn(g, K, N, dtype=dtype), randn(g, K, N, dtype=dtype)
+    for a, b in ((9, 11), (2000, 2500)):
+        x, dy = randn(g, a + b, K, dtype=dtype), randn(g, a + b, N, dtype=dtype)
+        start = R.start_of([a] + [0] * (G - 2) + [b], DEV)
+        small, ends = R.start_of([a, b], DEV), torch.stack([W[0], W[-1]])
+        for transpose, rows, depth in ((False, x, K), (True, dy, N)):
+            exact, mag = R.product(rows, ends, small, transpose)
+            R.assert_within(ops().grouped_matmul(rows, W, start, transpose), exact, R.sum_bound(exact, mag, depth, dtype), f'{a} {transpose}')
+        dW = ops().grouped_matmul_wgrad(x, dy, start)
+        exact, mag, terms = R.wgrad(x, dy, small)
+        R.assert_within(torch.stack([dW[0], dW[-1]]), exact, R.sum_bound(exact, mag, terms, dtype), f'dW {a}')
+        assert int(dW[1:-1].count_nonzero()) == 0
+        del dW
+
+
+def test_largest_number_of_keys():
+    nkeys = 2 ** 31 - 2
+    for n in (5, 150000):
+        keys = torch.randint(0, nkeys, (n,), generator=gen(n), device=DEV)
+        keys[0], keys[1], keys[3] = nkeys - 1, -1, nkeys
+        order, start = ops().group_by_key(keys, nkeys)
+        inside = (keys >= 0) & (keys < nkeys)
+        ref = torch.sort(torch.where(inside, keys, torch.full_like(keys, nkeys)), stable=True)[1].int()
+        assert torch.equal(order, ref)
+        used = int(inside.sum())
+        assert int(start[0]) == 0 and int(start[-1]) == used and int(start[-2]) == used - int((keys == nkeys - 1).sum())
+        at = keys[ref[:used].long()]
+        rank = torch.searchsorted(at, at)                                  # first position of the same key
+        assert torch.equal(start[at].long(), rank)
+        del start
+
+
+def test_outputs_do_not_overlap_inputs():
+    from qml_lightning_b200 import cabi
+    x, W, start = torch.zeros(6, 8, device=DEV), torch.zeros(1, 8, 8, device=DEV), R.start_of([6], DEV)
+    idx = torch.arange(6, device=DEV)
+    order, first = cabi.group_by_key(idx, 6)
+    for call in (lambda: cabi.grouped_matmul(x, W, start, out=x), lambda: cabi.grouped_matmul_wgrad(W[0], W[0], start, out=W),
+                 lambda: cabi.embedding(idx, x, out=x), lambda: cabi.embedding_grad(x, idx, order, first, out=x)):
+        with pytest.raises(RuntimeError, match='overlap'):
+            call()
+
+
 def test_empty_products():
     for dtype in R.TYPES:
         W = torch.ones(2, 3, 4, dtype=dtype, device=DEV)
