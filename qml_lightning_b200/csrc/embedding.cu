@@ -253,13 +253,15 @@ join_kernel(const int *__restrict__ tail_key, const float *__restrict__ pieces, 
     if (last < b + JOIN_LANES) {
         if (blockIdx.y) return;
         for (int c = (int)threadIdx.x * VEC; c < width; c += JOIN_THREADS * VEC) {
-            float s[VEC], v[VEC];
+            float s[VEC], v[4][VEC];
             load(b, c, s);
-#pragma unroll 4
-            for (unsigned j = b + 1; j <= last; ++j) {
-                load(j, c, v);
+            for (unsigned j = b + 1; j <= last; j += 4) {        // addresses are clamped instead of tested: the loads are in flight together
 #pragma unroll
-                for (int q = 0; q < VEC; ++q) s[q] += v[q];
+                for (unsigned u = 0; u < 4; ++u) load(min(j + u, last), c, v[u]);
+#pragma unroll
+                for (unsigned u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) s[q] += j + u <= last ? v[u][q] : 0.f;
             }
             store(c, s);
         }
@@ -268,15 +270,17 @@ join_kernel(const int *__restrict__ tail_key, const float *__restrict__ pieces, 
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     for (int c0 = blockIdx.y * 32 * VEC; c0 < width; c0 += gridDim.y * 32 * VEC) {
         const int c = c0 + lane * VEC;
-        float s[VEC], v[VEC];
+        float s[VEC], v[8][VEC];
 #pragma unroll
         for (int q = 0; q < VEC; ++q) s[q] = 0.f;
         if (c < width) {
-#pragma unroll 8
-            for (unsigned j = b + (unsigned)w; j <= last; j += JOIN_LANES) {
-                load(j, c, v);
+            for (unsigned j = b + (unsigned)w; j <= last; j += 8 * JOIN_LANES) {
 #pragma unroll
-                for (int q = 0; q < VEC; ++q) s[q] += v[q];
+                for (unsigned u = 0; u < 8; ++u) load(min(j + u * JOIN_LANES, last), c, v[u]);
+#pragma unroll
+                for (unsigned u = 0; u < 8; ++u)
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) s[q] += j + u * JOIN_LANES <= last ? v[u][q] : 0.f;
             }
         }
 #pragma unroll

@@ -273,14 +273,16 @@ join_kernel(const int *__restrict__ start, const float *__restrict__ partial, in
         for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < (size_t)K * per_row; i += (size_t)gridDim.x * 256) {
             const unsigned k = (unsigned)(i / per_row), c = (unsigned)(i - (size_t)k * per_row) * VEC;
             const float *src = partial + ((size_t)gr.split[g] * K + k) * row + c;
-            float s[VEC], v[VEC];
+            float s[VEC], v[8][VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) s[e] = 0.f;
-#pragma unroll 8
-            for (int q = 0; q < parts; ++q) {
-                qmlb::load_f32<float, VEC>(src + (size_t)q * K * row, v);
+            for (int q = 0; q < parts; q += 8) {                 // addresses are clamped instead of tested: eight loads in flight
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) s[e] += v[e];
+                for (int u = 0; u < 8; ++u) qmlb::load_f32<float, VEC>(src + (size_t)min(q + u, parts - 1) * K * row, v[u]);
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) s[e] += q + u < parts ? v[u][e] : 0.f;
             }
             T *to = dW + ((size_t)g * K + k) * N + c;
 #pragma unroll
