@@ -618,12 +618,16 @@ pack_kernel(const float *__restrict__ W, Shape p, int N, unsigned char *__restri
     const int cl = TRANS ? threadIdx.x >> 4 : threadIdx.x & 15, kl = TRANS ? threadIdx.x & 15 : threadIdx.x >> 4;
     const int col = blockIdx.x * 16 + cl;
     const float *Wg = W + (size_t)g * p.K * p.out;
-    const float *base = TRANS ? Wg + (size_t)col * N : Wg + col;
+    const int inside = min(col, p.out - 1);              // addresses are clamped instead of tested: the loads are in flight together
+    const float *base = TRANS ? Wg + (size_t)inside * N : Wg + inside;
     const size_t step = TRANS ? 1 : (size_t)N;
     float m = 0.f;
-    if (col < p.out) {
-#pragma unroll 8
-        for (int k = kl; k < p.K; k += 16) m = fmaxf(m, fabsf(base[(size_t)k * step]));
+    for (int k = kl; k < p.K; k += 16 * 16) {
+        float t[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) t[u] = base[(size_t)min(k + u * 16, p.K - 1) * step];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) m = fmaxf(m, fabsf(t[u]));
     }
     most[cl][kl] = m;
     __syncthreads();
@@ -633,14 +637,18 @@ pack_kernel(const float *__restrict__ W, Shape p, int N, unsigned char *__restri
     scales(m, 268, s, inv);
     const int tile = col / p.NT, in = col - tile * p.NT;               // the grid covers whole tiles
     const size_t image = (size_t)(g * p.ntiles + tile) * p.nchunks;
+#pragma unroll 2
     for (int c0 = 0; c0 < p.nchunks; c0 += 2) {                        // two stretches: 16 threads of 8 values per column
         const int c = c0 + (kl >> 3), k0 = c0 * BK + kl * 8;
         if (c >= p.nchunks) continue;
+        float t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = base[(size_t)min(k0 + i, p.K - 1) * step];
         float2 v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            v[i].x = (col < p.out && k0 + i * 2 < p.K) ? base[(size_t)(k0 + i * 2) * step] : 0.f;
-            v[i].y = (col < p.out && k0 + i * 2 + 1 < p.K) ? base[(size_t)(k0 + i * 2 + 1) * step] : 0.f;
+            v[i].x = col < p.out && k0 + i * 2 < p.K ? t[i * 2] : 0.f;
+            v[i].y = col < p.out && k0 + i * 2 + 1 < p.K ? t[i * 2 + 1] : 0.f;
         }
         uint32_t hi[4], lo[4];
 #pragma unroll
