@@ -14,8 +14,8 @@
 // every PERIOD-th row (2, 4 or 8) has the same offset from a 16-byte boundary, so a tile takes 128 rows of one offset, by a tensor
 // map that starts at the boundary; its sums begin `shift` elements early, against zero rows of the matrix (coordinates in front of
 // its first row), and the issuing warp overwrites what the rows bring there.  (780 deep, 330,001 rows: 231 us with cp.async of
-// 8 bytes, 177 us so; 781 deep: 664 us with 2-byte loads, 181 us so.)  Transposed, the matrix's lines would have to move along, so warps 12-19 bring the rows with cp.async of 8 or
-// 4 bytes, or 2-byte loads, into the same swizzled stages.
+// 8 bytes, 177 us so; 781 deep: 664 us with 2-byte loads, 181 us so.)  Transposed, the matrix's lines would have to move along, so
+// warps 12-19 bring the rows with cp.async of 8 or 4 bytes, or 2-byte loads, into the same swizzled stages.
 // Every wait is bounded; a block that gives up fills its remaining tiles with NaN and counts the event (qmlb_tc_timeouts).
 #include "grouped_tc.cuh"
 #include "grouped_rows.cuh"
@@ -355,7 +355,8 @@ int run(const void *x, const void *W, const int *start, size_t n, int G, int K, 
     // Columns per tile: as many as one accumulator holds, so that the rows are read once, in equal parts; fewer when the row
     // tiles alone do not give every SM a tile.
     const long mtiles = (long)((n + BM - 1) / BM);
-    const bool aligned = p.in_access == 16, shifted = !aligned && !transpose, loaded = !aligned && transpose, pair = aligned && p.K >= PAIR_DEPTH && n / G >= PAIR_ROWS && mtiles * ((p.out + 255) / 256) >= 2 * 148;
+    const bool aligned = p.in_access == 16, shifted = !aligned && !transpose, loaded = !aligned && transpose;
+    const bool pair = aligned && p.K >= PAIR_DEPTH && n / G >= PAIR_ROWS && mtiles * ((p.out + 255) / 256) >= 2 * 148;
     const int blocks_per_tile = pair ? 2 : 1;
     long nt = (p.out + 255) / 256;
     const long wanted = (148 + mtiles - 1) / mtiles, most = (p.out + 63) / 64;
