@@ -12,7 +12,7 @@
 // Work split.  One persistent block per SM takes tiles of 128 x NT results:
 //   warp 0          bulk copies of the matrix operand's images (products of rows; a packing kernel makes the images)
 //   warp 1          issues tcgen05.mma, several tensor-memory accumulators in turn
-//   warps 2-3       zero rows outside the groups
+//   warps 2-3       zero rows outside the groups, zero matrices of groups without rows
 //   loading warps   load float32 rows, find the scales, split, and write the swizzled operand images to shared memory
 //   folding warps   (eight) add the finished accumulators to their registers, and store the tile
 // Products of rows: NT <= 256, 4 loading warps, 128 sums per folding thread.  Gradient of the matrices: both operands are loaded
@@ -230,7 +230,9 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
             if (lane == 0) mma_commit(bar(done));
             __syncwarp();
             for (int tries = 0; tries < WAIT_LIMIT && !mbar_try(bar(done), 0u); ++tries) {}
-        } else if (!GRAD) {
+        } else if (GRAD) {
+            zero_empty_groups(gr, p.G, reinterpret_cast<unsigned char *>(out), (size_t)p.K * p.out * 4, p.out_access, blockIdx.x * 2 + warp - 2, gridDim.x * 2, lane);
+        } else {
             const int first = gr.start[0], last = max(gr.start[p.G], first), outside = first + (p.n - last);
             for (int i = blockIdx.x * 2 + (warp - 2); i < outside; i += gridDim.x * 2) {
                 float *row = out + (size_t)(i < first ? i : last + (i - first)) * p.out;

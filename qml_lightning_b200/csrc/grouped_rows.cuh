@@ -89,6 +89,21 @@ __device__ __forceinline__ void store_if(void *p, uint16_t v, bool wanted) {
                  : "memory");
 }
 
+// Zeros into the matrices [K][row_bytes] of the groups without rows, by warp `i` of `count`; a row is a multiple of `access` bytes.
+__device__ __forceinline__ void zero_empty_groups(const Groups &s, int G, unsigned char *out, size_t matrix_bytes, int access, int i, int count, int lane) {
+    const size_t first = (size_t)i * 32 + lane, step = (size_t)count * 32;
+    for (int g = 0; g < G; ++g) {
+        if (s.parts[g + 1] != s.parts[g]) continue;
+        unsigned char *to = out + (size_t)g * matrix_bytes;
+        if (access == 16)
+            for (size_t k = first; k < matrix_bytes / 16; k += step) reinterpret_cast<uint4 *>(to)[k] = make_uint4(0, 0, 0, 0);
+        else if (access >= 4)
+            for (size_t k = first; k < matrix_bytes / 4; k += step) reinterpret_cast<uint32_t *>(to)[k] = 0;
+        else
+            for (size_t k = first; k < matrix_bytes / 2; k += step) reinterpret_cast<uint16_t *>(to)[k] = 0;
+    }
+}
+
 // Byte `c` of row `r` in a warp's epilogue tile: 16-byte pieces in an order that changes every two rows, so that neither the
 // writes by rows nor the reads along rows collide in the banks.
 __device__ __forceinline__ int tile_at(int r, int c) { return r * 64 + (((c >> 4) ^ ((r >> 1) & 3)) << 4) + (c & 15); }

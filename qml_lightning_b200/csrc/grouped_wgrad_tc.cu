@@ -5,7 +5,8 @@
 // The rows are the depth of the product, so both operands lie in memory with their lines (64 columns of one row) across
 // the depth; tcgen05.mma takes them that way and nothing is transposed.  A unit of work is one tile of 128 columns of x by
 // NT columns of dy over at most `split` rows of one group.  Groups of one part are finished by their unit; the parts of the
-// others go to scratch in 32 bits and a second kernel adds them in order, so the result never depends on scheduling.
+// others go to scratch in 32 bits and a second kernel adds them in order, so the result never depends on scheduling.  Groups
+// without rows are filled with zeros by warps 2-3.
 // The split is chosen on the host from sizes alone (wgrad_split).  It is at most 16,384 rows, because the tensor core truncates
 // when it adds: 1,024 additions are off by 3e-5 on average, far below the half step of the result.
 // Roles as in the forward product.  The last slice of a part may hold rows of the next group: the issuing warp overwrites
@@ -153,7 +154,9 @@ wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
         if (lane == 0) mma_commit(bar(done));
         __syncwarp();
         for (int tries = 0; tries < WAIT_LIMIT && !mbar_try(bar(done), 0u); ++tries) {}
-    } else if (warp >= EPI_WARP && warp < LOAD_WARP) {
+    } else if (warp < EPI_WARP) {
+        zero_empty_groups(gr, p.G, reinterpret_cast<unsigned char *>(dW), (size_t)p.K * p.N * 2, p.out_access, blockIdx.x * 2 + warp - 2, gridDim.x * 2, lane);
+    } else if (warp < LOAD_WARP) {
         // warps w and w + 4 share a quarter of the rows and take every other 32 columns
         const int quarter = warp & 3, c_first = ((warp - EPI_WARP) >> 2) * 32;
         unsigned char *mine = epi + (warp - EPI_WARP) * EPI_TILE;
@@ -216,7 +219,7 @@ wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
                 }
             }
         }
-    } else if (LOADED && warp >= LOAD_WARP) {
+    } else if (LOADED) {
         const int t = tid - LOAD_WARP * 32;
         const unsigned char *xs = reinterpret_cast<const unsigned char *>(x), *ds = reinterpret_cast<const unsigned char *>(dy);
         int it = 0;
@@ -255,51 +258,64 @@ wgrad_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
     if (warp == MMA_WARP) tmem_free(tmem, TMEM_COLS);
 }
 
-// Groups of several parts: their sum, in order.  Groups without rows: zeros.  blockIdx.y walks the groups; `row` is the
+// Groups of several parts: their sum, in order.  blockIdx.y takes the y-th of them (there are at most n / split); `row` is the
 // row length of the parts.  VEC columns per thread: four, or one where that leaves too few threads to hide the latency.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
 join_kernel(const int *__restrict__ start, const float *__restrict__ partial, int n, int G, int K, int N, int split, size_t row, T *__restrict__ dW) {
     extern __shared__ int sm[];
+    __shared__ int which;
     Groups gr;
     gr.start = sm;
     gr.parts = sm + G + 1;
     gr.split = gr.parts + G + 1;
     read_groups(gr, start, G, n, split);
-    const unsigned per_row = ((unsigned)N + VEC - 1u) / VEC;
-    for (int g = blockIdx.y; g < G; g += gridDim.y) {
-        const int parts = gr.parts[g + 1] - gr.parts[g];
-        if (parts == 1) continue;
-        for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < (size_t)K * per_row; i += (size_t)gridDim.x * 256) {
-            const unsigned k = (unsigned)(i / per_row), c = (unsigned)(i - (size_t)k * per_row) * VEC;
-            const float *src = partial + ((size_t)gr.split[g] * K + k) * row + c;
-            float s[VEC], v[8][VEC];
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) s[e] = 0.f;
-            for (int q = 0; q < parts; q += 8) {                 // addresses are clamped instead of tested: eight loads in flight
-#pragma unroll
-                for (int u = 0; u < 8; ++u) qmlb::load_f32<float, VEC>(src + (size_t)min(q + u, parts - 1) * K * row, v[u]);
-#pragma unroll
-                for (int u = 0; u < 8; ++u)
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) s[e] += q + u < parts ? v[u][e] : 0.f;
-            }
-            T *to = dW + ((size_t)g * K + k) * N + c;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e)
-                if (c + e < (unsigned)N) to[e] = qmlb::from_f32<T>(s[e]);
+    if (threadIdx.x < 32) {
+        int left = (int)blockIdx.y, found = -1;
+        for (int g0 = 0; g0 < G && found < 0; g0 += 32) {
+            const int g = g0 + (int)threadIdx.x;
+            const unsigned m = __ballot_sync(QMLB_FULL_MASK, g < G && gr.parts[g + 1] - gr.parts[g] > 1);
+            if (left < __popc(m)) found = g0 + (int)__fns(m, 0, left + 1);
+            left -= __popc(m);
         }
+        if (threadIdx.x == 0) which = found;
+    }
+    __syncthreads();
+    const int g = which;
+    if (g < 0) return;
+    const int parts = gr.parts[g + 1] - gr.parts[g];
+    const unsigned per_row = ((unsigned)N + VEC - 1u) / VEC;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < (size_t)K * per_row; i += (size_t)gridDim.x * 256) {
+        const unsigned k = (unsigned)(i / per_row), c = (unsigned)(i - (size_t)k * per_row) * VEC;
+        const float *src = partial + ((size_t)gr.split[g] * K + k) * row + c;
+        float s[VEC], v[8][VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s[e] = 0.f;
+        for (int q = 0; q < parts; q += 8) {                     // addresses are clamped instead of tested: eight loads in flight
+#pragma unroll
+            for (int u = 0; u < 8; ++u) qmlb::load_f32<float, VEC>(src + (size_t)min(q + u, parts - 1) * K * row, v[u]);
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) s[e] += q + u < parts ? v[u][e] : 0.f;
+        }
+        T *to = dW + ((size_t)g * K + k) * N + c;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+            if (c + e < (unsigned)N) to[e] = qmlb::from_f32<T>(s[e]);
     }
 }
 
 template <typename T>
 int join(T *dW, const int *start, size_t n, int G, int K, int N, int split, size_t row, const float *partial, cudaStream_t st) {
+    const size_t several = n / split < (size_t)G ? n / split : (size_t)G;       // groups of several parts, at most
+    if (several == 0 || n == (size_t)split) return qmlb::check_launch("qmlb_grouped_matmul_wgrad");
     // Four values a thread once they fill the SMs (784 x 256, 5 groups of 330,000 rows: 203 us against 209 us for the whole call;
-    // 18 groups of 240 x 1080: 174 against 201; 240 x 228: 26 against 24).  At most 16 blocks an SM over all groups: a group of one
-    // part needs none of its blocks: 64 groups of 256 rows take 2 us more than with 8, 8 groups of 2048 x 2048 15 us less.
+    // 18 groups of 240 x 1080: 174 against 201; 240 x 228: 26 against 24).  16 blocks an SM over the groups (8 groups of 2,048 x 2,048:
+    // 620 us, with 8 blocks 636 us).
     const bool small = (size_t)K * N < (size_t)148 * 512;
-    const size_t per = ((size_t)K * (small ? N : (N + 3) / 4) + 255) / 256, most = (size_t)(148 * 16 + G - 1) / G;
-    const dim3 grid((unsigned)(per < most ? per : most), (unsigned)G);
+    const size_t per = ((size_t)K * (small ? N : (N + 3) / 4) + 255) / 256, most = (148 * 16 + several - 1) / several;
+    const dim3 grid((unsigned)(per < most ? per : most), (unsigned)several);
     const size_t smem = (size_t)3 * (G + 1) * 4;
     if (small) join_kernel<T, 1><<<grid, 256, smem, st>>>(start, partial, (int)n, G, K, N, split, row, dW);
     else join_kernel<T, 4><<<grid, 256, smem, st>>>(start, partial, (int)n, G, K, N, split, row, dW);
