@@ -134,6 +134,29 @@ def test_gradient_with_segments_of_chosen_lengths():
             R.assert_within(got, exact, R.sum_bound(exact, mag, terms.view(-1, 1), dtype), str(lengths[:8]))
 
 
+@pytest.mark.parametrize('dtype', R.TYPES)
+@pytest.mark.parametrize('width', [4, 5, 7, 8, 9, 10, 15, 17, 18, 33, 301])
+@pytest.mark.parametrize('n', [1, 2, 3, 29, 1000, 20001])
+def test_lookup_of_odd_widths(n, width, dtype):
+    """Rows that end anywhere in a 16-byte piece of the result: every element is its own, nothing behind the result is written,
+    and rows that nothing names may hold anything."""
+    from qml_lightning_b200 import cabi
+    g = gen(n + width)
+    rows = 37
+    table = randn(g, rows, width, dtype=dtype)
+    table[0] = float('nan')                                            # read for an index outside, and not used
+    for bits in (torch.int32, torch.int64):
+        idx = torch.randint(-1, rows + 2, (n,), generator=g, device=DEV, dtype=bits)
+        idx[idx == 0] = -5
+        flat = torch.full((n * width + 64,), 9.0, dtype=dtype, device=DEV)
+        exact = R.lookup(idx, table, 1.5)
+        out = cabi.embedding(idx, table, 1.5, out=flat[:n * width].view(n, width))
+        R.assert_within(out, exact, R.lookup_bound(exact, dtype), f'{n} {width}')
+        assert (flat[n * width:] == 9).all()
+        shifted = flat[3:3 + n * width].view(n, width)                 # a result off the 16-byte boundary
+        R.assert_within(cabi.embedding(idx, table, 1.5, out=shifted), exact, R.lookup_bound(exact, dtype), f'{n} {width} shifted')
+
+
 def test_lookup_special_inputs():
     from qml_lightning_b200 import cabi
     table = randn(gen(0), 5, 6)
