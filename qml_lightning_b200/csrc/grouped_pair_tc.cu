@@ -21,6 +21,11 @@
 // them, two per scheduler.  Measured on 210,000 x (336, 256): gradient 486 us with 4 and NT = 256, 368 us with 8 and NT = 128;
 // products of rows 182 us with 4 and NT = 256, 251 us with 8 and NT = 128 (there every row is split twice).
 // Registers are moved between the warps by setmaxnreg.
+//
+// Results that are not finite.  An infinity times the zero low part of another number is NaN, and sums in scaled units leave the
+// range before their results do.  So a folding warp remembers its tiles with such results and, when no other warp waits for it any
+// more, forms these results again as plain sums of fused multiply-adds over the operands as they are: they come out as a product in
+// 32 bits gives them.  Finite tiles pay one packed multiply-add per two results for the test.
 #include <cuda_fp16.h>
 #include <string.h>
 
@@ -62,6 +67,7 @@ struct Shape {
     int stages;
     uint32_t b_half;         // one image of the NT-wide operand
     int a_access, b_access, out_access;
+    size_t w_depth, w_col;   // steps of the matrix as it is, along the depth and along the columns (products of rows)
 };
 
 // power of two that takes the largest magnitude `m` to [2^(top - 254), 2^(top - 253)), and its inverse; both normal numbers
@@ -112,7 +118,25 @@ __device__ __forceinline__ void sts64(uint32_t at, uint32_t a, uint32_t b) {
     asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(a), "r"(b) : "memory");
 }
 
-// Products of rows: a = x [n, K], packed/pack_scales = images of the matrices, result y [n, out].
+// sum of a[d * a_step] * b[d * b_step] over the depth in 32 bits, by all lanes of a warp; only `wanted` ones go on for the others
+__device__ __forceinline__ float plain_sum(const float *__restrict__ a, size_t a_step, const float *__restrict__ b, size_t b_step, int depth, bool wanted) {
+    float s = 0.f;
+    for (int d0 = 0; d0 < depth && __any_sync(QMLB_FULL_MASK, wanted && !isnan(s)); d0 += 8) {      // NaN stays
+        float u[8], v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {                    // addresses are clamped instead of tested: all loads are in flight together
+            const size_t d = (size_t)min(d0 + i, depth - 1);
+            u[i] = a[d * a_step];
+            v[i] = b[d * b_step];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (d0 + i < depth) s = fmaf(u[i], v[i], s);
+    }
+    return s;
+}
+
+// Products of rows: a = x [n, K], b = the matrices, packed/pack_scales = their images, result y [n, out].
 // GRAD: a = x [n, K], b = dy [n, out], result dW [G, K, out], partial = parts of split groups.
 template <bool GRAD>
 __global__ void __launch_bounds__(Config<GRAD>::THREADS, 1)
@@ -475,7 +499,33 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
         const uint32_t lane_field = (uint32_t)(quarter * 32) << 16;
         int it = 0, slot = 0;
         bool ok = true;
-        for (int unit = blockIdx.x; unit < total; unit += gridDim.x) {
+        // where a tile goes: rows of y, of dW, or of a part
+        auto target = [&](int g, int part, int r0, int r1, int k0, int nt, size_t &row_floats, int &rows, int &width, int &access) {
+            const int col0 = nt * p.NT + h * half;
+            float *to;
+            row_floats = (size_t)p.out;
+            width = p.out - col0;
+            access = p.out_access;
+            if (!GRAD) {
+                to = out + (size_t)(r0 + quarter * 32) * row_floats + col0;
+                rows = min(32, r1 - r0 - quarter * 32);
+            } else {
+                rows = min(32, p.K - k0 - quarter * 32);
+                if (gr.parts[g + 1] - gr.parts[g] == 1) {
+                    to = out + ((size_t)g * p.K + k0 + quarter * 32) * row_floats + col0;
+                } else {
+                    const size_t part_slot = (size_t)(gr.split[g] + part - gr.parts[g]);
+                    row_floats = (size_t)p.ntiles * p.NT;
+                    to = partial + (part_slot * p.K + k0 + quarter * 32) * row_floats + col0;
+                    width = half;
+                    access = 16;
+                }
+            }
+            width = min(width, half);
+            return to;
+        };
+        unsigned long long odd = 0;                             // units with results that are not finite (the last bit: all from the 64th on)
+        for (int unit = blockIdx.x, nth = 0; unit < total; unit += gridDim.x, ++nth) {
             int g, part, r0, r1, k0, nt;
             locate(unit, g, part, r0, r1, k0, nt);
             const int chunks = chunks_of(r0, r1);
@@ -533,33 +583,10 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
             }
             // undo the columns' scales (of the last chunk; every chunk carries them)
             const float *cols = scale + (size_t)(slot == 0 ? slots - 1 : slot - 1) * SLOT + 128 + h * half;
-            // where the tile goes: rows of y, of dW, or of a part
-            const int col0 = nt * p.NT + h * half;
-            float *to;
             size_t row_floats;
             int rows, width, access;
-            if (!GRAD) {
-                row_floats = (size_t)p.out;
-                to = out + (size_t)(r0 + quarter * 32) * row_floats + col0;
-                rows = min(32, r1 - r0 - quarter * 32);
-                width = p.out - col0;
-                access = p.out_access;
-            } else {
-                rows = min(32, p.K - k0 - quarter * 32);
-                if (gr.parts[g + 1] - gr.parts[g] == 1) {
-                    row_floats = (size_t)p.out;
-                    to = out + ((size_t)g * p.K + k0 + quarter * 32) * row_floats + col0;
-                    width = p.out - col0;
-                    access = p.out_access;
-                } else {
-                    const size_t part_slot = (size_t)(gr.split[g] + part - gr.parts[g]);
-                    row_floats = (size_t)p.ntiles * p.NT;
-                    to = partial + (part_slot * p.K + k0 + quarter * 32) * row_floats + col0;
-                    width = half;
-                    access = 16;
-                }
-            }
-            width = min(width, half);
+            float *to = target(g, part, r0, r1, k0, nt, row_floats, rows, width, access);
+            float2 test = make_float2(0.f, 0.f);                // stays zero while all results are finite
 #pragma unroll
             for (int cc = 0; cc < HALF; cc += 16) {
                 if (cc < half) {
@@ -568,6 +595,10 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
                     for (int q = 0; q < 4; ++q) {
                         const float4 f = *reinterpret_cast<const float4 *>(cols + cc + q * 4);
                         const float2 lo = __fmul2_rn(acc[cc / 2 + q * 2], make_float2(f.x, f.y)), hi = __fmul2_rn(acc[cc / 2 + q * 2 + 1], make_float2(f.z, f.w));
+                        if (cc + q * 4 < half) {                // (what lies behind is no result of this warp)
+                            test = __ffma2_rn(lo, make_float2(0.f, 0.f), test);
+                            test = __ffma2_rn(hi, make_float2(0.f, 0.f), test);
+                        }
                         *reinterpret_cast<float4 *>(mine + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) = make_float4(lo.x, lo.y, hi.x, hi.y);
                     }
                     __syncwarp();
@@ -596,6 +627,31 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
                         }
                     }
                     __syncwarp();
+                }
+            }
+            if (__any_sync(QMLB_FULL_MASK, test.x + test.y != 0.f)) odd |= 1ull << min(nth, 63);
+        }
+        // what is not finite, as a product in 32 bits gives it (nobody waits for this warp any more)
+        for (int unit = blockIdx.x, nth = 0; unit < total && odd && ok; unit += gridDim.x, ++nth) {
+            if (!((odd >> min(nth, 63)) & 1)) continue;
+            int g, part, r0, r1, k0, nt, rows, width, access;
+            locate(unit, g, part, r0, r1, k0, nt);
+            size_t row_floats;
+            float *to = target(g, part, r0, r1, k0, nt, row_floats, rows, width, access);
+            width = min(width, p.out - nt * p.NT - h * half);   // a part's row has room for columns that do not exist
+            for (int r = 0; r < rows; ++r) {
+                for (int cc = 0; cc < width; cc += 32) {
+                    const int c = min(cc + lane, width - 1), col = nt * p.NT + h * half + c;
+                    float *at = to + (size_t)r * row_floats + c;
+                    const bool wanted = cc + lane < width && !isfinite(*at);
+                    if (!__any_sync(QMLB_FULL_MASK, wanted)) continue;
+                    float v;
+                    if (GRAD) {
+                        v = plain_sum(a_in + (size_t)r0 * p.K + k0 + quarter * 32 + r, (size_t)p.K, b_in + (size_t)r0 * p.out + col, (size_t)p.out, r1 - r0, wanted);
+                    } else {
+                        v = plain_sum(a_in + (size_t)(r0 + quarter * 32 + r) * p.K, 1, b_in + (size_t)g * p.K * p.out + (size_t)col * p.w_col, p.w_depth, p.K, wanted);
+                    }
+                    if (wanted) *at = v;
                 }
             }
         }
@@ -710,6 +766,8 @@ int grouped_pair(const float *x, const float *W, const int *start, size_t n, int
     Shape p = product_shape(n, G, K, N, transpose);
     p.a_access = access_bytes((size_t)p.K * 4, 4, x);
     p.out_access = access_bytes((size_t)p.out * 4, 4, out);
+    p.w_depth = transpose ? 1 : (size_t)N;
+    p.w_col = transpose ? (size_t)N : 1;
     unsigned char *packed = static_cast<unsigned char *>(workspace);
     const size_t images = (size_t)G * p.ntiles * p.nchunks;
     float *pack_scales = reinterpret_cast<float *>(packed + images * (2 * p.b_half));
@@ -719,7 +777,7 @@ int grouped_pair(const float *x, const float *W, const int *start, size_t n, int
     const long units = ((long)((n + BM - 1) / BM) + G) * p.ntiles;
     const size_t smem = smem_of<false>(p);
     if (int rc = ensure_smem(pair_kernel<false>, smem, "qmlb_grouped_matmul")) return rc;
-    pair_kernel<false><<<(unsigned)(units < 148 ? units : 148), Config<false>::THREADS, smem, st>>>(x, nullptr, packed, pack_scales, start, p, out, nullptr);
+    pair_kernel<false><<<(unsigned)(units < 148 ? units : 148), Config<false>::THREADS, smem, st>>>(x, W, packed, pack_scales, start, p, out, nullptr);
     return check_launch("qmlb_grouped_matmul");
 }
 
