@@ -1,32 +1,32 @@
 // Products of ragged groups of rows with one matrix each, float32 operands, on the 16-bit tensor cores.
 //
-// Arithmetic.  A stretch of 64 values along the depth (of one row or one column of an operand) is scaled by a power of two
-// so that its largest lies in [2^14, 2^15), and every scaled value x is split into two fp16 numbers, x ~ h + l:
-// h = fp16(x), l = fp16(x - h), off by at most 2^-22 |x| (and 2^-39 of the stretch's largest value, where l would be
-// subnormal).  A product is h h' + h l' + l h' (l l' is at most 2^-22 of it), so three 16-bit products give a 32-bit one
-// where bf16 parts would need six and tf32 parts three of twice the cost.  Sums: the tensor core truncates when it adds, so
-// an accumulator only ever covers one stretch (4 steps: the small cross terms first, then h h'), and warps of CUDA cores add
-// the stretches in registers in 32 bits, rounded, undoing both scales on the way.  Against 64 bits the results are off by
-// about 2e-7 of their norm, like a float32 product, and rows and columns keep their own magnitudes.
+// Arithmetic.  A value x is the sum of three bf16 numbers, x = a + b + c: a = bf16(x), b = bf16(x - a), c = x - a - b, each rounded to
+// nearest, 8 + 8 + 8 bits, |b| <= 2^-9 |x|, |c| <= 2^-18 |x|.  A product is a a' + a b' + b a' + b b' + a c' + c a'; the other three are
+// less than 2^-25 of it.  bf16 has the exponents of float32, so this holds for every value by itself, whatever stands beside it
+// (two fp16 parts on a common scale would take three products, but lose the small values of a stretch that holds large ones).  The
+// parts of values below 2^-110 would leave the range, so all values are multiplied by 2^16 on their way in, and sums by 2^-32 on
+// their way out: every normal number enters exactly, and a sum may reach 2^96 before it overflows (see below).  Sums: the tensor core
+// truncates when it adds, so an accumulator only ever covers one stretch of 64 values (the small products first, then a a'), and
+// warps of CUDA cores add the stretches in registers in 32 bits, rounded.  Against 64 bits the results are off by about 2e-7 of
+// their norm, like a float32 product.
 //
 // Work split.  One persistent block per SM takes tiles of 128 x NT results:
-//   warp 0          bulk copies of the matrix operand's images (products of rows; a packing kernel makes the images)
+//   warp 0          bulk copies of the matrix operand's images (products of rows; a packing kernel makes the images), one of the
+//                   three parts at a time: a part's place is free again once the products that need it are issued and done
 //   warp 1          issues tcgen05.mma, several tensor-memory accumulators in turn
 //   warps 2-3       zero rows outside the groups, zero matrices of groups without rows
-//   loading warps   load float32 rows, find the scales, split, and write the swizzled operand images to shared memory
+//   loading warps   load float32 rows, split, and write the swizzled operand images to shared memory
 //   folding warps   (eight) add the finished accumulators to their registers, and store the tile
 // Products of rows: NT <= 256, 4 loading warps, 128 sums per folding thread.  Gradient of the matrices: both operands are loaded
-// by the loading warps (the depth runs over the rows of the group, the operands' lines run across it, the stretches are 64 rows
-// of one column), so their chains of loads, shuffles and conversions bound the kernel; NT <= 128 leaves registers for eight of
-// them, two per scheduler.  Measured on 210,000 x (336, 256): gradient 486 us with 4 and NT = 256, 368 us with 8 and NT = 128;
-// products of rows 182 us with 4 and NT = 256, 251 us with 8 and NT = 128 (there every row is split twice).
+// by the loading warps (the depth runs over the rows of the group, the operands' lines run across it), and NT <= 128 leaves
+// registers for eight of them, two per scheduler.
 // Registers are moved between the warps by setmaxnreg.
 //
-// Results that are not finite.  An infinity times the zero low part of another number is NaN, and sums in scaled units leave the
-// range before their results do.  So a folding warp remembers its tiles with such results and, when no other warp waits for it any
+// Results that are not finite.  An infinity times the zero low part of another number is NaN, and scaled sums leave the range before
+// their results do.  So a folding warp remembers its tiles with such results and, when no other warp waits for it any
 // more, forms these results again as plain sums of fused multiply-adds over the operands as they are: they come out as a product in
 // 32 bits gives them.  Finite tiles pay one packed multiply-add per two results for the test.
-#include <cuda_fp16.h>
+#include <cuda_bf16.h>
 #include <string.h>
 
 #include "grouped_rows.cuh"
@@ -37,9 +37,10 @@ namespace {
 using namespace qmlb::tc;
 
 constexpr int BM = 128;
-constexpr uint32_t A_HALF = BM * BK * 2;          // one image (high or low parts) of the 128-wide operand
+constexpr uint32_t A_IMAGE = BM * BK * 2;         // one part of the 128-wide operand
+constexpr float SCALE = 65536.f, UNSCALE = 1.f / (SCALE * SCALE);
 constexpr int TMA_WARP = 0, MMA_WARP = 1, LOAD_WARP = 4;
-constexpr int MAXST = 4;
+constexpr int MAXST = 4, MAXSLOT = 6;
 template <bool GRAD>
 struct Config {
     static constexpr int LOADERS = GRAD ? 8 : 4, FOLD_WARP = LOAD_WARP + LOADERS, THREADS = (FOLD_WARP + 8) * 32;
@@ -49,9 +50,6 @@ struct Config {
     // does not exceed what the block was launched with
     static constexpr int R_LAUNCH = GRAD ? 96 : 128, R_FIRST = 40, R_LOAD = 112, R_FOLD = GRAD ? 104 : 176;
     static_assert(R_FIRST * 4 + R_LOAD * LOADERS + R_FOLD * 8 <= R_LAUNCH * (4 + LOADERS + 8), "register split");
-    // per chunk: inverse scales of the 128 rows and of the columns of the tile; gradient: also the factors by which the columns'
-    // units change with this chunk, and a flag per loading warp that says whether any does
-    static constexpr int RATIO = 128 + NT, FLAGS = RATIO + NT, SLOT = GRAD ? FLAGS + 8 : 128 + NT;
 };
 constexpr int PART_COST = 384;                    // of a part of a sum through scratch, in rows
 constexpr int AHEAD = 4;                          // stretches by which rows are asked into L2 in front of their loads
@@ -64,25 +62,23 @@ struct Shape {
     int NT, ntiles, ktiles;  // ktiles: tiles of 128 columns of x (gradient)
     int nchunks;             // stretches of the depth (products of rows)
     int split;               // rows per part (gradient)
-    int stages;
-    uint32_t b_half;         // one image of the NT-wide operand
+    int stages;              // of the 128-wide operand's three parts (gradient: and the other's)
+    int slots;               // of one part of the NT-wide operand (products of rows)
+    uint32_t b_image;        // one part of the NT-wide operand
     int a_access, b_access, out_access;
     size_t w_depth, w_col;   // steps of the matrix as it is, along the depth and along the columns (products of rows)
 };
 
-// power of two that takes the largest magnitude `m` to [2^(top - 254), 2^(top - 253)), and its inverse; both normal numbers
-__device__ __forceinline__ void scales(float m, int top, float &s, float &inv) {
-    const int e = min(top - (int)(__float_as_uint(m) >> 23), 253);
-    s = __uint_as_float((uint32_t)e << 23);
-    inv = __uint_as_float((uint32_t)(254 - e) << 23);
-}
-// x s = h + l: high and low parts of two values
-__device__ __forceinline__ void split2(float2 x, float2 s, uint32_t &hi, uint32_t &lo) {
-    const __half2 h = __float22half2_rn(__fmul2_rn(x, s));
-    const float2 f = __half22float2(h);
-    const __half2 l = __float22half2_rn(__ffma2_rn(x, s, make_float2(-f.x, -f.y)));      // exact: s is a power of two
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = *reinterpret_cast<const uint32_t *>(&l);
+// the three parts of two values
+__device__ __forceinline__ void split2(float2 x, uint32_t (&part)[3]) {
+    x = __fmul2_rn(x, make_float2(SCALE, SCALE));
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        const __nv_bfloat162 h = __float22bfloat162_rn(x);
+        part[i] = *reinterpret_cast<const uint32_t *>(&h);
+        // minus the part: its bits are the upper halves of two floats
+        x = __fadd2_rn(x, make_float2(__uint_as_float((part[i] << 16) ^ 0x80000000u), __uint_as_float((part[i] & 0xffff0000u) ^ 0x80000000u)));
+    }
 }
 // Four consecutive floats, of which the first `valid` exist (the others become zeros).  Predicated loads without a branch: behind
 // a branch the compiler waits for each load before the next.
@@ -136,25 +132,24 @@ __device__ __forceinline__ float plain_sum(const float *__restrict__ a, size_t a
     return s;
 }
 
-// Products of rows: a = x [n, K], b = the matrices, packed/pack_scales = their images, result y [n, out].
+// Products of rows: a = x [n, K], b = the matrices, packed = their images, result y [n, out].
 // GRAD: a = x [n, K], b = dy [n, out], result dW [G, K, out], partial = parts of split groups.
 template <bool GRAD>
 __global__ void __launch_bounds__(Config<GRAD>::THREADS, 1)
 pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, const unsigned char *__restrict__ packed,
-            const float *__restrict__ pack_scales, const int *__restrict__ start, Shape p, float *__restrict__ out, float *__restrict__ partial) {
+            const int *__restrict__ start, Shape p, float *__restrict__ out, float *__restrict__ partial) {
     using C = Config<GRAD>;
-    constexpr int NACC = C::ACCS, NT_MAX = C::NT, FOLD_WARP = C::FOLD_WARP, SLOT = C::SLOT, RATIO = C::RATIO, FLAGS = C::FLAGS, HALF = C::NT / 2;
+    constexpr int NACC = C::ACCS, NT_MAX = C::NT, FOLD_WARP = C::FOLD_WARP, HALF = C::NT / 2;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t full[MAXST], empty[MAXST], acc_full[NACC], acc_free[NACC], done;
+    __shared__ __align__(8) uint64_t full[MAXST], empty[MAXST], b_full[MAXSLOT], b_empty[MAXSLOT], acc_full[NACC], acc_free[NACC], done;
     __shared__ uint32_t tmem_slot;
     __shared__ int failed;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
     unsigned char *sp = smem_raw + (sbase - smem_u32(smem_raw));
-    const uint32_t stage_bytes = 2 * A_HALF + 2 * p.b_half;
-    const int slots = p.stages + NACC + 1;        // scales outlive their stage until the accumulator is folded and stored
-    float *scale = reinterpret_cast<float *>(sp + (size_t)p.stages * stage_bytes);
-    unsigned char *epi = reinterpret_cast<unsigned char *>(scale + (size_t)slots * SLOT);
+    const uint32_t stage_bytes = 3 * A_IMAGE + (GRAD ? 3 * p.b_image : 0u);
+    const uint32_t b_ring = sbase + (uint32_t)p.stages * stage_bytes;                 // products of rows
+    unsigned char *epi = sp + (size_t)p.stages * stage_bytes + (GRAD ? 0u : (size_t)p.slots * p.b_image);
     Groups gr;
     gr.start = reinterpret_cast<int *>(epi + EPI);
     gr.parts = gr.start + p.G + 1;
@@ -163,9 +158,10 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
 
     if (tid == 0) {
         for (int s = 0; s < p.stages; ++s) {
-            mbar_init(bar(full[s]), C::LOADERS + (GRAD ? 0 : 1));     // the loading warps, and the issuer of the bulk copies
+            mbar_init(bar(full[s]), C::LOADERS);
             mbar_init(bar(empty[s]), 1);
         }
+        for (int s = 0; s < p.slots; ++s) { mbar_init(bar(b_full[s]), 1); mbar_init(bar(b_empty[s]), 1); }
         for (int i = 0; i < NACC; ++i) { mbar_init(bar(acc_full[i]), 1); mbar_init(bar(acc_free[i]), 8); }
         mbar_init(bar(done), 1);
         failed = 0;
@@ -195,59 +191,82 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::R_FIRST));
         if (warp == TMA_WARP) {
             if (!GRAD && lane == 0) {
-                int it = 0, slot = 0;
+                int it = 0;
                 bool ok = true;
                 for (int unit = blockIdx.x; unit < total && ok; unit += gridDim.x) {
                     int g, part, r0, r1, k0, nt;
                     locate(unit, g, part, r0, r1, k0, nt);
-                    const size_t image = (size_t)(g * p.ntiles + nt) * p.nchunks;
-                    for (int c = 0; c < p.nchunks; ++c, ++it) {
-                        const int s = it % p.stages;
-                        if (!mbar_wait(bar(empty[s]), ((uint32_t)(it / p.stages) & 1u) ^ 1u, gave_up)) { ok = false; break; }
-                        mbar_expect_tx(bar(full[s]), 2 * p.b_half + (uint32_t)p.NT * 4u);
-                        bulk_copy(sbase + (uint32_t)s * stage_bytes + 2 * A_HALF, packed + (image + c) * (2 * p.b_half), 2 * p.b_half, bar(full[s]));
-                        bulk_copy(smem_u32(scale + (size_t)slot * SLOT + 128), pack_scales + (image + c) * p.NT, (uint32_t)p.NT * 4u, bar(full[s]));
-                        slot = slot + 1 == slots ? 0 : slot + 1;
+                    const unsigned char *image = packed + (size_t)(g * p.ntiles + nt) * p.nchunks * (3 * p.b_image);
+                    for (int c = 0; c < p.nchunks * 3; ++c, ++it) {           // c, b, a of every stretch
+                        const int s = it % p.slots;
+                        if (!mbar_wait(bar(b_empty[s]), ((uint32_t)(it / p.slots) & 1u) ^ 1u, gave_up)) { ok = false; break; }
+                        mbar_expect_tx(bar(b_full[s]), p.b_image);
+                        bulk_copy(b_ring + (uint32_t)s * p.b_image, image + (size_t)c * p.b_image, p.b_image, bar(b_full[s]));
                     }
                 }
                 if (!ok) failed = 1;
-                for (int i = max(0, it - p.stages); i < it; ++i)          // no copy may be in flight when the block leaves
-                    for (int tries = 0; tries < WAIT_LIMIT && !mbar_try(bar(full[i % p.stages]), (uint32_t)(i / p.stages) & 1u); ++tries) {}
+                for (int i = max(0, it - p.slots); i < it; ++i)           // no copy may be in flight when the block leaves
+                    for (int tries = 0; tries < WAIT_LIMIT && !mbar_try(bar(b_full[i % p.slots]), (uint32_t)(i / p.slots) & 1u); ++tries) {}
             }
         } else if (warp == MMA_WARP) {
-            const uint32_t idesc = instr_desc(false, GRAD, GRAD, BM, p.NT);
+            const uint32_t idesc = instr_desc(true, GRAD, GRAD, BM, p.NT);
             constexpr uint32_t step = GRAD ? 128u : 2u, block = GRAD ? 8192u : 16u;
-            int it = 0;
+            int it = 0, bt = 0;
             bool ok = true;
             for (int unit = blockIdx.x; unit < total && ok; unit += gridDim.x) {
                 int g, part, r0, r1, k0, nt;
                 locate(unit, g, part, r0, r1, k0, nt);
                 const int chunks = chunks_of(r0, r1), depth = GRAD ? r1 - r0 : p.K;
-                for (int c = 0; c < chunks; ++c, ++it) {
+                for (int c = 0; c < chunks && ok; ++c, ++it) {
                     const int s = it % p.stages, buf = it % NACC;
                     bool w = mbar_wait(bar(acc_free[buf]), ((uint32_t)(it / NACC) & 1u) ^ 1u, gave_up);
                     w = w && mbar_wait(bar(full[s]), (uint32_t)(it / p.stages) & 1u, gave_up, it ? WAIT_LIMIT : QMLB_TEST_FIRST_WAIT_POLLS);
                     if (!__all_sync(QMLB_FULL_MASK, w)) { ok = false; break; }
                     fence_after();
                     const int steps = min(BK / 16, (depth - c * BK + 15) / 16);
-                    const uint32_t a = sbase + (uint32_t)s * stage_bytes, b = a + 2 * A_HALF, d = tmem + (uint32_t)buf * NT_MAX;
-                    const uint32_t ah = desc_lo(a, block), al = desc_lo(a + A_HALF, block), bh = desc_lo(b, block), bl = desc_lo(b + p.b_half, block);
-                    if (elect_one()) {
+                    const uint32_t a = sbase + (uint32_t)s * stage_bytes, d = tmem + (uint32_t)buf * NT_MAX;
+                    // part i of the one operand times the part at `b` of the other
+                    auto multiply = [&](int i, uint32_t b, bool first) {
+                        const uint32_t al = desc_lo(a + (uint32_t)i * A_IMAGE, block), bl = desc_lo(b, block);
 #pragma unroll
                         for (int k = 0; k < BK / 16; ++k) {
                             if (k >= steps) break;
-                            mma_f16(d, ah + k * step, DESC_HI_SW128, bl + k * step, DESC_HI_SW128, idesc, k ? 1u : 0u);
-                            mma_f16(d, al + k * step, DESC_HI_SW128, bh + k * step, DESC_HI_SW128, idesc, 1u);
+                            mma_f16(d, al + k * step, DESC_HI_SW128, bl + k * step, DESC_HI_SW128, idesc, first && k == 0 ? 0u : 1u);
                         }
-#pragma unroll
-                        for (int k = 0; k < BK / 16; ++k) {
-                            if (k >= steps) break;
-                            mma_f16(d, ah + k * step, DESC_HI_SW128, bh + k * step, DESC_HI_SW128, idesc, 1u);
+                    };
+                    if (GRAD) {
+                        const uint32_t b = a + 3 * A_IMAGE;
+                        if (elect_one()) {
+                            multiply(0, b + 2 * p.b_image, true);
+                            multiply(2, b, false);
+                            multiply(1, b + p.b_image, false);
+                            multiply(0, b + p.b_image, false);
+                            multiply(1, b, false);
+                            multiply(0, b, false);
+                            mma_commit(bar(empty[s]));
+                            mma_commit(bar(acc_full[buf]));
                         }
-                        mma_commit(bar(empty[s]));
-                        mma_commit(bar(acc_full[buf]));
+                        __syncwarp();
+                    } else {
+#pragma unroll 1
+                        for (int j = 2; j >= 0; --j, ++bt) {                  // parts c, b, a of the matrix
+                            const int slot = bt % p.slots;
+                            w = mbar_wait(bar(b_full[slot]), (uint32_t)(bt / p.slots) & 1u, gave_up);
+                            if (!__all_sync(QMLB_FULL_MASK, w)) { ok = false; break; }
+                            const uint32_t b = b_ring + (uint32_t)slot * p.b_image;
+                            if (elect_one()) {
+                                if (j == 0) multiply(2, b, false);
+                                if (j <= 1) multiply(1, b, false);
+                                multiply(0, b, j == 2);
+                                mma_commit(bar(b_empty[slot]));
+                                if (j == 0) {
+                                    mma_commit(bar(empty[s]));
+                                    mma_commit(bar(acc_full[buf]));
+                                }
+                            }
+                            __syncwarp();
+                        }
                     }
-                    __syncwarp();
                 }
             }
             if (!ok) failed = 1;
@@ -337,7 +356,7 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
             place();
             fetch(0, v[0]);
             fetch(1, v[1]);
-            int s = 0, slot = 0;
+            int s = 0;
             uint32_t phase = 1;
             while (unit < total) {
                 ok = __all_sync(QMLB_FULL_MASK, mbar_wait(bar(empty[s]), phase, gave_up));
@@ -346,21 +365,19 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
                 auto put = [&](int h, const float2 (&t)[4][4]) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        float m = 0.f;
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) m = fmaxf(m, fmaxf(fabsf(t[i][q].x), fabsf(t[i][q].y)));
-#pragma unroll
-                        for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(QMLB_FULL_MASK, m, o));
-                        float sc, inv;
-                        scales(m, 268, sc, inv);
                         const int r = w * 32 + (h * 4 + i) * 4 + lr;
-                        if (kc == 0) scale[(size_t)slot * SLOT + r] = inv;
-                        uint32_t hi[4], lo[4];
+                        uint32_t v[3][4];
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) split2(t[i][q], make_float2(sc, sc), hi[q], lo[q]);
+                        for (int q = 0; q < 4; ++q) {
+                            uint32_t u[3];
+                            split2(t[i][q], u);
+                            v[0][q] = u[0];
+                            v[1][q] = u[1];
+                            v[2][q] = u[2];
+                        }
                         const uint32_t at = a + (uint32_t)r * 128u + ((uint32_t)(kc ^ (r & 7)) << 4);
-                        sts128(at, hi);
-                        sts128(at + A_HALF, lo);
+#pragma unroll
+                        for (int e = 0; e < 3; ++e) sts128(at + (uint32_t)e * A_IMAGE, v[e]);
                     }
                 };
                 prefetch();
@@ -372,7 +389,6 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(full[s]));
-                slot = slot + 1 == slots ? 0 : slot + 1;
                 if (++s == p.stages) { s = 0; phase ^= 1u; }
             }
         } else {
@@ -387,12 +403,11 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
                 locate(u.unit, g, part, u.r, u.r1, u.k0, nt);
                 u.n0 = nt * p.NT;
             };
-            auto advance = [&](Cursor &u) {                           // true: another part begins
+            auto advance = [&](Cursor &u) {
                 u.r += BK;
-                if (u.r < u.r1) return false;
+                if (u.r < u.r1) return;
                 u.unit += gridDim.x;
                 place(u);
-                return true;
             };
             auto fetch = [&](const Cursor &u, const float *in, int first, int width, int access, float2 (&t)[8][2]) {
                 if (u.unit >= total) return;
@@ -410,85 +425,35 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
             place(at);
             fetch(at, a_in, at.k0, p.K, p.a_access, v[0]);
             if (has_b) fetch(at, b_in, at.n0, p.out, p.b_access, v[1]);
-            int s = 0, slot = 0;
+            int s = 0;
             uint32_t phase = 1;
-            bool first = true;
-            float unit_of[4] = {1.f, 1.f, 1.f, 1.f};                  // present scales of this thread's columns of dy
-            auto largest = [&](const float2 (&t)[8][2], float (&m)[4]) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) m[q] = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    m[0] = fmaxf(m[0], fabsf(t[i][0].x));
-                    m[1] = fmaxf(m[1], fabsf(t[i][0].y));
-                    m[2] = fmaxf(m[2], fabsf(t[i][1].x));
-                    m[3] = fmaxf(m[3], fabsf(t[i][1].y));
-                }
-#pragma unroll
-                for (int o = 4; o < 32; o <<= 1)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) m[q] = fmaxf(m[q], __shfl_xor_sync(QMLB_FULL_MASK, m[q], o));
-            };
-            auto store = [&](const float2 (&t)[8][2], const float (&sc)[4], uint32_t to, uint32_t half) {
+            auto store = [&](const float2 (&t)[8][2], uint32_t to, uint32_t image) {
                 to += (uint32_t)(col >> 6) * 8192u + (uint32_t)rr * 128u + ((uint32_t)((col & 63) * 2) ^ ((uint32_t)rr << 4));
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    uint32_t h0, h1, l0, l1;
-                    split2(t[i][0], make_float2(sc[0], sc[1]), h0, l0);
-                    split2(t[i][1], make_float2(sc[2], sc[3]), h1, l1);
-                    sts64(to + (uint32_t)i * 1024u, h0, h1);
-                    sts64(to + half + (uint32_t)i * 1024u, l0, l1);
+                    uint32_t u[3], v[3];
+                    split2(t[i][0], u);
+                    split2(t[i][1], v);
+#pragma unroll
+                    for (int e = 0; e < 3; ++e) sts64(to + (uint32_t)e * image + (uint32_t)i * 1024u, u[e], v[e]);
                 }
             };
             while (at.unit < total) {
                 if (!(ok = __all_sync(QMLB_FULL_MASK, mbar_wait(bar(empty[s]), phase, gave_up)))) break;
                 const uint32_t stage = sbase + (uint32_t)s * stage_bytes;
-                float *mine = scale + (size_t)slot * SLOT;
                 Cursor next = at;
-                const bool begins = advance(next);
-                float m[4], sc[4], inv[4];
-                largest(v[0], m);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) scales(m[q], 268, sc[q], inv[q]);
-                if (rr == 0) *reinterpret_cast<float4 *>(mine + col) = make_float4(inv[0], inv[1], inv[2], inv[3]);
-                store(v[0], sc, stage, A_HALF);
+                advance(next);
+                store(v[0], stage, A_IMAGE);
                 fetch(next, a_in, next.k0, p.K, p.a_access, v[0]);
-                bool changed = false;
                 if (has_b) {
-                    // The sums of a column of dy are kept in its unit: the scale of the part's first stretch, with room for values up to
-                    // 32 times larger.  A stretch that needs more changes the unit, and the sums with it.
-                    float ratio[4];
-                    largest(v[1], m);
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        float now, inverse;
-                        scales(m[q], 264, now, inverse);
-                        const float had = unit_of[q];
-                        const bool keep = !first && m[q] * had < 60000.f;
-                        ratio[q] = 1.f;
-                        if (!first && !keep) {
-                            ratio[q] = __uint_as_float((uint32_t)max((int)(__float_as_uint(now) >> 23) - (int)(__float_as_uint(had) >> 23) + 127, 0) << 23);
-                            changed = true;
-                        }
-                        unit_of[q] = keep ? had : now;
-                        inv[q] = __uint_as_float((254u << 23) - __float_as_uint(unit_of[q]));
-                    }
-                    if (rr == 0) {
-                        *reinterpret_cast<float4 *>(mine + 128 + col) = make_float4(inv[0], inv[1], inv[2], inv[3]);
-                        *reinterpret_cast<float4 *>(mine + RATIO + col) = make_float4(ratio[0], ratio[1], ratio[2], ratio[3]);
-                    }
-                    store(v[1], unit_of, stage + 2 * A_HALF, p.b_half);
+                    store(v[1], stage + 3 * A_IMAGE, p.b_image);
                     fetch(next, b_in, next.n0, p.out, p.b_access, v[1]);
                 }
-                changed = __any_sync(QMLB_FULL_MASK, changed);
-                if (lane == 0) mine[FLAGS + w] = changed ? 1.f : 0.f;
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(full[s]));
-                slot = slot + 1 == slots ? 0 : slot + 1;
                 if (++s == p.stages) { s = 0; phase ^= 1u; }
                 at = next;
-                first = begins;
             }
         }
         if (!ok) failed = 1;
@@ -497,7 +462,7 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
         const int quarter = warp & 3, h = (warp - FOLD_WARP) >> 2, half = p.NT / 2;       // rows and columns of this warp
         unsigned char *mine = epi + (warp - FOLD_WARP) * 2048;
         const uint32_t lane_field = (uint32_t)(quarter * 32) << 16;
-        int it = 0, slot = 0;
+        int it = 0;
         bool ok = true;
         // where a tile goes: rows of y, of dW, or of a part
         auto target = [&](int g, int part, int r0, int r1, int k0, int nt, size_t &row_floats, int &rows, int &width, int &access) {
@@ -537,25 +502,6 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
                 ok = __all_sync(QMLB_FULL_MASK, mbar_wait(bar(acc_full[buf]), (uint32_t)(it / NACC) & 1u, gave_up));
                 if (!ok) break;
                 fence_after();
-                const float *sc = scale + (size_t)slot * SLOT;
-                const float row_scale = sc[quarter * 32 + lane];
-                const float2 rs = make_float2(row_scale, row_scale);
-                bool changed = false;
-                if (GRAD) {
-                    const float4 f = *reinterpret_cast<const float4 *>(sc + FLAGS), e = *reinterpret_cast<const float4 *>(sc + FLAGS + 4);
-                    changed = f.x + f.y + f.z + f.w + e.x + e.y + e.z + e.w != 0.f;
-                }
-                if (GRAD && changed) {              // columns whose unit changes with this chunk
-                    const float *ratio = sc + RATIO + h * half;
-#pragma unroll
-                    for (int cc = 0; cc < HALF; cc += 4) {
-                        if (cc < half) {
-                            const float4 f = *reinterpret_cast<const float4 *>(ratio + cc);
-                            acc[cc / 2] = __fmul2_rn(acc[cc / 2], make_float2(f.x, f.y));
-                            acc[cc / 2 + 1] = __fmul2_rn(acc[cc / 2 + 1], make_float2(f.z, f.w));
-                        }
-                    }
-                }
                 const uint32_t from = tmem + (uint32_t)buf * NT_MAX + lane_field + (uint32_t)(h * half);
                 // 16 columns at a time, the next 16 on their way from tensor memory meanwhile
                 uint32_t t[2][16];
@@ -568,21 +514,18 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
                         const uint32_t(&u)[16] = t[(cc / 16) & 1];
 #pragma unroll
                         for (int q = 0; q < 8; ++q)
-                            acc[cc / 2 + q] = __ffma2_rn(make_float2(__uint_as_float(u[q * 2]), __uint_as_float(u[q * 2 + 1])), rs, acc[cc / 2 + q]);
+                            acc[cc / 2 + q] = __fadd2_rn(make_float2(__uint_as_float(u[q * 2]), __uint_as_float(u[q * 2 + 1])), acc[cc / 2 + q]);
                     }
                 }
                 fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(acc_free[buf]));
-                slot = slot + 1 == slots ? 0 : slot + 1;
             }
             if (!ok) {
                 failed = 1;                                     // at once: the other roles stop waiting
 #pragma unroll
                 for (int i = 0; i < HALF / 2; ++i) acc[i] = make_float2(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
             }
-            // undo the columns' scales (of the last chunk; every chunk carries them)
-            const float *cols = scale + (size_t)(slot == 0 ? slots - 1 : slot - 1) * SLOT + 128 + h * half;
             size_t row_floats;
             int rows, width, access;
             float *to = target(g, part, r0, r1, k0, nt, row_floats, rows, width, access);
@@ -593,8 +536,8 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
                     // 32 rows x 16 columns through shared memory: 64-byte pieces of rows
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        const float4 f = *reinterpret_cast<const float4 *>(cols + cc + q * 4);
-                        const float2 lo = __fmul2_rn(acc[cc / 2 + q * 2], make_float2(f.x, f.y)), hi = __fmul2_rn(acc[cc / 2 + q * 2 + 1], make_float2(f.z, f.w));
+                        const float2 unscale = make_float2(UNSCALE, UNSCALE);
+                        const float2 lo = __fmul2_rn(acc[cc / 2 + q * 2], unscale), hi = __fmul2_rn(acc[cc / 2 + q * 2 + 1], unscale);
                         if (cc + q * 4 < half) {                // (what lies behind is no result of this warp)
                             test = __ffma2_rn(lo, make_float2(0.f, 0.f), test);
                             test = __ffma2_rn(hi, make_float2(0.f, 0.f), test);
@@ -664,13 +607,11 @@ pair_kernel(const float *__restrict__ a_in, const float *__restrict__ b_in, cons
     if (warp == MMA_WARP) tmem_free(tmem, TMEM_COLS);
 }
 
-// Images of the matrices: per group, column tile and stretch of 64 along the depth NT lines of 64 high parts and NT lines of
-// low parts, swizzled as the kernel's shared memory wants them, and NT inverse scales (one per column for the whole depth, so
-// that they are undone once per tile).  One block: 16 columns of one group, read twice (the second time from the cache).
+// Images of the matrices: per group, column tile and stretch of 64 along the depth the parts c, b and a, NT lines of 64 values each,
+// swizzled as the kernel's shared memory wants them.  One block: 16 columns of one group, two stretches at a time.
 template <bool TRANS>
 __global__ void __launch_bounds__(256)
-pack_kernel(const float *__restrict__ W, Shape p, int N, unsigned char *__restrict__ packed, float *__restrict__ pack_scales) {
-    __shared__ float most[16][17];
+pack_kernel(const float *__restrict__ W, Shape p, int N, unsigned char *__restrict__ packed) {
     const int g = blockIdx.y;
     // neighbouring threads read neighbouring addresses: along the columns, or along the depth of the transposed matrix
     const int cl = TRANS ? threadIdx.x >> 4 : threadIdx.x & 15, kl = TRANS ? threadIdx.x & 15 : threadIdx.x >> 4;
@@ -679,52 +620,39 @@ pack_kernel(const float *__restrict__ W, Shape p, int N, unsigned char *__restri
     const int inside = min(col, p.out - 1);              // addresses are clamped instead of tested: the loads are in flight together
     const float *base = TRANS ? Wg + (size_t)inside * N : Wg + inside;
     const size_t step = TRANS ? 1 : (size_t)N;
-    float m = 0.f;
-    for (int k = kl; k < p.K; k += 16 * 16) {
-        float t[16];
-#pragma unroll
-        for (int u = 0; u < 16; ++u) t[u] = base[(size_t)min(k + u * 16, p.K - 1) * step];
-#pragma unroll
-        for (int u = 0; u < 16; ++u) m = fmaxf(m, fabsf(t[u]));
-    }
-    most[cl][kl] = m;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) m = fmaxf(m, most[cl][i]);
-    float s, inv;
-    scales(m, 268, s, inv);
     const int tile = col / p.NT, in = col - tile * p.NT;               // the grid covers whole tiles
     const size_t image = (size_t)(g * p.ntiles + tile) * p.nchunks;
 #pragma unroll 2
-    for (int c0 = 0; c0 < p.nchunks; c0 += 2) {                        // two stretches: 16 threads of 8 values per column
+    for (int c0 = (int)blockIdx.z * 2; c0 < p.nchunks; c0 += (int)gridDim.z * 2) {      // 16 threads of 8 values per column
         const int c = c0 + (kl >> 3), k0 = c0 * BK + kl * 8;
         if (c >= p.nchunks) continue;
         float t[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) t[i] = base[(size_t)min(k0 + i, p.K - 1) * step];
-        float2 v[4];
+        uint32_t v[3][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            v[i].x = col < p.out && k0 + i * 2 < p.K ? t[i * 2] : 0.f;
-            v[i].y = col < p.out && k0 + i * 2 + 1 < p.K ? t[i * 2 + 1] : 0.f;
+            const float2 x = make_float2(col < p.out && k0 + i * 2 < p.K ? t[i * 2] : 0.f, col < p.out && k0 + i * 2 + 1 < p.K ? t[i * 2 + 1] : 0.f);
+            uint32_t u[3];
+            split2(x, u);
+            v[0][i] = u[0];
+            v[1][i] = u[1];
+            v[2][i] = u[2];
         }
-        uint32_t hi[4], lo[4];
+        unsigned char *line = packed + (image + c) * (3 * p.b_image) + (size_t)in * 128 + (((kl & 7) ^ (in & 7)) << 4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) split2(v[i], make_float2(s, s), hi[i], lo[i]);
-        unsigned char *line = packed + (image + c) * (2 * p.b_half) + (size_t)in * 128 + (((kl & 7) ^ (in & 7)) << 4);
-        *reinterpret_cast<uint4 *>(line) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4 *>(line + p.b_half) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        if ((kl & 7) == 0) pack_scales[(image + c) * p.NT + in] = inv;
+        for (int e = 0; e < 3; ++e) *reinterpret_cast<uint4 *>(line + (size_t)(2 - e) * p.b_image) = make_uint4(v[e][0], v[e][1], v[e][2], v[e][3]);
     }
 }
 
 template <bool GRAD>
 size_t smem_of(const Shape &p) {
-    using C = Config<GRAD>;
-    return (size_t)p.stages * (2 * A_HALF + 2 * p.b_half) + (size_t)(p.stages + C::ACCS + 1) * C::SLOT * 4 + EPI + (size_t)(GRAD ? 3 : 2) * (p.G + 1) * 4 + 1024;
+    const size_t operands = GRAD ? (size_t)p.stages * 3 * (A_IMAGE + p.b_image) : (size_t)p.stages * 3 * A_IMAGE + (size_t)p.slots * p.b_image;
+    return operands + EPI + (size_t)(GRAD ? 3 : 2) * (p.G + 1) * 4 + 1024;
 }
 
-// Columns per tile and stages.  Many groups leave less shared memory for the stages: then the tiles get narrower.
+// Columns per tile and stages.  Many groups leave less shared memory for the stages: then the tiles get narrower.  Products of rows:
+// three slots let a part of the matrix arrive while the products of the two others run; a third stage of the rows comes before more.
 template <bool GRAD>
 void tile_columns(Shape &p, int out) {
     const size_t limit = SMEM_LIMIT - 512;
@@ -732,10 +660,16 @@ void tile_columns(Shape &p, int out) {
         const int nt = (out + widest - 1) / widest;
         p.NT = ((out + nt - 1) / nt + 15) / 16 * 16;
         p.ntiles = (out + p.NT - 1) / p.NT;
-        p.b_half = GRAD ? (uint32_t)((p.NT + 63) / 64) * 8192u : (uint32_t)p.NT * 128u;
-        p.stages = MAXST;
+        p.b_image = GRAD ? (uint32_t)((p.NT + 63) / 64) * 8192u : (uint32_t)p.NT * 128u;
+        p.slots = GRAD ? 0 : 3;
+        p.stages = GRAD ? MAXST : 3;
         while (p.stages > 2 && smem_of<GRAD>(p) > limit) --p.stages;
-        if (smem_of<GRAD>(p) <= limit || widest == 64) return;
+        const bool fits = smem_of<GRAD>(p) <= limit;
+        while (!GRAD && fits && p.slots < MAXSLOT) {
+            ++p.slots;
+            if (smem_of<GRAD>(p) > limit) { --p.slots; break; }
+        }
+        if (fits || widest == 64) return;
     }
 }
 
@@ -758,7 +692,7 @@ namespace qmlb {
 size_t grouped_pair_workspace(size_t n, int G, int K, int N, int transpose) {
     const Shape p = product_shape(n, G, K, N, transpose);
     const size_t images = (size_t)G * p.ntiles * p.nchunks;
-    return images * (2 * p.b_half + (size_t)p.NT * 4) + 256;
+    return images * (3 * p.b_image) + 256;
 }
 
 int grouped_pair(const float *x, const float *W, const int *start, size_t n, int G, int K, int N, int transpose, float *out, void *workspace,
@@ -769,15 +703,14 @@ int grouped_pair(const float *x, const float *W, const int *start, size_t n, int
     p.w_depth = transpose ? 1 : (size_t)N;
     p.w_col = transpose ? (size_t)N : 1;
     unsigned char *packed = static_cast<unsigned char *>(workspace);
-    const size_t images = (size_t)G * p.ntiles * p.nchunks;
-    float *pack_scales = reinterpret_cast<float *>(packed + images * (2 * p.b_half));
-    const dim3 pg((unsigned)(p.ntiles * p.NT / 16), (unsigned)G);
-    if (transpose) pack_kernel<true><<<pg, 256, 0, st>>>(W, p, N, packed, pack_scales);
-    else pack_kernel<false><<<pg, 256, 0, st>>>(W, p, N, packed, pack_scales);
+    const unsigned pairs = (unsigned)(p.nchunks + 1) / 2;
+    const dim3 pg((unsigned)(p.ntiles * p.NT / 16), (unsigned)G, pairs < 64 ? pairs : 64);
+    if (transpose) pack_kernel<true><<<pg, 256, 0, st>>>(W, p, N, packed);
+    else pack_kernel<false><<<pg, 256, 0, st>>>(W, p, N, packed);
     const long units = ((long)((n + BM - 1) / BM) + G) * p.ntiles;
     const size_t smem = smem_of<false>(p);
     if (int rc = ensure_smem(pair_kernel<false>, smem, "qmlb_grouped_matmul")) return rc;
-    pair_kernel<false><<<(unsigned)(units < 148 ? units : 148), Config<false>::THREADS, smem, st>>>(x, W, packed, pack_scales, start, p, out, nullptr);
+    pair_kernel<false><<<(unsigned)(units < 148 ? units : 148), Config<false>::THREADS, smem, st>>>(x, W, packed, start, p, out, nullptr);
     return check_launch("qmlb_grouped_matmul");
 }
 
@@ -799,7 +732,7 @@ int grouped_wgrad_pair(const float *x, const float *dy, const int *start, size_t
     const size_t smem = smem_of<true>(p);
     float *partial = static_cast<float *>(workspace);
     if (int rc = ensure_smem(pair_kernel<true>, smem, "qmlb_grouped_matmul_wgrad")) return rc;
-    pair_kernel<true><<<(unsigned)(units < 148 ? units : 148), Config<true>::THREADS, smem, st>>>(x, dy, nullptr, nullptr, start, p, dW, partial);
+    pair_kernel<true><<<(unsigned)(units < 148 ? units : 148), Config<true>::THREADS, smem, st>>>(x, dy, nullptr, start, p, dW, partial);
     return wgrad_join(dW, QMLB_F32, start, n, G, K, N, p.split, p.ntiles * p.NT, partial, st);
 }
 
