@@ -9,7 +9,8 @@
 // whole FCHL19 -> PCA -> SORF -> energy chain with the coordinate gradient computed in the same pass (and its RFF
 // twin qml_lightning_b200::rff_energy for RandomFourrierFeaturesModel.forward).
 // qml_lightning_b200::{group_by_key, embedding, embedding_grad, grouped_matmul, grouped_matmul_wgrad} work on rows that
-// belong to groups (elements, species, tokens); all but the first are differentiable, any number of times.
+// belong to groups (elements, species, tokens); all but the first are differentiable, any number of times, in reverse and in
+// forward mode.
 //
 // This file contains no device code: it only allocates tensors, picks the current stream and device, and forwards
 // raw pointers to libqmlb200.so.  Unlike upstream it honours the current CUDA stream and device of the inputs.
@@ -435,6 +436,36 @@ void on_device(const Tensor &t, const torch::Device &dev, const char *name) {
 bool differentiable(const Tensor &a) { return at::GradMode::is_enabled() && a.requires_grad(); }
 bool differentiable(const Tensor &a, const Tensor &b) { return at::GradMode::is_enabled() && (a.requires_grad() || b.requires_grad()); }
 
+// Forward mode.  Every one of these maps is linear in each of its tensors, so a tangent is a call of the same operator.  Primal value
+// and tangent (undefined if there is none) of an argument, and a result of both:
+std::tuple<Tensor, Tensor> primal_and_tangent(const Tensor &t) {
+    if (!t._fw_grad(0).defined()) return {t, Tensor()};
+    return at::_unpack_dual(t, 0);
+}
+bool has_tangent(const Tensor &a) { return a._fw_grad(0).defined(); }
+bool has_tangent(const Tensor &a, const Tensor &b) { return has_tangent(a) || has_tangent(b); }
+Tensor dual(const Tensor &primal, const Tensor &tangent) { return at::_make_dual(primal, tangent, 0); }
+
+// What a backward pass saves of two arguments: the tensors with their tangents, where the function itself was called with the primal
+// values, so that forward mode passes through a backward pass.
+struct Kept {
+    Tensor a, b;
+};
+
+// f(a, b, kept) of two dual tensors, f linear in both
+template <typename F>
+Tensor bilinear_dual(const Tensor &a, const Tensor &b, F f) {
+    Tensor pa, ta, pb, tb, tangent;
+    std::tie(pa, ta) = primal_and_tangent(a);
+    std::tie(pb, tb) = primal_and_tangent(b);
+    if (ta.defined()) tangent = f(ta, pb, Kept{ta, pb});
+    if (tb.defined()) {
+        const Tensor t = f(pa, tb, Kept{pa, tb});
+        tangent = tangent.defined() ? tangent + t : t;
+    }
+    return dual(f(pa, pb, Kept{a, b}), tangent);
+}
+
 // Uninitialised tensor on the device of `like`, without a pass through the dispatcher: the smallest calls of these operators are
 // bound by the host.
 Tensor new_tensor(at::IntArrayRef sizes, const Tensor &like, at::ScalarType type) {
@@ -542,10 +573,20 @@ class EmbeddingGradFn : public torch::autograd::Function<EmbeddingGradFn> {
 };
 
 Tensor embedding(const Tensor &indices, const Tensor &table, double scale) {
+    if (has_tangent(table)) {
+        Tensor p, t;
+        std::tie(p, t) = primal_and_tangent(table);
+        return dual(embedding(indices, p, scale), embedding(indices, t, scale));
+    }
     return differentiable(table) ? EmbeddingFn::apply(indices, table, scale)[0] : embedding_call(indices, table, scale);
 }
 
 Tensor embedding_grad(const Tensor &grad, const Tensor &indices, const Tensor &order, const Tensor &group_start, int64_t rows, double scale) {
+    if (has_tangent(grad)) {
+        Tensor p, t;
+        std::tie(p, t) = primal_and_tangent(grad);
+        return dual(embedding_grad(p, indices, order, group_start, rows, scale), embedding_grad(t, indices, order, group_start, rows, scale));
+    }
     return differentiable(grad) ? EmbeddingGradFn::apply(grad, indices, order, group_start, rows, scale)[0]
                                 : embedding_grad_call(grad, indices, order, group_start, rows, scale);
 }
@@ -609,8 +650,8 @@ Tensor grouped_matmul_wgrad_call(const Tensor &x, const Tensor &dy, const Tensor
 // another's derivatives, so every backward calls the differentiable operators again.
 class GroupedMatmulFn : public torch::autograd::Function<GroupedMatmulFn> {
    public:
-    static variable_list forward(AutogradContext *ctx, Tensor x, Tensor W, Tensor group_start, bool transpose) {
-        ctx->save_for_backward({x, W, group_start});
+    static variable_list forward(AutogradContext *ctx, Tensor x, Tensor W, Tensor group_start, bool transpose, Kept kept) {
+        ctx->save_for_backward({kept.a, kept.b, group_start});
         ctx->saved_data["transpose"] = transpose;
         return {grouped_matmul_call(x, W, group_start, transpose)};
     }
@@ -620,14 +661,14 @@ class GroupedMatmulFn : public torch::autograd::Function<GroupedMatmulFn> {
         Tensor g = grad_output[0], dx, dW, u;
         if (ctx->needs_input_grad(0)) dx = grouped_matmul_any(g, s[1], s[2], !transpose);
         if (ctx->needs_input_grad(1)) dW = transpose ? grouped_matmul_wgrad(g, s[0], s[2]) : grouped_matmul_wgrad(s[0], g, s[2]);
-        return {dx, dW, u, u};
+        return {dx, dW, u, u, u};
     }
 };
 
 class GroupedWgradFn : public torch::autograd::Function<GroupedWgradFn> {
    public:
-    static variable_list forward(AutogradContext *ctx, Tensor x, Tensor dy, Tensor group_start) {
-        ctx->save_for_backward({x, dy, group_start});
+    static variable_list forward(AutogradContext *ctx, Tensor x, Tensor dy, Tensor group_start, Kept kept) {
+        ctx->save_for_backward({kept.a, kept.b, group_start});
         return {grouped_matmul_wgrad_call(x, dy, group_start)};
     }
     static variable_list backward(AutogradContext *ctx, variable_list grad_output) {
@@ -635,12 +676,15 @@ class GroupedWgradFn : public torch::autograd::Function<GroupedWgradFn> {
         Tensor dx, ddy, u;
         if (ctx->needs_input_grad(0)) dx = grouped_matmul_any(s[1], grad_output[0], s[2], true);
         if (ctx->needs_input_grad(1)) ddy = grouped_matmul_any(s[0], grad_output[0], s[2], false);
-        return {dx, ddy, u};
+        return {dx, ddy, u, u};
     }
 };
 
 Tensor grouped_matmul_any(const Tensor &x, const Tensor &W, const Tensor &group_start, bool transpose) {
-    return differentiable(x, W) ? GroupedMatmulFn::apply(x, W, group_start, transpose)[0] : grouped_matmul_call(x, W, group_start, transpose);
+    auto call = [&](const Tensor &a, const Tensor &b, const Kept &kept) {
+        return differentiable(a, b) ? GroupedMatmulFn::apply(a, b, group_start, transpose, kept)[0] : grouped_matmul_call(a, b, group_start, transpose);
+    };
+    return has_tangent(x, W) ? bilinear_dual(x, W, call) : call(x, W, Kept{x, W});
 }
 
 Tensor grouped_matmul(const Tensor &x, const Tensor &W, const Tensor &group_start, bool transpose) {
@@ -648,7 +692,10 @@ Tensor grouped_matmul(const Tensor &x, const Tensor &W, const Tensor &group_star
 }
 
 Tensor grouped_matmul_wgrad(const Tensor &x, const Tensor &dy, const Tensor &group_start) {
-    return differentiable(x, dy) ? GroupedWgradFn::apply(x, dy, group_start)[0] : grouped_matmul_wgrad_call(x, dy, group_start);
+    auto call = [&](const Tensor &a, const Tensor &b, const Kept &kept) {
+        return differentiable(a, b) ? GroupedWgradFn::apply(a, b, group_start, kept)[0] : grouped_matmul_wgrad_call(a, b, group_start);
+    };
+    return has_tangent(x, dy) ? bilinear_dual(x, dy, call) : call(x, dy, Kept{x, dy});
 }
 
 }  // namespace
