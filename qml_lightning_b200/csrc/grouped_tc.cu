@@ -16,6 +16,9 @@
 // its first row), and the issuing warp overwrites what the rows bring there.  (780 deep, 330,001 rows: 231 us with cp.async of
 // 8 bytes, 177 us so; 781 deep: 664 us with 2-byte loads, 181 us so.)  Transposed, the matrix's lines would have to move along, so
 // warps 12-19 bring the rows with cp.async of 8 or 4 bytes, or 2-byte loads, into the same swizzled stages.
+// Sums longer than 16,384 values are cut, because the tensor core truncates when it adds (1,024 additions of one sign are off by up to
+// 1e-4 of their sum): every piece fills an accumulator of its own, and the draining warps add them in 32 bits in a place of the
+// workspace that only they use.
 // Every wait is bounded; a block that gives up fills its remaining tiles with NaN and counts the event (qmlb_tc_timeouts).
 #include "grouped_tc.cuh"
 #include "grouped_rows.cuh"
@@ -35,6 +38,9 @@ constexpr uint32_t A_BYTES = BM * BK * 2;
 // 116; but 256 deep, 784 columns (330,000 rows): 193 -> 238, and 336 deep, 256 columns (210,000 rows): 62 -> 70.
 constexpr int PAIR_DEPTH = 768;
 constexpr size_t PAIR_ROWS = 512;                // rows per group, on average
+constexpr int PIECE = 256;                       // chunks of 64 values that one accumulator sums up
+constexpr int SUMS = BM * 256;                   // 32-bit sums of one block
+constexpr int MAX_BLOCKS = 148;
 constexpr int TMA_WARP = 0, MMA_WARP = 1, EPI_WARP = 4, LOAD_WARP = EPI_WARP + EPI_WARPS, LOAD_WARPS = 8;
 constexpr int NTHREADS = LOAD_WARP * 32, NTHREADS_LOADED = NTHREADS + LOAD_WARPS * 32;
 
@@ -49,11 +55,13 @@ struct Shape {
     int out_access;
     int period;              // rows that lie at the same offset from a 16-byte boundary: every period-th
     int shift[8];            // that offset, in elements
+    float *sums;             // [blocks][SUMS], where a sum has several pieces
 };
 
 struct RowMaps { CUtensorMap map[8]; };          // one per offset
 
-template <typename T, bool TRANS, bool LOADED, bool PAIR, bool SHIFTED>
+// DEEP: sums of several pieces, a variant of its own (210,000 rows of 256, transposed to 336 bf16: 67 us, by this variant 72 us)
+template <typename T, bool TRANS, bool LOADED, bool PAIR, bool SHIFTED, bool DEEP>
 __global__ void __launch_bounds__(LOADED ? NTHREADS_LOADED : NTHREADS, 1)
 grouped_kernel(const __grid_constant__ RowMaps maps, const __grid_constant__ CUtensorMap map_w, const T *__restrict__ in,
                const int *__restrict__ start, Shape p, T *__restrict__ out) {
@@ -157,8 +165,7 @@ grouped_kernel(const __grid_constant__ RowMaps maps, const __grid_constant__ CUt
         const uint32_t idesc = instr_desc(std::is_same<T, __nv_bfloat16>::value, false, !TRANS, TILE_ROWS, p.NT);
         int it = 0, j = 0;
         bool ok = true;
-        for (int tile = unit0; tile < total && ok; tile += units, ++j) {
-            const int buf = j & 1;
+        for (int tile = unit0; tile < total && ok; tile += units) {
             int chunks = p.nchunks, shift = 0;
             if (SHIFTED) {
                 int g, row0, row1, col0;
@@ -166,37 +173,40 @@ grouped_kernel(const __grid_constant__ RowMaps maps, const __grid_constant__ CUt
                 chunks = chunks_of(row0);
                 shift = shift_of(row0);
             }
-            bool w = mbar_wait(bar(acc_free[buf]), ((uint32_t)(j >> 1) & 1u) ^ 1u, gave_up);
-            for (int c = 0; c < chunks; ++c, ++it) {
-                const int s = it % p.stages;
-                w = w && mbar_wait(bar(full[s]), (uint32_t)(it / p.stages) & 1u, gave_up, it ? WAIT_LIMIT : QMLB_TEST_FIRST_WAIT_POLLS);
-                if (!__all_sync(QMLB_FULL_MASK, w)) { ok = false; break; }
-                if (SHIFTED && c == 0 && shift) {                   // what lies in front of the rows is not theirs
-                    unsigned char *rows = sp + (size_t)s * stage_bytes;
-                    for (int r = lane; r < BM; r += 32)
-                        for (int i = 0; i < shift; ++i) *reinterpret_cast<uint16_t *>(rows + r * 128 + ((r & 7) << 4) + i * 2) = 0;
-                    fence_async_smem();
+            for (int first = 0; first < chunks && ok; first += DEEP ? PIECE : chunks, ++j) {
+                const int buf = j & 1, end = DEEP ? min(first + PIECE, chunks) : chunks;
+                bool w = mbar_wait(bar(acc_free[buf]), ((uint32_t)(j >> 1) & 1u) ^ 1u, gave_up);
+                for (int c = first; c < end; ++c, ++it) {
+                    const int s = it % p.stages;
+                    w = w && mbar_wait(bar(full[s]), (uint32_t)(it / p.stages) & 1u, gave_up, it ? WAIT_LIMIT : QMLB_TEST_FIRST_WAIT_POLLS);
+                    if (!__all_sync(QMLB_FULL_MASK, w)) { ok = false; break; }
+                    if (SHIFTED && c == 0 && shift) {               // what lies in front of the rows is not theirs
+                        unsigned char *rows = sp + (size_t)s * stage_bytes;
+                        for (int r = lane; r < BM; r += 32)
+                            for (int i = 0; i < shift; ++i) *reinterpret_cast<uint16_t *>(rows + r * 128 + ((r & 7) << 4) + i * 2) = 0;
+                        fence_async_smem();
+                        __syncwarp();
+                    }
+                    if (LOADED) fence_async_smem();                 // copies and stores of the loading threads, as seen through the barrier
+                    fence_after();
+                    const uint32_t a = sbase + (uint32_t)s * stage_bytes, d = tmem + (uint32_t)buf * BUF_COLS;
+                    const uint32_t al = desc_lo(a, 16), bl = desc_lo(a + A_BYTES, TRANS ? 16 : 8192);
+                    constexpr uint32_t b_step = TRANS ? 2u : 128u;          // 16 deep: 32 bytes along the lines, or 16 lines
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < BK / 16; ++k) {
+                            if (PAIR) mma_f16_pair(d, al + k * 2u, DESC_HI_SW128, bl + k * b_step, DESC_HI_SW128, idesc, (c > first || k) ? 1u : 0u);
+                            else mma_f16(d, al + k * 2u, DESC_HI_SW128, bl + k * b_step, DESC_HI_SW128, idesc, (c > first || k) ? 1u : 0u);
+                        }
+                        if (PAIR) mma_commit_pair(bar(empty[s]));
+                        else mma_commit(bar(empty[s]));
+                        if (c == end - 1) {
+                            if (PAIR) mma_commit_pair(bar(acc_full[buf]));
+                            else mma_commit(bar(acc_full[buf]));
+                        }
+                    }
                     __syncwarp();
                 }
-                if (LOADED) fence_async_smem();                     // copies and stores of the loading threads, as seen through the barrier
-                fence_after();
-                const uint32_t a = sbase + (uint32_t)s * stage_bytes, d = tmem + (uint32_t)buf * BUF_COLS;
-                const uint32_t al = desc_lo(a, 16), bl = desc_lo(a + A_BYTES, TRANS ? 16 : 8192);
-                constexpr uint32_t b_step = TRANS ? 2u : 128u;              // 16 deep: 32 bytes along the lines, or 16 lines
-                if (elect_one()) {
-#pragma unroll
-                    for (int k = 0; k < BK / 16; ++k) {
-                        if (PAIR) mma_f16_pair(d, al + k * 2u, DESC_HI_SW128, bl + k * b_step, DESC_HI_SW128, idesc, (c | k) ? 1u : 0u);
-                        else mma_f16(d, al + k * 2u, DESC_HI_SW128, bl + k * b_step, DESC_HI_SW128, idesc, (c | k) ? 1u : 0u);
-                    }
-                    if (PAIR) mma_commit_pair(bar(empty[s]));
-                    else mma_commit(bar(empty[s]));
-                    if (c == chunks - 1) {
-                        if (PAIR) mma_commit_pair(bar(acc_full[buf]));
-                        else mma_commit(bar(acc_full[buf]));
-                    }
-                }
-                __syncwarp();
             }
         }
         if (!ok) failed = 1;
@@ -223,46 +233,63 @@ grouped_kernel(const __grid_constant__ RowMaps maps, const __grid_constant__ CUt
             if (PAIR) mbar_arrive_cluster(map_rank(bar(acc_free[buf]), 0));
             else mbar_arrive(bar(acc_free[buf]));
         };
+        // this thread's sums of a column group: [32 columns][32 lanes] per warp and group
+        float *kept = p.sums + (size_t)blockIdx.x * SUMS + (size_t)(warp - EPI_WARP) * (SUMS / EPI_WARPS) + lane;
         int j = 0;
         bool ok = true;
-        for (int tile = unit0; tile < total; tile += units, ++j) {
-            const int buf = j & 1;
+        for (int tile = unit0; tile < total; tile += units) {
             int g, row0, row1, col0;
             locate(tile, g, row0, row1, col0);
             const int row = row0 + quarter * 32 * period;
             const int rows = min(32, (row1 - row + period - 1) / period);
-            ok = ok && mbar_wait(bar(acc_full[buf]), (uint32_t)(j >> 1) & 1u, gave_up);
-            ok = __all_sync(QMLB_FULL_MASK, ok);
-            if (!ok) failed = 1;                                // at once: the other roles stop waiting
-            fence_after();
-            const uint32_t from = tmem + (uint32_t)buf * BUF_COLS + ((uint32_t)(quarter * 32) << 16);
-            if (ok && c_first >= p.NT) {
-                __syncwarp();
-                if (lane == 0) release(buf);
-            }
-            for (int c = c_first; c < p.NT; c += 64) {
-                uint32_t v[32];
-                const int left = p.NT - c;
-                if (ok) {
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                        if (u * 16 < left) tmem_ld16(from + (uint32_t)(c + u * 16), v + u * 16);
-                    tmem_ld_wait();
-                    if (c + 64 >= p.NT) {                       // the accumulator is free once it sits in registers
-                        fence_before();
-                        __syncwarp();
-                        if (lane == 0) release(buf);
-                    }
-                } else {
-#pragma unroll
-                    for (int u = 0; u < 32; ++u) v[u] = 0x7fc00000u;
+            const int pieces = DEEP ? (chunks_of(row0) + PIECE - 1) / PIECE : 1;
+            for (int piece = 0; piece < pieces; ++piece, ++j) {
+                const int buf = j & 1;
+                ok = ok && mbar_wait(bar(acc_full[buf]), (uint32_t)(j >> 1) & 1u, gave_up);
+                ok = __all_sync(QMLB_FULL_MASK, ok);
+                if (!ok) failed = 1;                            // at once: the other roles stop waiting
+                fence_after();
+                const uint32_t from = tmem + (uint32_t)buf * BUF_COLS + ((uint32_t)(quarter * 32) << 16);
+                if (ok && c_first >= p.NT) {
+                    __syncwarp();
+                    if (lane == 0) release(buf);
                 }
-                stage_row<T>(mine, lane, v);
-                __syncwarp();
-                const int bytes = min(min(32, left), p.out - col0 - c) * 2;
-                unsigned char *to = reinterpret_cast<unsigned char *>(out) + (size_t)row * row_bytes + (size_t)(col0 + c) * 2;
-                store_tile(mine, to, row_step, rows, bytes, lane, p.out_access);
-                __syncwarp();
+                for (int c = c_first; c < p.NT; c += 64) {
+                    uint32_t v[32];
+                    const int left = p.NT - c;
+                    if (ok) {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            if (u * 16 < left) tmem_ld16(from + (uint32_t)(c + u * 16), v + u * 16);
+                        tmem_ld_wait();
+                        if (c + 64 >= p.NT) {                   // the accumulator is free once it sits in registers
+                            fence_before();
+                            __syncwarp();
+                            if (lane == 0) release(buf);
+                        }
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 32; ++u) v[u] = 0x7fc00000u;
+                    }
+                    if (DEEP && pieces > 1) {
+                        float *sum = kept + (size_t)(c >> 6) * 1024;
+                        if (piece > 0) {
+#pragma unroll
+                            for (int u = 0; u < 32; ++u) v[u] = __float_as_uint(__uint_as_float(v[u]) + sum[u * 32]);
+                        }
+                        if (piece < pieces - 1) {
+#pragma unroll
+                            for (int u = 0; u < 32; ++u) sum[u * 32] = __uint_as_float(v[u]);
+                            continue;
+                        }
+                    }
+                    stage_row<T>(mine, lane, v);
+                    __syncwarp();
+                    const int bytes = min(min(32, left), p.out - col0 - c) * 2;
+                    unsigned char *to = reinterpret_cast<unsigned char *>(out) + (size_t)row * row_bytes + (size_t)(col0 + c) * 2;
+                    store_tile(mine, to, row_step, rows, bytes, lane, p.out_access);
+                    __syncwarp();
+                }
             }
         }
     } else if (LOADED) {
@@ -315,12 +342,16 @@ pad_kernel(const T *__restrict__ W, size_t rows, int N, int Np, T *__restrict__ 
     }
 }
 
+// a sum may begin up to seven values early
+bool several_pieces(int depth) { return (depth + 7 + BK - 1) / BK > PIECE; }
+size_t padded_bytes(int G, int K, int N) { return ((size_t)G * K * ((N + 7) & ~7) * 2 + 255) & ~(size_t)255; }
+
 bool needs_pad(const void *W, int N) { return ((uintptr_t)W & 15) != 0 || (N & 7) != 0; }
 
-template <typename T, bool TRANS, bool LOADED, bool PAIR, bool SHIFTED>
-int launch(const RowMaps &mi, const CUtensorMap &mw, const T *in, const int *start, const Shape &p, int blocks, T *out, cudaStream_t st) {
+template <typename T, bool TRANS, bool LOADED, bool PAIR, bool SHIFTED, bool DEEP>
+int launch_as(const RowMaps &mi, const CUtensorMap &mw, const T *in, const int *start, const Shape &p, int blocks, T *out, cudaStream_t st) {
     const size_t smem = (size_t)p.stages * (A_BYTES + p.b_bytes) + EPI_BYTES + (size_t)2 * (p.G + 1) * 4 + 1024;
-    auto kernel = grouped_kernel<T, TRANS, LOADED, PAIR, SHIFTED>;
+    auto kernel = grouped_kernel<T, TRANS, LOADED, PAIR, SHIFTED, DEEP>;
     if (int rc = qmlb::ensure_smem(kernel, smem, "qmlb_grouped_matmul")) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)blocks);
@@ -339,6 +370,12 @@ int launch(const RowMaps &mi, const CUtensorMap &mw, const T *in, const int *sta
         return QMLB_ERR_CUDA;
     }
     return qmlb::check_launch("qmlb_grouped_matmul");
+}
+
+template <typename T, bool TRANS, bool LOADED, bool PAIR, bool SHIFTED>
+int launch(const RowMaps &mi, const CUtensorMap &mw, const T *in, const int *start, const Shape &p, int blocks, T *out, cudaStream_t st) {
+    return several_pieces(p.K) ? launch_as<T, TRANS, LOADED, PAIR, SHIFTED, true>(mi, mw, in, start, p, blocks, out, st)
+                               : launch_as<T, TRANS, LOADED, PAIR, SHIFTED, false>(mi, mw, in, start, p, blocks, out, st);
 }
 
 template <typename T>
@@ -385,6 +422,7 @@ int run(const void *x, const void *W, const int *start, size_t n, int G, int K, 
     if (int rc = qmlb::encode_tiles(&mw, Wp, bf16, (uint64_t)N, (uint64_t)K, (uint64_t)G, (uint64_t)Np * 2, transpose ? (uint32_t)own : 64u,
                                     "qmlb_grouped_matmul"))
         return rc;
+    p.sums = reinterpret_cast<float *>(static_cast<unsigned char *>(workspace) + padded_bytes(G, K, N));
     const uint64_t row_bytes = (uint64_t)p.K * 2;
     p.period = 1;
     if (shifted) {
@@ -405,7 +443,7 @@ int run(const void *x, const void *W, const int *start, size_t n, int G, int K, 
     }
     const long rows_per_tile = (long)BM * blocks_per_tile * p.period;
     const long tiles = ((long)((n + rows_per_tile - 1) / rows_per_tile) + G) * p.period * p.ntiles * blocks_per_tile;
-    const int blocks = (int)(tiles < 148 ? tiles : 148);
+    const int blocks = (int)(tiles < MAX_BLOCKS ? tiles : MAX_BLOCKS);
     const T *xi = static_cast<const T *>(x);
     T *o = static_cast<T *>(out);
     if (loaded) return launch<T, true, true, false, false>(mi, mw, xi, start, p, blocks, o, st);
@@ -421,7 +459,9 @@ int run(const void *x, const void *W, const int *start, size_t n, int G, int K, 
 
 namespace qmlb {
 
-size_t grouped_tc_workspace(int G, int K, int N) { return (size_t)G * K * ((N + 7) & ~7) * 2 + 256; }
+size_t grouped_tc_workspace(int G, int K, int N, int transpose) {
+    return padded_bytes(G, K, N) + (several_pieces(transpose ? N : K) ? (size_t)MAX_BLOCKS * SUMS * 4 : 0) + 256;
+}
 
 int grouped_tc(const void *x, const void *W, const int *start, int dtype, size_t n, int G, int K, int N, int transpose, void *out,
                void *workspace, cudaStream_t st) {
