@@ -54,10 +54,26 @@ __device__ __forceinline__ unsigned same_digit(uint32_t d, int nbits, bool in) {
     return m;
 }
 
+// Long runs of keys that do not occur have one start, which the warp that finds the run stores 512 bytes at a time (at most 20 us).
+// From FAR_KEYS keys on it leaves the whole segments of SEGMENT keys in the run to gap_kernel, a launch of 4 to 6 us.  (All keys equal:
+// 131,072 keys of 300,000: 451 -> 69 us, 300,000 of 2,000,000: 2,830 -> 57 us, against 32 starts at a time.)
+constexpr uint32_t SEGMENT = 4096, FAR_KEYS = 524288, LONG_RUN = 256;
+
+// group_start[from .. end - 1] = value, by a warp, 16 bytes per lane
+__device__ __forceinline__ void fill_run(int *__restrict__ group_start, uint32_t from, uint32_t end, int value) {
+    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t head = min(end, from + (uint32_t)(((16 - ((uintptr_t)(group_start + from) & 15)) & 15) / 4));
+    if (from + lane < head) group_start[from + lane] = value;
+    const uint32_t words = (end - head) / 4;
+    int4 *to4 = reinterpret_cast<int4 *>(group_start + head);
+    for (uint32_t i = lane; i < words; i += 32) to4[i] = make_int4(value, value, value, value);
+    if (head + words * 4 + lane < end) group_start[head + words * 4 + lane] = value;
+}
+
 // group_start[v] = first position whose sorted key is not below v, for the v that the 32 positions p0 .. p0 + 31 answer: those
 // above the key in front of them and not above their last one (positions behind the end count as the key nkeys).  `key`: the key
 // of position p0 + lane, `front`: the key of position p0 - 1, or -1.  All lanes of the warp take part; writes are whole lines.
-__device__ __forceinline__ void write_starts(uint32_t key, int64_t front, uint32_t p0, int *__restrict__ group_start) {
+__device__ __forceinline__ void write_starts(uint32_t key, int64_t front, uint32_t p0, uint32_t nkeys, int *__restrict__ group_start) {
     const uint32_t last = __shfl_sync(QMLB_FULL_MASK, key, 31);
     for (int64_t v0 = front + 1; v0 <= (int64_t)last; v0 += 32) {
         const uint32_t v = (uint32_t)v0 + (threadIdx.x & 31);
@@ -65,8 +81,35 @@ __device__ __forceinline__ void write_starts(uint32_t key, int64_t front, uint32
 #pragma unroll
         for (int step = 16; step; step >>= 1)
             if (__shfl_sync(QMLB_FULL_MASK, key, below + step - 1) < v) below += step;
+        const int first = __shfl_sync(QMLB_FULL_MASK, below, 0);
+        const uint32_t end = __shfl_sync(QMLB_FULL_MASK, key, first);          // of the run of absent keys that v0 lies in
+        if (end - (uint32_t)v0 >= LONG_RUN) {
+            uint32_t from = (uint32_t)v0, to = end + 1;
+            const uint32_t a = (from + SEGMENT - 1) / SEGMENT * SEGMENT, b = to / SEGMENT * SEGMENT;
+            const bool parts = nkeys >= FAR_KEYS && a < b;       // [from, a) and [b, to)
+            if (parts) to = a;
+#pragma unroll 1
+            for (int i = 0; i < (parts ? 2 : 1); ++i, from = b, to = end + 1)
+                if (from < to) fill_run(group_start, from, to, (int)(p0 + first));
+            v0 = (int64_t)end + 1 - 32;
+            continue;
+        }
         if (v <= last) group_start[v] = (int)(p0 + below);
     }
+}
+
+// first position whose sorted key is not below v, by a warp: 32 probes at a time
+__device__ __forceinline__ uint32_t warp_lower_bound(const uint32_t *__restrict__ sorted, uint32_t n, uint32_t v) {
+    uint32_t lo = 0, hi = n;
+    while (lo < hi) {
+        const uint32_t lane = threadIdx.x & 31, at = lo + (uint32_t)(((uint64_t)(hi - lo) * lane) >> 5);
+        const int below = __popc(__ballot_sync(QMLB_FULL_MASK, sorted[at] < v));
+        if (below == 0) break;
+        const uint32_t next = __shfl_sync(QMLB_FULL_MASK, at, below & 31);
+        lo = __shfl_sync(QMLB_FULL_MASK, at, below - 1) + 1;
+        if (below < 32) hi = next;
+    }
+    return lo;
 }
 
 // FIRST: keys come from the caller's tensor; else from the pairs of the previous pass
@@ -210,7 +253,21 @@ fill_kernel(const uint32_t *__restrict__ sorted, uint32_t n, uint32_t nkeys, int
     const uint32_t p0 = (blockIdx.x * WARPS + (threadIdx.x >> 5)) * 32, p = p0 + (threadIdx.x & 31);
     if (p0 > n) return;
     const uint32_t key = p < n ? sorted[p] : nkeys;
-    write_starts(key, p0 == 0 ? -1 : (int64_t)sorted[p0 - 1], p0, group_start);
+    write_starts(key, p0 == 0 ? -1 : (int64_t)sorted[p0 - 1], p0, nkeys, group_start);
+}
+
+// segments of keys of which none but the last occurs, one warp each: the others are written by the positions around them
+__global__ void __launch_bounds__(THREADS)
+gap_kernel(const uint32_t *__restrict__ sorted, uint32_t n, uint32_t segments, int *__restrict__ group_start) {
+    for (uint32_t i = blockIdx.x * WARPS + (threadIdx.x >> 5); i < segments; i += gridDim.x * WARPS) {
+        const uint32_t from = i * SEGMENT, to = from + SEGMENT - 1, start = warp_lower_bound(sorted, n, from);
+        if (start == n || sorted[start] >= to) fill_run(group_start, from, to + 1, (int)start);
+    }
+}
+void fill_gaps(const uint32_t *sorted, size_t n, int nkeys, int *group_start, cudaStream_t st) {
+    if ((uint32_t)nkeys < FAR_KEYS) return;
+    const uint32_t segments = ((uint32_t)nkeys + 1) / SEGMENT, blocks = (segments + WARPS - 1) / WARPS;
+    gap_kernel<<<blocks < 1184 ? blocks : 1184, THREADS, 0, st>>>(sorted, (uint32_t)n, segments, group_start);
 }
 
 // the same by a search per key: many more keys than positions would leave wide gaps to few warps
@@ -359,9 +416,9 @@ cluster_kernel(const K *__restrict__ keys, uint32_t n, uint32_t nkeys, int passe
 #pragma unroll
     for (int i = 0; i < C_ITEMS; ++i) {
         const uint32_t p0 = w0 + i * 32;
-        if (i < items && p0 <= n) write_starts(p0 + lane < n ? here[i] : nkeys, p0 == 0 ? -1 : (int64_t)left[i], p0, group_start);
+        if (i < items && p0 <= n) write_starts(p0 + lane < n ? here[i] : nkeys, p0 == 0 ? -1 : (int64_t)left[i], p0, nkeys, group_start);
     }
-    if (w0 + (uint32_t)(32 * items) == n) write_starts(nkeys, sorted[n - 1], n, group_start);      // nobody's positions lie behind the end
+    if (w0 + (uint32_t)(32 * items) == n) write_starts(nkeys, sorted[n - 1], n, nkeys, group_start);      // nobody's positions lie behind the end
 }
 
 template <typename K>
@@ -394,10 +451,12 @@ int run_cluster(const K *keys, size_t n, int nkeys, int *order, int *group_start
     if (cudaLaunchKernelEx(&cfg, cluster_kernel<K>, keys, (uint32_t)n, (uint32_t)nkeys, passes, nbits, items, order, group_start, pairs, row,
                            (int)fill) != cudaSuccess)
         return qmlb::check_launch("qmlb_group_by_key");
+    const uint32_t *sorted = pairs + ((passes - 1) & 1) * row;
     if (passes > 1 && !fill) {
         const uint32_t sb = ((uint32_t)nkeys + THREADS) / THREADS;
-        start_kernel<<<sb < 1184 ? sb : 1184, THREADS, 0, st>>>(pairs + ((passes - 1) & 1) * row, (uint32_t)n, (uint32_t)nkeys, group_start);
+        start_kernel<<<sb < 1184 ? sb : 1184, THREADS, 0, st>>>(sorted, (uint32_t)n, (uint32_t)nkeys, group_start);
     }
+    if (fill) fill_gaps(sorted, n, nkeys, group_start, st);
     return qmlb::check_launch("qmlb_group_by_key");
 }
 
@@ -448,8 +507,10 @@ int run_sort(const K *keys, size_t n, int nkeys, int *order, int *group_start, u
         scatter<<<p.blocks, THREADS, scat_smem, st>>>(keys, ik, ip, un, uk, shift, p.nbits, counts, totals, ok, op, group_start);
         if (last && !first) {
             const uint32_t sb = (uk + THREADS) / THREADS;
-            if ((size_t)nkeys <= 16 * n) fill_kernel<<<un / (WARPS * 32) + 1, THREADS, 0, st>>>(ok, un, uk, group_start);
-            else start_kernel<<<sb < 1184 ? sb : 1184, THREADS, 0, st>>>(ok, un, uk, group_start);
+            if ((size_t)nkeys <= 16 * n) {
+                fill_kernel<<<un / (WARPS * 32) + 1, THREADS, 0, st>>>(ok, un, uk, group_start);
+                fill_gaps(ok, n, nkeys, group_start, st);
+            } else start_kernel<<<sb < 1184 ? sb : 1184, THREADS, 0, st>>>(ok, un, uk, group_start);
         }
     }
     return qmlb::check_launch("qmlb_group_by_key");
