@@ -16,21 +16,14 @@ int check_launch(const char *what);
 
 inline cudaStream_t as_stream(qmlb_stream_t s) { return reinterpret_cast<cudaStream_t>(s); }
 
-// Opt a kernel into more than 48 KB of dynamic shared memory when needed.
+// Opt a kernel into as much dynamic shared memory as it may have.  Always the same size, whatever this call wants: a smaller one
+// could come between the setting and the launch of another host thread.
+int opt_in_smem(const void *kernel, size_t bytes, const char *what);
+
+// The same when more than 48 KB of dynamic shared memory are wanted.
 template <typename K>
 inline int ensure_smem(K kernel, size_t bytes, const char *what) {
-    if (bytes > 227 * 1024) {
-        set_error("%s: needs %zu bytes of shared memory per block, above the 227 KB limit", what, bytes);
-        return QMLB_ERR_UNSUPPORTED;
-    }
-    if (bytes > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-        if (e != cudaSuccess) {
-            set_error("%s: cudaFuncSetAttribute(%zu): %s", what, bytes, cudaGetErrorString(e));
-            return QMLB_ERR_CUDA;
-        }
-    }
-    return QMLB_OK;
+    return bytes > 48 * 1024 ? opt_in_smem(reinterpret_cast<const void *>(kernel), bytes, what) : QMLB_OK;
 }
 
 }  // namespace qmlb
