@@ -12,10 +12,13 @@
 // by ballots or a match, and the warp's running count per digit stays in shared memory.  What bounds a pass is
 // latency and the scattered writes, not arithmetic: 8 + 8 bytes per key and pass.
 // With one pass the digit totals are the group sizes; with more, group_start is read off the sorted keys.
-// Up to CLUSTER_KEYS keys take one launch of one thread-block cluster: the same passes, with the digit totals read from the
-// neighbours' shared memory and cluster barriers between the steps.  (Separate launches took 20 us for one pass and 57 us for two
-// whatever the number of keys; most of it the launches and the few busy SMs.)
+// Up to CLUSTER_KEYS keys (PORTABLE_KEYS where the device runs no clusters of sixteen blocks) take one launch of one thread-block
+// cluster: the same passes, with the digit totals read from the neighbours' shared memory and cluster barriers between the steps.
+// (Separate launches took 20 us for one pass and 57 us for two whatever the number of keys; most of it the launches and the few
+// busy SMs.)
 #include <cooperative_groups.h>
+
+#include <atomic>
 
 #include "typed.cuh"
 
@@ -289,7 +292,7 @@ __global__ void empty_kernel(uint32_t nkeys, int *__restrict__ group_start) {
 
 // ---- one cluster ----------------------------------------------------------------------------------------------------
 constexpr int C_THREADS = 1024, C_WARPS = 32, C_ITEMS = 8, C_BITS = 9, C_MAX = 16;
-constexpr uint32_t CLUSTER_KEYS = C_MAX * C_THREADS * C_ITEMS;      // 131,072
+constexpr uint32_t CLUSTER_KEYS = C_MAX * C_THREADS * C_ITEMS, PORTABLE_KEYS = 8 * C_THREADS * C_ITEMS;      // 131,072 and 65,536
 
 // `items` keys per thread; pairs: scratch of two buffers of n keys and two of n positions
 template <typename K>
@@ -421,34 +424,76 @@ cluster_kernel(const K *__restrict__ keys, uint32_t n, uint32_t nkeys, int passe
     if (w0 + (uint32_t)(32 * items) == n) write_starts(nkeys, sorted[n - 1], n, nkeys, group_start);      // nobody's positions lie behind the end
 }
 
+// Two keys per thread, then more; sixteen blocks, where the device runs such clusters, only where ranking counts.
+struct ClusterPlan {
+    int passes, nbits, blocks, items;
+    size_t smem;
+};
+ClusterPlan plan_cluster(size_t n, int nkeys, bool wide) {
+    ClusterPlan p;
+    const int bits = bits_for((unsigned)nkeys), most = wide && (bits > C_BITS || n > PORTABLE_KEYS) ? C_MAX : 8;
+    p.passes = (bits + C_BITS - 1) / C_BITS;
+    p.nbits = (bits + p.passes - 1) / p.passes;
+    p.blocks = 1;
+    while (p.blocks < most && (size_t)p.blocks * C_THREADS * 2 < n) p.blocks <<= 1;
+    p.items = (int)((n + (size_t)p.blocks * C_THREADS - 1) / ((size_t)p.blocks * C_THREADS));
+    p.smem = ((size_t)16 << p.nbits) + ((size_t)C_WARPS * 2 << p.nbits) + (p.nbits > 5 ? (size_t)8 * C_THREADS * p.items : 0);
+    return p;
+}
+
+cudaLaunchConfig_t cluster_config(const ClusterPlan &p, cudaLaunchAttribute *at, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.blocks);
+    cfg.blockDim = dim3(C_THREADS);
+    cfg.dynamicSmemBytes = p.smem;
+    cfg.stream = st;
+    at->id = cudaLaunchAttributeClusterDimension;
+    at->val.clusterDim.x = (unsigned)p.blocks;
+    at->val.clusterDim.y = at->val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cfg;
+}
+
+// Whether the current device runs clusters of sixteen blocks, which is more than every device promises; asked once per device.
 template <typename K>
-int run_cluster(const K *keys, size_t n, int nkeys, int *order, int *group_start, unsigned char *scratch, cudaStream_t st) {
-    const int bits = bits_for((unsigned)nkeys), passes = (bits + C_BITS - 1) / C_BITS, nbits = (bits + passes - 1) / passes;
-    int blocks = 1;
-    // two keys per thread, then more; sixteen blocks (more than every device promises) only where ranking counts
-    const int most = passes > 1 || n > (size_t)8 * C_THREADS * C_ITEMS ? C_MAX : 8;
-    while (blocks < most && (size_t)blocks * C_THREADS * 2 < n) blocks <<= 1;
-    const int items = (int)((n + (size_t)blocks * C_THREADS - 1) / ((size_t)blocks * C_THREADS));
+bool wide_clusters() {
+#ifdef QMLB_TEST_NO_WIDE_CLUSTERS
+    return false;                                                // for a test of the way without
+#else
+    constexpr int DEVICES = 64;
+    static std::atomic<signed char> known[DEVICES];              // 0: not asked yet
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    if (dev < DEVICES)
+        if (const signed char k = known[dev].load(std::memory_order_relaxed)) return k > 0;
+    const ClusterPlan p = plan_cluster(CLUSTER_KEYS, (1 << C_BITS) - 1, true);       // the largest launch
+    cudaLaunchAttribute at;
+    const cudaLaunchConfig_t cfg = cluster_config(p, &at, nullptr);
+    int clusters = 0;
+    const bool yes = qmlb::ensure_smem(cluster_kernel<K>, p.smem, "qmlb_group_by_key") == QMLB_OK &&
+                     cudaFuncSetAttribute(cluster_kernel<K>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                     cudaOccupancyMaxActiveClusters(&clusters, cluster_kernel<K>, &cfg) == cudaSuccess && clusters > 0;
+    if (!yes) cudaGetLastError();                                // a refusal is an answer
+    if (dev < DEVICES) known[dev].store(yes ? 1 : -1, std::memory_order_relaxed);
+    return yes;
+#endif
+}
+
+template <typename K>
+int run_cluster(const ClusterPlan &p, const K *keys, size_t n, int nkeys, int *order, int *group_start, unsigned char *scratch, cudaStream_t st) {
+    const int passes = p.passes;
     // many more keys than positions: the gaps are wide, and a search per key on all SMs fills them sooner
     const bool fill = passes > 1 && (size_t)nkeys <= 16 * n;
     const uint32_t row = (uint32_t)(((n * 4 + 255) & ~(size_t)255) / 4);
     uint32_t *pairs = reinterpret_cast<uint32_t *>(scratch);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)blocks);
-    cfg.blockDim = dim3(C_THREADS);
-    cfg.dynamicSmemBytes = ((size_t)16 << nbits) + ((size_t)C_WARPS * 2 << nbits) + (nbits > 5 ? (size_t)8 * C_THREADS * items : 0);
-    if (blocks > 8 && cudaFuncSetAttribute(cluster_kernel<K>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+    cudaLaunchAttribute at;
+    const cudaLaunchConfig_t cfg = cluster_config(p, &at, st);
+    if (p.blocks > 8 && cudaFuncSetAttribute(cluster_kernel<K>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
         return qmlb::check_launch("qmlb_group_by_key(cluster size)");
     // (1 KB more: the kernel's own variables count towards the 48 KB that need no opting in)
-    if (int rc = qmlb::ensure_smem(cluster_kernel<K>, cfg.dynamicSmemBytes + 1024, "qmlb_group_by_key")) return rc;
-    cfg.stream = st;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = (unsigned)blocks;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, cluster_kernel<K>, keys, (uint32_t)n, (uint32_t)nkeys, passes, nbits, items, order, group_start, pairs, row,
+    if (int rc = qmlb::ensure_smem(cluster_kernel<K>, p.smem + 1024, "qmlb_group_by_key")) return rc;
+    if (cudaLaunchKernelEx(&cfg, cluster_kernel<K>, keys, (uint32_t)n, (uint32_t)nkeys, passes, p.nbits, p.items, order, group_start, pairs, row,
                            (int)fill) != cudaSuccess)
         return qmlb::check_launch("qmlb_group_by_key");
     const uint32_t *sorted = pairs + ((passes - 1) & 1) * row;
@@ -519,7 +564,13 @@ int run_sort(const K *keys, size_t n, int nkeys, int *order, int *group_start, u
 template <typename K>
 int run(const void *keys, size_t n, int nkeys, int *order, int *group_start, unsigned char *scratch, cudaStream_t st) {
     const K *k = static_cast<const K *>(keys);
-    if (n <= CLUSTER_KEYS) return run_cluster(k, n, nkeys, order, group_start, scratch, st);
+    if (n <= CLUSTER_KEYS) {
+        // a wide cluster has to be asked for only where one would be used
+        ClusterPlan p = plan_cluster(n, nkeys, true);
+        const bool wide = p.blocks <= 8 || wide_clusters<K>();
+        if (!wide) p = plan_cluster(n, nkeys, false);
+        if (wide || n <= PORTABLE_KEYS) return run_cluster(p, k, n, nkeys, order, group_start, scratch, st);
+    }
     return items_for(n) == FEW ? run_sort<K, FEW>(k, n, nkeys, order, group_start, scratch, st)
                                : run_sort<K, MANY>(k, n, nkeys, order, group_start, scratch, st);
 }
@@ -528,8 +579,10 @@ int run(const void *keys, size_t n, int nkeys, int *order, int *group_start, uns
 
 extern "C" size_t qmlb_group_by_key_scratch_bytes(size_t n, int nkeys) {
     if (n == 0 || n >= (size_t)1 << 31 || nkeys <= 0 || nkeys == INT32_MAX) return 0;
-    if (n <= CLUSTER_KEYS) return bits_for((unsigned)nkeys) <= C_BITS ? 0 : 4 * ((n * 4 + 255) & ~(size_t)255);
-    return make_plan(n, nkeys).bytes;
+    const size_t cluster = bits_for((unsigned)nkeys) <= C_BITS ? 0 : 4 * ((n * 4 + 255) & ~(size_t)255);
+    if (n <= PORTABLE_KEYS) return cluster;
+    const size_t launches = make_plan(n, nkeys).bytes;
+    return n <= CLUSTER_KEYS && cluster > launches ? cluster : launches;
 }
 
 extern "C" int qmlb_group_by_key(const void *keys, int key_bits, size_t n, int nkeys, int *order, int *group_start, void *scratch,
