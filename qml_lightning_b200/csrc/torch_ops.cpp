@@ -601,8 +601,8 @@ Tensor bounds(const Tensor &group_start, const Tensor &like, int64_t groups) {
     on_device(group_start, like.device(), "group_start");
     TORCH_CHECK(group_start.dim() == 1 && (groups < 0 ? group_start.numel() >= 2 : group_start.numel() == groups + 1),
                 "group_start must have one entry per group and one more");
-    index_bits(group_start, "group_start");
-    return i32c(group_start);
+    // what 32 bits do not hold lies outside the rows: clamped like every other such bound, not cut off
+    return index_bits(group_start, "group_start") == 64 ? group_start.clamp(0, INT32_MAX).to(torch::kInt32).contiguous() : group_start.contiguous();
 }
 
 Tensor grouped_matmul_call(const Tensor &x, const Tensor &W, const Tensor &group_start, bool transpose) {
