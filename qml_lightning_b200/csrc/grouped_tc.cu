@@ -426,8 +426,8 @@ int run(const void *x, const void *W, const int *start, size_t n, int G, int K, 
     const uint64_t row_bytes = (uint64_t)p.K * 2;
     p.period = 1;
     if (shifted) {
-        while ((row_bytes * p.period) & 15) p.period <<= 1;
-        if (p.period == 1) p.period = 2;                       // an offset view of aligned rows: a map's rows must not overlap
+        // a map's rows must not overlap: they begin up to seven elements early (offset views, and depths of 2 and 4)
+        while (((row_bytes * p.period) & 15) || p.K + 7 > p.K * p.period) p.period <<= 1;
     }
     for (int q = 0; q < 8; ++q) {
         const uintptr_t at = (uintptr_t)x + q * row_bytes;
