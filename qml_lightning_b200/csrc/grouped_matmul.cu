@@ -164,7 +164,7 @@ bool few_rows_grad(size_t n, int G, int K, int N, int dtype) {
 extern "C" size_t qmlb_grouped_matmul_workspace_bytes(size_t n, int ngroups, int K, int N, int dtype, int transpose) {
     if (n == 0 || ngroups <= 0 || K <= 0 || N <= 0) return 0;
     if (dtype == QMLB_F32) return few_rows(n, ngroups, K, N) ? 0 : qmlb::grouped_pair_workspace(n, ngroups, K, N, transpose);
-    return qmlb::grouped_tc_workspace(ngroups, K, N, transpose);
+    return qmlb::grouped_tc_workspace(n, ngroups, K, N, transpose);
 }
 
 extern "C" int qmlb_grouped_matmul(const void *x, const void *W, const int *group_start, int dtype, size_t n, int ngroups, int K, int N,

@@ -13,7 +13,7 @@
 // Rows whose address is no multiple of 16 bytes (odd widths, offset views) cannot be fetched by TMA one after the other.  Forward:
 // every PERIOD-th row (2, 4 or 8) has the same offset from a 16-byte boundary, so a tile takes 128 rows of one offset, by a tensor
 // map that starts at the boundary; its sums begin `shift` elements early, against zero rows of the matrix (coordinates in front of
-// its first row), and the issuing warp overwrites what the rows bring there.  (780 deep, 330,001 rows: 231 us with cp.async of
+// its first row), and the issuing warp overwrites what the rows bring there; small groups are copied instead.  (780 deep, 330,001 rows: 231 us with cp.async of
 // 8 bytes, 177 us so; 781 deep: 664 us with 2-byte loads, 181 us so.)  Transposed, the matrix's lines would have to move along, so
 // warps 12-19 bring the rows with cp.async of 8 or 4 bytes, or 2-byte loads, into the same swizzled stages.
 // Sums longer than 16,384 values are cut, because the tensor core truncates when it adds (1,024 additions of one sign are off by up to
@@ -330,20 +330,43 @@ grouped_kernel(const __grid_constant__ RowMaps maps, const __grid_constant__ CUt
     }
 }
 
-// W [G][K][N] with rows that no 16-byte access can follow -> the same with rows padded to a multiple of 8 elements
+// Rows of `cols` values that no 16-byte access can follow -> the same with rows padded to a multiple of 8 values, 8 per thread
 template <typename T>
 __global__ void __launch_bounds__(256)
-pad_kernel(const T *__restrict__ W, size_t rows, int N, int Np, T *__restrict__ to) {
-    const size_t total = rows * (size_t)Np;
+pad_kernel(const T *__restrict__ in, size_t rows, int cols, int padded, T *__restrict__ to) {
+    const unsigned words = (unsigned)padded / 8;
+    const size_t total = rows * words;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
-        const size_t r = i / (unsigned)Np;
-        const int c = (int)(i - r * (unsigned)Np);
-        to[i] = c < N ? W[r * N + c] : qmlb::from_f32<T>(0.f);
+        const size_t r = i / words;
+        const int c = (int)(i - r * words) * 8;
+        const T *src = in + r * cols;
+        qmlb::Pack<T, 8> k;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) k.item[u] = src[min(c + u, cols - 1)];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (c + u >= cols) k.item[u] = qmlb::from_f32<T>(0.f);
+        reinterpret_cast<uint4 *>(to)[i] = k.word;
     }
+}
+template <typename T>
+void pad_rows(const void *in, size_t rows, int cols, void *to, cudaStream_t st) {
+    const int padded = (cols + 7) & ~7;
+    const size_t b = (rows * (padded / 8) + 255) / 256;
+    pad_kernel<T><<<(unsigned)(b < 148 * 16 ? b : 148 * 16), 256, 0, st>>>(static_cast<const T *>(in), rows, cols, padded, static_cast<T *>(to));
+}
+
+// Every offset has tiles of its own in every group, so rows in groups of few rows per offset are copied to the 16-byte boundaries first.
+// 64 groups of 781 deep bf16 rows, 256 columns (eight offsets): 20 rows each 99 -> 32 us, 256 63 -> 34, 500 45 -> 49, 1,000 47 -> 83; 2,048
+// columns, 16 groups of 500: 72 -> 48; 782 deep (four): 256 rows 40 -> 34, 500 28 -> 48; 780 deep (two): 100 rows 30 -> 26, 256 24 -> 34.
+bool copies_rows(size_t n, int G, int depth, int transpose) {
+    const int offsets = (depth & 1) ? 8 : (depth & 2) ? 4 : (depth & 4) ? 2 : 1;
+    return !transpose && offsets > 1 && n / G <= (size_t)64 * offsets;
 }
 
 // a sum may begin up to seven values early
 bool several_pieces(int depth) { return (depth + 7 + BK - 1) / BK > PIECE; }
+size_t sums_bytes(int depth) { return several_pieces(depth) ? (size_t)MAX_BLOCKS * SUMS * 4 : 0; }
 size_t padded_bytes(int G, int K, int N) { return ((size_t)G * K * ((N + 7) & ~7) * 2 + 255) & ~(size_t)255; }
 
 bool needs_pad(const void *W, int N) { return ((uintptr_t)W & 15) != 0 || (N & 7) != 0; }
@@ -387,7 +410,14 @@ int run(const void *x, const void *W, const int *start, size_t n, int G, int K, 
     p.K = transpose ? N : K;
     p.out = transpose ? K : N;
     p.nchunks = (p.K + BK - 1) / BK;
-    p.in_access = qmlb::access_bytes((size_t)p.K * 2, 2, x);
+    uint64_t row_bytes = (uint64_t)p.K * 2;
+    if (copies_rows(n, G, p.K, transpose)) {
+        void *copy = static_cast<unsigned char *>(workspace) + padded_bytes(G, K, N) + sums_bytes(p.K);
+        pad_rows<T>(x, n, p.K, copy, st);
+        x = copy;
+        row_bytes = (uint64_t)((p.K + 7) & ~7) * 2;
+    }
+    p.in_access = qmlb::access_bytes(row_bytes, 2, x);
     p.out_access = qmlb::access_bytes((size_t)p.out * 2, 2, out);
     // Columns per tile: as many as one accumulator holds, so that the rows are read once, in equal parts; fewer when the row
     // tiles alone do not give every SM a tile.
@@ -412,8 +442,7 @@ int run(const void *x, const void *W, const int *start, size_t n, int G, int K, 
     int Np = N;
     if (needs_pad(W, N)) {
         Np = (N + 7) & ~7;
-        const size_t total = (size_t)G * K * Np, b = (total + 1023) / 1024;
-        pad_kernel<T><<<(unsigned)(b < 2368 ? b : 2368), 256, 0, st>>>(static_cast<const T *>(W), (size_t)G * K, N, Np, static_cast<T *>(workspace));
+        pad_rows<T>(W, (size_t)G * K, N, workspace, st);
         Wp = workspace;
     }
     RowMaps mi;
@@ -423,7 +452,6 @@ int run(const void *x, const void *W, const int *start, size_t n, int G, int K, 
                                     "qmlb_grouped_matmul"))
         return rc;
     p.sums = reinterpret_cast<float *>(static_cast<unsigned char *>(workspace) + padded_bytes(G, K, N));
-    const uint64_t row_bytes = (uint64_t)p.K * 2;
     p.period = 1;
     if (shifted) {
         // a map's rows must not overlap: they begin up to seven elements early (offset views, and depths of 2 and 4)
@@ -459,8 +487,9 @@ int run(const void *x, const void *W, const int *start, size_t n, int G, int K, 
 
 namespace qmlb {
 
-size_t grouped_tc_workspace(int G, int K, int N, int transpose) {
-    return padded_bytes(G, K, N) + (several_pieces(transpose ? N : K) ? (size_t)MAX_BLOCKS * SUMS * 4 : 0) + 256;
+size_t grouped_tc_workspace(size_t n, int G, int K, int N, int transpose) {
+    const size_t copy = copies_rows(n, G, K, transpose) ? n * ((K + 7) & ~7) * 2 : 0;
+    return padded_bytes(G, K, N) + sums_bytes(transpose ? N : K) + copy + 256;
 }
 
 int grouped_tc(const void *x, const void *W, const int *start, int dtype, size_t n, int G, int K, int N, int transpose, void *out,

@@ -6,7 +6,7 @@
 
 namespace qmlb {
 
-size_t grouped_tc_workspace(int G, int K, int N, int transpose);
+size_t grouped_tc_workspace(size_t n, int G, int K, int N, int transpose);
 int grouped_tc(const void *x, const void *W, const int *start, int dtype, size_t n, int G, int K, int N, int transpose, void *out,
                void *workspace, cudaStream_t st);
 int grouped_tc_timeouts();
