@@ -33,3 +33,28 @@ def test_long_sums_of_one_sign(depth, out, n, dtype):
         assert torch.equal(y, ops().grouped_matmul(x, W, start, transpose))
     from qml_lightning_b200 import cabi
     assert cabi.tc_timeouts() == 0
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('depth,sizes,offset', [(16640, [20000, 20100], 0), (20001, [1500, 1250], 0), (17000, [300, 900], 3)])
+def test_long_sums_of_large_groups_and_odd_rows(depth, sizes, offset, dtype):
+    """The same for pairs of blocks (many deep rows), and for rows off the 16-byte boundaries; the ends of every group are compared."""
+    g = torch.Generator(device=DEV).manual_seed(depth)
+    n, out = sum(sizes) + 3, 256
+    start = R.start_of(sizes, DEV)
+    flat = torch.empty(n * depth + 8, dtype=dtype, device=DEV)
+    x = flat[offset:offset + n * depth].view(n, depth)
+    for a in range(0, n, 4096):
+        x[a:a + 4096] = torch.rand(min(4096, n - a), depth, generator=g, device=DEV).to(dtype)
+    bounds = R.groups_of(start, n)
+    rows = torch.cat([torch.cat((torch.arange(a, a + 150), torch.arange(b - 150, b))) for a, b in bounds]).to(DEV)
+    few = R.start_of([300] * len(sizes), DEV)
+    for transpose in (False, True):
+        W = (torch.rand((len(sizes), out, depth) if transpose else (len(sizes), depth, out), generator=g, device=DEV) / depth).mul_(512).to(dtype)
+        y = ops().grouped_matmul(x, W, start, transpose)
+        exact, mag = R.product(x[rows], W, few, transpose)
+        bound = exact.abs() * (R.half_step(dtype) + 2.0 ** -13 + (depth // 16384 + 2) * R.U) * 1.001
+        R.assert_within(y[rows], exact, bound, f'{transpose}')
+        assert (y[-3:] == 0).all()
+    from qml_lightning_b200 import cabi
+    assert cabi.tc_timeouts() == 0
