@@ -126,3 +126,19 @@ def test_values_near_the_ends_of_the_range(n, a, b):
                                                ('dW of exchanged operands', ops().grouped_matmul_wgrad(dy, x, start), R.wgrad(dy, x, start), 0)):
         assert bool((exact.abs() < 3e38).all())
         R.assert_within(got, exact, R.sum_bound(exact, mag, terms[0] if terms else m, torch.float32) + tiny * R.U, name)
+
+
+def test_infinities_in_many_tiles():
+    """More tiles per block than it keeps apart: infinities in the first, in the last, and in few between."""
+    g = gen(6)
+    n, K, N = 1500007, 6, 10
+    x, W = torch.randn(n, K, generator=g, device=DEV), torch.randn(2, K, N, generator=g, device=DEV)
+    start = R.start_of([n // 2, n - n // 2 - 4], DEV)
+    for r, v in ((0, float('inf')), (700000, float('nan')), (1300000, -float('inf')), (1400001, 3e38), (n - 5, float('inf'))):
+        x[r, r % K] = v
+    y = ops().grouped_matmul(x, W, start)
+    exact, _ = R.product(x, W, start)
+    same_kind(y, exact)
+    ok = exact.float().isfinite()                                      # (3e38 times a weight may leave the range of float32)
+    size = x.double().abs().nan_to_num(0, 0).sum(1, keepdim=True) * W.abs().max()
+    assert bool(((y.double() - exact).abs()[ok] <= 64 * R.U * size.expand_as(exact)[ok]).all())
