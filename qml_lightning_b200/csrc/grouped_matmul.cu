@@ -148,12 +148,14 @@ int run_wgrad(const void *x, const void *dy, const int *start, int G, int n, int
     return qmlb::check_launch("qmlb_grouped_matmul_wgrad");
 }
 
-// Few rows or many.  Measured (float32, B200): the FFMA kernel takes 8 us and 2 n K N operations at 10 TFLOP/s, the tensor-core
-// path 24 us and 12 bytes per matrix element for the images; equal at n = 9 G + 8e7 / (K N).  (3 groups, 336 x 256: 8 against
-// 26 us at n = 64, 29 against 28 us at n = 1,024; 32 groups, 1,024 x 1,024: 74 against 107 us at n = 256, 127 against 109 us at
-// n = 512.)  Beyond 2,048 rows a block would walk too many of them.
+// Few rows or many.  The FFMA kernel takes a few us and 2 n K N operations at 10 TFLOP/s, the tensor-core path 24 us and 16 bytes per
+// matrix element for the images; about equal at n = 9 G + 8e7 / (K N).  (Whole calls, of which the host takes 18 us.  3 groups, 336 x
+// 256: 23 against 30 us at n = 512, 28 against 30 at 1,024, 50 against 31 at 2,000, transposed 23 against 23 to 30, 36 against 24 to 30,
+// 63 against 24; 32 groups, 1,024 x 1,024: 63 against 114 us at n = 256, 89 against 115 at 512, 154 against 117 at 1,024, transposed 81
+// against 111, 114 against 112, 198 against 112; 64 groups, 256 x 512: 32 against 37 at 512, 45 against 38 at 1,024, transposed 30
+// against 46, 35 against 46.)  Beyond 2,048 rows a block would walk too many of them.
 bool few_rows(size_t n, int G, int K, int N) { return n <= 2048 && (double)n <= 9.0 * G + 8e7 / ((double)K * N); }
-// Gradient of the matrices.  float32: 16 against 18 us at n = 256, 27 against 23 us at n = 512 (3 groups, 336 x 256).  16-bit: 6 to
+// Gradient of the matrices.  float32: 19 against 19 to 24 us at n = 256, 44 against 24 to 30 us at n = 1,024 (3 groups, 336 x 256).  16-bit: 6 to
 // 10 against 16 us (which are mostly launches) while the result is small; 57 against 34 us for 32 groups, 1,024 x 1,024.
 bool few_rows_grad(size_t n, int G, int K, int N, int dtype) {
     return dtype == QMLB_F32 ? n < 256 : n <= 128 && (double)G * K * N <= 4e6;

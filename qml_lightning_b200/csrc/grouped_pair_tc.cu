@@ -7,8 +7,8 @@
 // parts of values below 2^-110 would leave the range, so all values are multiplied by 2^16 on their way in, and sums by 2^-32 on
 // their way out: every normal number enters exactly, and a sum may reach 2^96 before it overflows (see below).  Sums: the tensor core
 // truncates when it adds, so an accumulator only ever covers one stretch of 64 values (the small products first, then a a'), and
-// warps of CUDA cores add the stretches in registers in 32 bits, rounded.  Against 64 bits the results are off by about 2e-7 of
-// their norm, like a float32 product.
+// warps of CUDA cores add the stretches in registers in 32 bits, rounded.  Against 64 bits the results are off by about 1e-7 of
+// their norm, a float32 product by 3e-7.
 //
 // Work split.  One persistent block per SM takes tiles of 128 x NT results:
 //   warp 0          bulk copies of the matrix operand's images (products of rows; a packing kernel makes the images), one of the
@@ -19,7 +19,11 @@
 //   folding warps   (eight) add the finished accumulators to their registers, and store the tile
 // Products of rows: NT <= 256, 4 loading warps, 128 sums per folding thread.  Gradient of the matrices: both operands are loaded
 // by the loading warps (the depth runs over the rows of the group, the operands' lines run across it), and NT <= 128 leaves
-// registers for eight of them, two per scheduler.
+// registers for eight of them, two per scheduler, and room for two stages (six parts of 128 are 96 KB; of 128 and 256 144 KB).
+// 210,000 x (336, 256): products of rows 232 us, transposed 256 us (the six products alone take 132 us at the rate of a library
+// product), gradient 386 us.  60,000 x 1,024 x 1,024 of 32 groups: 815, 820 and 1,092 us (461 us).  Of 5,600 cycles per stretch the
+// issuing warp spends 2,500 issuing, 1,300 waiting for a part of the matrix, 900 for an accumulator while a tile is stored (11,000
+// cycles per tile, of which two stretches hide half) and 850 for the rows; with smaller copies of the parts nothing changes.
 // Registers are moved between the warps by setmaxnreg.
 //
 // Results that are not finite.  An infinity times the zero low part of another number is NaN, and scaled sums leave the range before

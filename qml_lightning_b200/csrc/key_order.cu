@@ -2,8 +2,9 @@
 // order, and group_start[v] = number of valid keys below v.  Keys outside [0, nkeys) (the -1 of a padded slot) count as
 // the key nkeys: they come behind all groups, in their original order.
 //
-// Least-significant-digit radix sort with digits of at most RADIX_BITS bits, so up to 1,023 keys (every element or
-// species numbering) take ONE pass and 1,048,575 take two.  A pass over blocks of 1,024 or 2,048 keys:
+// Least-significant-digit radix sort with digits of at most RADIX_BITS bits in separate launches, C_BITS in a cluster, so up to 1,023 keys
+// (in a cluster 511; every element or species numbering) take ONE pass and 1,048,575 (262,143) take two.  A pass over blocks of 1,024
+// or 2,048 keys:
 //   1. histogram : counts[digit][block]
 //   2. scan      : one block per digit turns its row into an exclusive prefix over the blocks and writes the digit's total
 //   3. scatter   : every block ranks its keys again (the same order, so the result never depends on scheduling) and
@@ -26,7 +27,7 @@ namespace {
 
 constexpr int RADIX_BITS = 10;                 // widest digit
 constexpr int THREADS = 256, WARPS = THREADS / 32;
-// keys per thread: few while the blocks do not fill the device (3.3 million keys of 5: 32 us with 8, 36 with 16, 42 with 32)
+// keys per thread: few while the blocks do not fill the device (3.3 million keys of 5: 27.5 us with 8, 31.6 with 16, 37 with 32)
 constexpr int FEW = 4, MANY = 8;
 inline int items_for(size_t n) { return n < (size_t)148 * 8 * THREADS * FEW ? FEW : MANY; }
 
