@@ -411,8 +411,9 @@ int qmlb_embedding_grad(const void *dout, int dtype, const void *index, int inde
  *   transpose = 1: out [n, K], out[r] = x[r] . W[g]^T     x [n, N]   (gradient of the rows)
  * Rows in front of the first group or behind the last become zero rows.  32-bit sums, one rounding to `dtype`.  16-bit products are
  * added by the tensor core, which truncates: at most 16,384 of them in one sum, the sums of a longer depth are added in 32 bits.
- * float32: every product by itself is as exact as in 32 bits, whatever stands beside it; infinities, NaN and sums beyond the range
- * come out as a product in 32 bits gives them, about a hundred times slower.
+ * float32: every product by itself is as exact as in 32 bits, whatever stands beside it (numbers below 1e-36 enter with an error of at
+ * most 2^-144).  Infinities, NaN, sums beyond the range, and what involves values above 1e35 or sums above 1e32, come out as a product
+ * in 32 bits gives them, about a hundred times slower.
  * ngroups <= 1024.  workspace: qmlb_grouped_matmul_workspace_bytes bytes of device memory, 256-byte aligned. */
 size_t qmlb_grouped_matmul_workspace_bytes(size_t n, int ngroups, int K, int N, int dtype, int transpose);
 int qmlb_grouped_matmul(const void *x, const void *W, const int *group_start, int dtype, size_t n, int ngroups, int K, int N,

@@ -4,8 +4,9 @@
 // nearest, 8 + 8 + 8 bits, |b| <= 2^-9 |x|, |c| <= 2^-18 |x|.  A product is a a' + a b' + b a' + b b' + a c' + c a'; the other three are
 // less than 2^-25 of it.  bf16 has the exponents of float32, so this holds for every value by itself, whatever stands beside it
 // (two fp16 parts on a common scale would take three products, but lose the small values of a stretch that holds large ones).  The
-// parts of values below 2^-110 would leave the range, so all values are multiplied by 2^16 on their way in, and sums by 2^-32 on
-// their way out: every normal number enters exactly, and a sum may reach 2^96 before it overflows (see below).  Sums: the tensor core
+// parts of values below 2^-110 would leave the range, so all values are multiplied by 2^10 on their way in, and sums by 2^-20 on
+// their way out: numbers above 2^-120 enter exactly, smaller ones are off by at most 2^-144, and values may reach 2^117 and sums 2^108
+// before they overflow (see below; room for masks of 1e30).  Sums: the tensor core
 // truncates when it adds, so an accumulator only ever covers one stretch of 64 values (the small products first, then a a'), and
 // warps of CUDA cores add the stretches in registers in 32 bits, rounded.  Against 64 bits the results are off by about 1e-7 of
 // their norm, a float32 product by 3e-7.
@@ -42,7 +43,7 @@ using namespace qmlb::tc;
 
 constexpr int BM = 128;
 constexpr uint32_t A_IMAGE = BM * BK * 2;         // one part of the 128-wide operand
-constexpr float SCALE = 65536.f, UNSCALE = 1.f / (SCALE * SCALE);
+constexpr float SCALE = 1024.f, UNSCALE = 1.f / (SCALE * SCALE);
 constexpr int TMA_WARP = 0, MMA_WARP = 1, LOAD_WARP = 4;
 constexpr int MAXST = 4, MAXSLOT = 6;
 template <bool GRAD>

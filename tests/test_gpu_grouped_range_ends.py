@@ -142,3 +142,27 @@ def test_infinities_in_many_tiles():
     ok = exact.float().isfinite()                                      # (3e38 times a weight may leave the range of float32)
     size = x.double().abs().nan_to_num(0, 0).sum(1, keepdim=True) * W.abs().max()
     assert bool(((y.double() - exact).abs()[ok] <= 64 * R.U * size.expand_as(exact)[ok]).all())
+
+
+def test_large_finite_values_cost_little():
+    """Masks of 1e30 among ordinary rows, whose products are finite, take no more time than other rows."""
+    n, K, N = 100000, 128, 64
+    start = R.start_of([n // 2, n // 2], DEV)
+    g = gen(7)
+    x, W = torch.randn(n, K, generator=g, device=DEV), torch.randn(2, K, N, generator=g, device=DEV)
+
+    def microseconds(x):
+        times = []
+        for _ in range(9):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            y = ops().grouped_matmul(x, W, start)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b) * 1e3)
+        assert y.isfinite().all()
+        return sorted(times[2:])[3]
+
+    masked = x.clone()
+    masked[::2] = -1e30
+    assert microseconds(masked) < 2.5 * microseconds(x)
